@@ -95,7 +95,9 @@ EXPORTED_SYMBOLS = (
     "bsg_comm_last_error", "bsg_comm_unique_id", "bsg_comm_create", "bsg_comm_destroy",
     "bsg_comm_all_gather", "bsg_comm_wait", "bsg_comm_get_info", "bsg_step_gather",
     "bsg_comm_all_reduce", "bsg_set_params", "bsg_trajectory_bytes", "bsg_set_trajectory",
-    "bsg_trajectory_info",
+    "bsg_trajectory_info", "bsg_delta_forward", "bsg_delta_backward", "bsg_delta_step",
+    "bsg_attention_forward", "bsg_attention_backward", "bsg_attention_step_bytes",
+    "bsg_attention_step",
 )
 TRAJ_SYNC = 1                # include/bsg.h BSG_TRAJ_SYNC
 # include/bsg.h BSG_MP_*: MergeEnv-v0's module constants (merge_env.py:13-46), in this order,
@@ -122,6 +124,46 @@ class BsgSacActor(C.Structure):
     _fields_ = [("obs_dim", C.c_int32), ("act_dim", C.c_int32), ("hidden", C.c_int32),
                 ("reserved", C.c_int32)] + [(n, C.c_void_p) for n in (
                     "w0", "b0", "w1", "b1", "w_mu", "b_mu", "w_ls", "b_ls")]
+
+F32, BF16 = 0, 1             # include/bsg.h BSG_F32, BSG_BF16
+DELTA_CHUNK = 64             # BSG_DELTA_CHUNK
+
+
+class BsgRows(C.Structure):
+    """include/bsg.h bsg_rows: a strided [env][step][head][dim] view."""
+    _fields_ = [("p", C.c_void_p), ("env", C.c_int64), ("step", C.c_int64), ("head", C.c_int64)]
+
+
+class BsgDelta(C.Structure):
+    """include/bsg.h bsg_delta."""
+    _fields_ = [(n, C.c_int32) for n in ("num_envs", "steps", "heads_k", "heads_v", "dim_k", "dim_v",
+                                         "dtype", "gate_dtype")] + \
+        [("scale", C.c_float), ("reserved", C.c_int32)] + \
+        [(n, BsgRows) for n in ("q", "k", "v", "g", "beta", "out")] + \
+        [("first", C.c_void_p), ("first_env", C.c_int64), ("first_step", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("lengths", "state", "final_state", "kept_states", "kept_w")] + \
+        [(n, BsgRows) for n in ("dout", "dq", "dk", "dv", "dg", "dbeta")] + \
+        [(n, C.c_void_p) for n in ("dfinal", "dstate", "work_states", "work_w")]
+
+
+class BsgAttention(C.Structure):
+    """include/bsg.h bsg_attention."""
+    _fields_ = [(n, C.c_int32) for n in ("num_envs", "steps", "heads_q", "heads_k", "dim", "dtype", "window")] + \
+        [("scale", C.c_float), ("softcap", C.c_float), ("reserved", C.c_int32)] + \
+        [(n, BsgRows) for n in ("q", "k", "v", "out")] + \
+        [("slopes", C.c_void_p), ("first", C.c_void_p), ("first_env", C.c_int64), ("first_step", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("lengths", "begins", "lse")] + \
+        [(n, BsgRows) for n in ("dout", "dq", "dk", "dv")] + [("delta", C.c_void_p)]
+
+
+class BsgAttentionAct(C.Structure):
+    """include/bsg.h bsg_attention_act."""
+    _fields_ = [(n, C.c_int32) for n in ("num_envs", "slots", "heads_q", "heads_k", "dim", "dtype")] + \
+        [("scale", C.c_float), ("softcap", C.c_float)] + \
+        [(n, BsgRows) for n in ("q", "k", "v", "out")] + \
+        [("slopes", C.c_void_p), ("first", C.c_void_p), ("first_env", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("steps", "k_cache", "v_cache", "work")] + [("work_bytes", C.c_int64)]
+
 
 _lib = None
 
@@ -211,6 +253,13 @@ def load_library(path: str | None = None):
     lib.bsg_step_gather.restype = C.c_int32
     lib.bsg_step_gather.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                     C.c_void_p, C.c_int32, C.c_void_p]
+    for fn, args in (("bsg_delta_forward", BsgDelta), ("bsg_delta_backward", BsgDelta),
+                     ("bsg_delta_step", BsgDelta), ("bsg_attention_forward", BsgAttention),
+                     ("bsg_attention_backward", BsgAttention), ("bsg_attention_step", BsgAttentionAct)):
+        getattr(lib, fn).restype = C.c_int32
+        getattr(lib, fn).argtypes = [C.POINTER(args), C.c_void_p]
+    lib.bsg_attention_step_bytes.restype = C.c_int64
+    lib.bsg_attention_step_bytes.argtypes = [C.POINTER(BsgAttentionAct)]
     if lib.bsg_abi_version() != ABI_VERSION:
         raise BsgError(f"libbsg ABI {lib.bsg_abi_version()} != expected {ABI_VERSION}")
     if path is None:

@@ -1,0 +1,406 @@
+"""Operators of a policy with memory, as fused HIP kernels (``bsg_delta_*`` and
+``bsg_attention_*``, include/bsg.h; csrc/bsg_delta.hip, csrc/bsg_attention.hip): the sequence
+layers a policy needs where one observation does not tell the state (the wind and uncertainty
+wrappers, bluesky_gym/wrappers).  The reference's actors are feed-forward; these stand beside
+``policy.SACPolicy``.
+
+Two layers, each in two forms that compute the same function:
+
+===========================  ======================================  ==========================
+layer                        learns from rollouts (with gradients)   acts for one RL step
+===========================  ======================================  ==========================
+gated delta rule             :func:`gated_delta_rule`                :func:`gated_delta_step`
+attention over the episode   :func:`episode_attention`               :func:`episode_attention_step`
+===========================  ======================================  ==========================
+
+Rollout tensors are ``[E, T, heads, dim]``: ``E`` envs, ``T`` steps.  Any strides serve; rollouts
+collected step by step as ``[T, E, ...]`` are passed as ``x.transpose(0, 1)`` and read in place
+(rows that are not contiguous, or not 16-byte aligned, are copied first).  fp32 or bf16, head
+dims 32, 64 or 128, everything on one HIP device; sums, softmax statistics and states are fp32.
+
+``first[e, t]`` (bool or uint8) says that step ``t`` is the first of an episode: nothing from
+before it is seen.  ``lengths[e]`` (int32, in ``[0, T]``) ends the rollout of env ``e`` early: the
+steps behind it are padding, never read, and their outputs and gradients are zero.  A non-finite
+value may reach every output of its env's rollout, but no other env's.
+
+Work is enqueued on the current stream of the tensors' device; all calls can be captured into a
+HIP graph.  ``first`` and ``lengths`` are read again by the backward pass.  No CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as nat
+
+HEAD_DIMS = (32, 64, 128)
+_DTYPES = {torch.float32: nat.F32, torch.bfloat16: nat.BF16}
+
+__all__ = ["gated_delta_rule", "gated_delta_step", "episode_attention", "episode_attention_step"]
+
+
+# ---- checks and views -----------------------------------------------------------------------
+
+def _tensors(who, ref, **named):
+    """Every tensor on one HIP device."""
+    dev = ref.device
+    if dev.type != "cuda":
+        raise nat.BsgError(f"{who} runs on a HIP device (no CPU fallback)")
+    for n, x in named.items():
+        if x is not None and x.device != dev:
+            raise ValueError(f"{who}: {n} is on {x.device}, q is on {dev}")
+
+
+def _shape(who, name, x, *shape, dtype=None):
+    if tuple(x.shape) != shape:
+        raise ValueError(f"{who}: {name} has shape {tuple(x.shape)}, expected {shape}")
+    if dtype is not None and x.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+        raise ValueError(f"{who}: {name} has dtype {x.dtype}, expected {dtype}")
+
+
+def _heads(who, q, k, v, dims, rank):
+    """Type and shape of q, k, v; returns the dtype code."""
+    if q.dim() != rank or k.dim() != rank or v.dim() != rank:
+        raise ValueError(f"{who}: q, k and v must have {rank} axes")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{who}: q, k and v must share one dtype, float32 or bfloat16 "
+                         f"(got {q.dtype}, {k.dtype}, {v.dtype})")
+    for n, d in dims.items():
+        if d not in HEAD_DIMS:
+            raise ValueError(f"{who}: {n} must be 32, 64 or 128 (got {d})")
+    return _DTYPES[q.dtype]
+
+
+def _aligned(x):
+    """Whether the kernels can read or write x's rows in 16-byte vectors."""
+    b = x.element_size()
+    return x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and \
+        all(n == 1 or s * b % 16 == 0 for n, s in zip(x.shape[:-1], x.stride()[:-1]))
+
+
+def _vectors(x):
+    return x if _aligned(x) else x.clone(memory_format=torch.contiguous_format)
+
+
+def _empty_like(x):
+    """A dense tensor in x's order of axes, with rows the kernels can write."""
+    y = torch.empty_like(x)
+    return y if _aligned(y) else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _rows(x, heads_last=False):
+    """x [E, T, H(, D)] (rollouts) or [E, H(, D)] (a step) as a bsg_rows."""
+    s = [0 if n == 1 else st for n, st in zip(x.shape, x.stride())]
+    if not heads_last:
+        s = s[:-1]
+    return nat.BsgRows(x.data_ptr(), s[0], s[1] if len(s) == 3 else 0, s[-1])
+
+
+def _ptr(x):
+    return None if x is None else x.data_ptr()
+
+
+def _flags(who, first, shape):
+    if first is not None:
+        _shape(who, "first", first, *shape, dtype=(torch.bool, torch.uint8))
+
+
+def _numbers(who, scale, dim, softcap=0.0, window=0):
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 <= softcap < float("inf"):
+        raise ValueError(f"{who}: softcap must be finite and >= 0 (0 = none), got {softcap}")
+    if window < 0:
+        raise ValueError(f"{who}: window must be >= 0 (0 = the whole episode), got {window}")
+    return scale
+
+
+def _slopes(who, slopes, heads):
+    if slopes is None:
+        return None
+    _shape(who, "slopes", slopes, heads, dtype=torch.float32)
+    if slopes.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{who}: slopes are constants; they get no gradient")
+    return slopes.contiguous()
+
+
+def _no_grad(who, *xs):
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        raise ValueError(f"{who} has no gradient: act under torch.no_grad()")
+
+
+def _call(fn, args, dev):
+    with torch.cuda.device(dev):               # the launch goes to the tensors' device
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        nat.check(getattr(nat.load_library(), fn)(C.byref(args), stream), fn)
+
+
+# ---- the gated delta rule -------------------------------------------------------------------
+
+def _delta_args(dtype, scale, q, k, v, g, beta, first):
+    a = nat.BsgDelta()
+    a.num_envs, a.steps = (v.shape[0], v.shape[1]) if v.dim() == 4 else (v.shape[0], 1)
+    a.heads_k, a.heads_v, a.dim_k, a.dim_v = q.shape[-2], v.shape[-2], q.shape[-1], v.shape[-1]
+    a.dtype, a.gate_dtype, a.scale = dtype, _DTYPES[g.dtype], scale
+    a.q, a.k, a.v = _rows(q), _rows(k), _rows(v)
+    a.g, a.beta = _rows(g, True), _rows(beta, True)
+    if first is not None:
+        a.first, a.first_env = first.data_ptr(), first.stride(0)
+        a.first_step = first.stride(1) if first.dim() == 2 else 0
+    return a
+
+
+def _delta_check(who, q, k, v, g, beta, state, first, lead):
+    E, Hk, Dk, H, Dv = q.shape[0], q.shape[-2], q.shape[-1], v.shape[-2], v.shape[-1]
+    _shape(who, "k", k, *lead, Hk, Dk)
+    _shape(who, "q", q, *lead, Hk, Dk)
+    if Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"{who}: {H} value heads do not share {Hk} key heads evenly")
+    gates = (torch.float32, q.dtype)
+    _shape(who, "g", g, *lead, H, dtype=gates)
+    _shape(who, "beta", beta, *lead, H, dtype=(g.dtype,))
+    if state is not None:
+        _shape(who, "state", state, E, H, Dk, Dv, dtype=torch.float32)
+    _flags(who, first, lead)
+
+
+class _DeltaRule(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, first, lengths, scale, dtype, keep):
+        q, k, v = _vectors(q), _vectors(k), _vectors(v)
+        state = None if state is None else state.contiguous()
+        E, T, H, Dv = v.shape
+        Dk, dev = q.shape[-1], v.device
+        a = _delta_args(dtype, scale, q, k, v, g, beta, first)
+        out = _empty_like(v)
+        final = torch.empty((E, H, Dk, Dv), dtype=torch.float32, device=dev)
+        a.out, a.lengths, a.state, a.final_state = _rows(out), _ptr(lengths), _ptr(state), final.data_ptr()
+        kept = ()
+        if keep:
+            n = -(-T // nat.DELTA_CHUNK)
+            kept = (torch.empty((E, H, n, Dk, Dv), dtype=torch.float32, device=dev),
+                    torch.empty((E, H, n * nat.DELTA_CHUNK, Dv), dtype=torch.float32, device=dev))
+            a.kept_states, a.kept_w = kept[0].data_ptr(), kept[1].data_ptr()
+        _call("bsg_delta_forward", a, dev)
+        if keep:
+            ctx.save_for_backward(q, k, v, g, beta, first, lengths, *kept)
+            ctx.rest = scale, dtype
+            ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dfinal):
+        q, k, v, g, beta, first, lengths, states, w = ctx.saved_tensors
+        scale, dtype = ctx.rest
+        dout = torch.zeros_like(v, memory_format=torch.contiguous_format) if dout is None else _vectors(dout)
+        dfinal = None if dfinal is None else dfinal.contiguous()
+        dq, dk, dv = _empty_like(q), _empty_like(k), _empty_like(v)
+        dg, db = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (g, beta))
+        dstate = None
+        if ctx.needs_input_grad[5]:
+            dstate = torch.empty((v.shape[0], v.shape[2], q.shape[-1], v.shape[-1]), dtype=torch.float32, device=v.device)
+        ws, ww = torch.empty_like(states), torch.empty_like(w)
+        a = _delta_args(dtype, scale, q, k, v, g, beta, first)
+        a.lengths, a.kept_states, a.kept_w = _ptr(lengths), states.data_ptr(), w.data_ptr()
+        a.dout, a.dq, a.dk, a.dv = _rows(dout), _rows(dq), _rows(dk), _rows(dv)
+        a.dg, a.dbeta = _rows(dg, True), _rows(db, True)
+        a.dfinal, a.dstate, a.work_states, a.work_w = _ptr(dfinal), _ptr(dstate), ws.data_ptr(), ww.data_ptr()
+        _call("bsg_delta_backward", a, v.device)
+        return dq, dk, dv, dg, db, dstate, None, None, None, None, None
+
+
+def gated_delta_rule(q, k, v, g, beta, state=None, first=None, lengths=None, *, scale=None):
+    """The gated delta rule over a rollout: per env and value head, with a state ``S`` [Dk, Dv],
+
+        S <- exp(g) S  (0 at a first step);  S <- S + beta k (v - S^T k)^T;  out = scale S^T q
+
+    q, k [E, T, Hk, Dk]; v [E, T, Hv, Dv], Hv a multiple of Hk (key head h serves value heads
+    h r .. h r + r - 1); g (log decay, <= 0) and beta [E, T, Hv], both in q's dtype or fp32;
+    ``state`` fp32 [E, Hv, Dk, Dv] before the first step (None = 0).  Keys are used as given: make
+    them unit vectors (beta in [0, 2] then keeps S from growing).  scale: Dk ** -0.5 by default.
+
+    Returns ``out`` [E, T, Hv, Dv] and the state after the last step, fp32.  Differentiable once in
+    q, k, v, g, beta and state."""
+    who = "gated_delta_rule"
+    dtype = _heads(who, q, k, v, {"Dk": q.shape[-1], "Dv": v.shape[-1]}, 4)
+    E, T, H, Dv = v.shape
+    _delta_check(who, q, k, v, g, beta, state, first, (E, T))
+    if lengths is not None:
+        _shape(who, "lengths", lengths, E, dtype=torch.int32)
+        lengths = lengths.contiguous()
+    _tensors(who, q, k=k, v=v, g=g, beta=beta, state=state, first=first, lengths=lengths)
+    scale = _numbers(who, scale, q.shape[-1])
+    if E == 0 or T == 0:
+        zero = torch.zeros((E, H, q.shape[-1], Dv), dtype=torch.float32, device=v.device)
+        return v.clone(), zero if state is None else zero + state
+    keep = torch.is_grad_enabled() and any(
+        x is not None and x.requires_grad for x in (q, k, v, g, beta, state))
+    return _DeltaRule.apply(q, k, v, g, beta, state, first, lengths, scale, dtype, keep)
+
+
+def gated_delta_step(q, k, v, g, beta, state, first=None, *, scale=None, out=None):
+    """One RL step of the gated delta rule for a batch of envs, ``state`` updated in place.
+
+    q, k [E, Hk, Dk]; v [E, Hv, Dv]; g, beta [E, Hv]; state fp32 [E, Hv, Dk, Dv], contiguous;
+    ``first`` [E]: envs whose episode begins with this step (their state is forgotten, whatever it
+    holds).  Returns out [E, Hv, Dv] (``out=`` to write into a given tensor).  No gradient: a
+    learner replays the steps through :func:`gated_delta_rule`."""
+    who = "gated_delta_step"
+    dtype = _heads(who, q, k, v, {"Dk": q.shape[-1], "Dv": v.shape[-1]}, 3)
+    E = v.shape[0]
+    if state is None:
+        raise ValueError(f"{who}: state is updated in place and must be given")
+    _delta_check(who, q, k, v, g, beta, state, first, (E,))
+    _tensors(who, q, k=k, v=v, g=g, beta=beta, state=state, first=first, out=out)
+    _no_grad(who, q, k, v, g, beta, state)
+    if not state.is_contiguous() or state.data_ptr() % 16:
+        raise ValueError(f"{who}: state must be contiguous and 16-byte aligned")
+    out = _out(who, out, v)
+    if E == 0:
+        return out
+    q, k, v = _vectors(q), _vectors(k), _vectors(v)
+    a = _delta_args(dtype, _numbers(who, scale, q.shape[-1]), q, k, v, g, beta, first)
+    a.out, a.state, a.final_state = _rows(out), state.data_ptr(), state.data_ptr()
+    _call("bsg_delta_step", a, v.device)
+    return out
+
+
+def _out(who, out, like):
+    if out is None:
+        return _empty_like(like)
+    _shape(who, "out", out, *like.shape, dtype=like.dtype)
+    if not _aligned(out):
+        raise ValueError(f"{who}: out must have contiguous, 16-byte aligned rows")
+    return out
+
+
+# ---- attention over the episode -------------------------------------------------------------
+
+def _attention_args(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, out):
+    a = nat.BsgAttention()
+    a.num_envs, a.steps, a.heads_q, a.dim = q.shape
+    a.heads_k, a.dtype = k.shape[2], dtype
+    a.scale, a.softcap, a.window = numbers
+    a.q, a.k, a.v, a.out = _rows(q), _rows(k), _rows(v), _rows(out)
+    a.slopes, a.lengths, a.begins, a.lse = _ptr(slopes), _ptr(lengths), _ptr(begins), _ptr(lse)
+    if first is not None:
+        a.first, a.first_env, a.first_step = first.data_ptr(), first.stride(0), first.stride(1)
+    return a
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, first, lengths, slopes, numbers, dtype, keep):
+        q, k, v = _vectors(q), _vectors(k), _vectors(v)
+        E, T, H, _ = q.shape
+        dev = q.device
+        out = _empty_like(q)
+        begins = lse = None
+        if first is not None or numbers[2] > 0:
+            begins = torch.empty((E, T), dtype=torch.int32, device=dev)
+        if keep:
+            lse = torch.empty((E, H, T), dtype=torch.float32, device=dev)
+        _call("bsg_attention_forward",
+              _attention_args(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, out), dev)
+        if keep:
+            ctx.save_for_backward(q, k, v, first, lengths, slopes, begins, lse, out)
+            ctx.rest = numbers, dtype
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, first, lengths, slopes, begins, lse, out = ctx.saved_tensors
+        numbers, dtype = ctx.rest
+        dout = _vectors(dout)
+        dq, dk, dv, delta = _empty_like(q), _empty_like(k), _empty_like(v), torch.empty_like(lse)
+        a = _attention_args(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, out)
+        a.dout, a.dq, a.dk, a.dv, a.delta = _rows(dout), _rows(dq), _rows(dk), _rows(dv), delta.data_ptr()
+        _call("bsg_attention_backward", a, q.device)
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+def episode_attention(q, k, v, first=None, lengths=None, *, scale=None, softcap=0.0, slopes=None, window=0):
+    """Attention of each step of a rollout to the steps of its episode so far, itself included:
+
+        s_ij = scale q_i.k_j;  softcap tanh(s_ij / softcap) if softcap > 0;  - slopes[h] (i - j)
+        out_i = sum_j softmax_j(s_ij) v_j
+
+    q [E, T, Hq, D]; k, v [E, T, Hkv, D], Hq a multiple of Hkv (key head h serves query heads
+    h r .. h r + r - 1).  ``slopes`` fp32 [Hq] (>= 0: older steps count less) or None.  ``window``:
+    the number of last steps that are seen (0 = all of the episode).  scale: D ** -0.5 by default.
+    Returns out [E, T, Hq, D].  Differentiable once in q, k and v."""
+    who = "episode_attention"
+    dtype = _heads(who, q, k, v, {"the head dim": q.shape[-1]}, 4)
+    E, T, H, D = q.shape
+    Hk = k.shape[2]
+    _shape(who, "k", k, E, T, Hk, D)
+    _shape(who, "v", v, E, T, Hk, D)
+    if Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"{who}: {H} query heads do not share {Hk} key heads evenly")
+    _flags(who, first, (E, T))
+    if lengths is not None:
+        _shape(who, "lengths", lengths, E, dtype=torch.int32)
+        lengths = lengths.contiguous()
+    _tensors(who, q, k=k, v=v, first=first, lengths=lengths, slopes=slopes)
+    scale = _numbers(who, scale, D, softcap, window)
+    slopes = _slopes(who, slopes, H)
+    if E == 0 or T == 0:
+        return q.clone()
+    keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return _Attention.apply(q, k, v, first, lengths, slopes, (scale, float(softcap), min(int(window), T)), dtype, keep)
+
+
+def episode_attention_step(q, k, v, k_cache, v_cache, steps, first=None, *, scale=None, softcap=0.0,
+                           slopes=None, out=None):
+    """One RL step of :func:`episode_attention` for a batch of envs, over a ring of the last
+    steps' keys and values that the caller keeps: what ``episode_attention`` with
+    ``window=slots`` gives for that step.
+
+    q [E, Hq, D]; k, v [E, Hkv, D]; k_cache, v_cache [E, Hkv, slots, D], contiguous; ``steps``
+    int32 [E]: the steps of the running episode before this one (zeros at the start).  ``first``
+    [E]: envs whose episode begins with this step.  The step's key and value go into slot
+    ``n % slots`` (n = steps, 0 at a first step) and ``steps`` becomes n + 1, in place; a slot that
+    holds no step of the episode is not looked at, whatever it holds.  Returns out [E, Hq, D]
+    (``out=`` to write into a given tensor).  No gradient."""
+    who = "episode_attention_step"
+    dtype = _heads(who, q, k, v, {"the head dim": q.shape[-1]}, 3)
+    E, H, D = q.shape
+    Hk = k.shape[1]
+    _shape(who, "k", k, E, Hk, D)
+    _shape(who, "v", v, E, Hk, D)
+    if Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"{who}: {H} query heads do not share {Hk} key heads evenly")
+    if k_cache.dim() != 4 or k_cache.shape[2] < 1:
+        raise ValueError(f"{who}: k_cache must be [E, Hkv, slots, D] with at least one slot")
+    S = k_cache.shape[2]
+    _shape(who, "k_cache", k_cache, E, Hk, S, D, dtype=q.dtype)
+    _shape(who, "v_cache", v_cache, E, Hk, S, D, dtype=q.dtype)
+    _shape(who, "steps", steps, E, dtype=torch.int32)
+    _flags(who, first, (E,))
+    _tensors(who, q, k=k, v=v, k_cache=k_cache, v_cache=v_cache, steps=steps, first=first, slopes=slopes, out=out)
+    _no_grad(who, q, k, v, k_cache, v_cache)
+    for n, x in (("k_cache", k_cache), ("v_cache", v_cache), ("steps", steps)):
+        if not x.is_contiguous() or (n != "steps" and x.data_ptr() % 16):
+            raise ValueError(f"{who}: {n} must be contiguous and 16-byte aligned")
+    scale = _numbers(who, scale, D, softcap)
+    slopes = _slopes(who, slopes, H)
+    out = _out(who, out, q)
+    if E == 0:
+        return out
+    q, k, v = _vectors(q), _vectors(k), _vectors(v)
+    a = nat.BsgAttentionAct()
+    a.num_envs, a.slots, a.heads_q, a.heads_k, a.dim, a.dtype = E, S, H, Hk, D, dtype
+    a.scale, a.softcap = scale, softcap
+    a.q, a.k, a.v, a.out = _rows(q), _rows(k), _rows(v), _rows(out)
+    a.slopes, a.steps, a.k_cache, a.v_cache = _ptr(slopes), steps.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    if first is not None:
+        a.first, a.first_env = first.data_ptr(), first.stride(0)
+    need = nat.load_library().bsg_attention_step_bytes(C.byref(a))
+    if need > 0:
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.work, a.work_bytes = work.data_ptr(), need
+    _call("bsg_attention_step", a, q.device)
+    return out

@@ -812,6 +812,142 @@ int32_t bsg_policy_sac(const bsg_sac_actor* w, const float* obs, int32_t num_env
   return BSG_OK;
 }
 
+// ---- memory operators ----------------------------------------------------------------------
+namespace {
+
+bool head_dim(int d) { return d == 32 || d == 64 || d == 128; }
+
+// A view whose rows the kernels read or write in 16-byte vectors.
+bool vector_rows(const bsg_rows& r, int dtype) {
+  const int64_t bytes = dtype == BSG_BF16 ? 2 : 4;
+  return r.p && !(reinterpret_cast<uintptr_t>(r.p) & 15) && !((r.env * bytes) & 15) &&
+         !((r.step * bytes) & 15) && !((r.head * bytes) & 15);
+}
+
+int32_t check_delta(const bsg_delta* a, const char* who) {
+  if (!a) return fail(BSG_E_INVALID_ARG, "%s: null arguments", who);
+  if (a->num_envs < 0 || a->steps < 0) return fail(BSG_E_INVALID_ARG, "%s: num_envs or steps < 0", who);
+  if (a->heads_k < 1 || a->heads_v < 1 || a->heads_v % a->heads_k)
+    return fail(BSG_E_INVALID_ARG, "%s: heads_v (%d) must be a multiple of heads_k (%d)", who, a->heads_v, a->heads_k);
+  if (!head_dim(a->dim_k) || !head_dim(a->dim_v))
+    return fail(BSG_E_INVALID_ARG, "%s: dim_k and dim_v must be 32, 64 or 128 (got %d, %d)", who, a->dim_k, a->dim_v);
+  if ((a->dtype != BSG_F32 && a->dtype != BSG_BF16) || (a->gate_dtype != BSG_F32 && a->gate_dtype != a->dtype))
+    return fail(BSG_E_INVALID_ARG, "%s: dtype must be BSG_F32 or BSG_BF16, gate_dtype that or BSG_F32", who);
+  const int64_t chunks = ((int64_t)a->steps + BSG_DELTA_CHUNK - 1) / BSG_DELTA_CHUNK;
+  if ((int64_t)a->num_envs * a->heads_v * (chunks > 4 ? chunks : 4) > 0x7fffffffll)
+    return fail(BSG_E_INVALID_ARG, "%s: num_envs x heads_v x chunks exceeds 2^31 - 1", who);
+  return BSG_OK;
+}
+bool delta_inputs(const bsg_delta* a) {
+  return vector_rows(a->q, a->dtype) && vector_rows(a->k, a->dtype) && vector_rows(a->v, a->dtype) && a->g.p && a->beta.p;
+}
+
+int32_t check_heads(const char* who, int num_envs, int heads_q, int heads_k, int dim, int dtype, float softcap, int64_t per_head) {
+  if (num_envs < 0) return fail(BSG_E_INVALID_ARG, "%s: num_envs < 0", who);
+  if (heads_q < 1 || heads_k < 1 || heads_q % heads_k)
+    return fail(BSG_E_INVALID_ARG, "%s: heads_q (%d) must be a multiple of heads_k (%d)", who, heads_q, heads_k);
+  if (!head_dim(dim)) return fail(BSG_E_INVALID_ARG, "%s: dim must be 32, 64 or 128 (got %d)", who, dim);
+  if (dtype != BSG_F32 && dtype != BSG_BF16) return fail(BSG_E_INVALID_ARG, "%s: dtype must be BSG_F32 or BSG_BF16", who);
+  if (!(softcap >= 0.0f)) return fail(BSG_E_INVALID_ARG, "%s: softcap must be >= 0", who);
+  if ((int64_t)num_envs * heads_q * per_head > 0x7fffffffll)
+    return fail(BSG_E_INVALID_ARG, "%s: num_envs x heads_q x tiles exceeds 2^31 - 1", who);
+  return BSG_OK;
+}
+int32_t check_attention(const bsg_attention* a, const char* who) {
+  if (!a) return fail(BSG_E_INVALID_ARG, "%s: null arguments", who);
+  if (a->steps < 0 || a->window < 0) return fail(BSG_E_INVALID_ARG, "%s: steps or window < 0", who);
+  if (int32_t r = check_heads(who, a->num_envs, a->heads_q, a->heads_k, a->dim, a->dtype, a->softcap, ((int64_t)a->steps + 63) / 64)) return r;
+  if (a->num_envs == 0 || a->steps == 0) return BSG_OK;
+  if (!vector_rows(a->q, a->dtype) || !vector_rows(a->k, a->dtype) || !vector_rows(a->v, a->dtype) || !vector_rows(a->out, a->dtype))
+    return fail(BSG_E_INVALID_ARG, "%s: q, k, v and out must be there, with 16-byte aligned rows", who);
+  if ((a->first || a->window > 0) && !a->begins)
+    return fail(BSG_E_INVALID_ARG, "%s: first or window without begins", who);
+  return BSG_OK;
+}
+// without an episode or window mask every step sees from 0: begins is not read
+bsg_attention with_begins(const bsg_attention* a) {
+  bsg_attention b = *a;
+  if (!b.first && b.window <= 0) b.begins = nullptr;
+  return b;
+}
+
+}  // namespace
+
+int32_t bsg_delta_forward(const bsg_delta* a, void* stream) {
+  if (int32_t r = check_delta(a, "bsg_delta_forward")) return r;
+  if (a->num_envs == 0) return BSG_OK;
+  if (a->steps > 0 && (!delta_inputs(a) || !vector_rows(a->out, a->dtype)))
+    return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: q, k, v, g, beta and out must be there, with 16-byte aligned rows of q, k, v and out");
+  if (!a->kept_states != !a->kept_w) return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: kept_states and kept_w go together");
+  hipError_t e = bsg::launch_delta_forward(*a, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_delta_forward launch");
+}
+
+int32_t bsg_delta_backward(const bsg_delta* a, void* stream) {
+  if (int32_t r = check_delta(a, "bsg_delta_backward")) return r;
+  if (a->num_envs == 0 || a->steps == 0) return BSG_OK;
+  if (!delta_inputs(a) || !vector_rows(a->dout, a->dtype) || !vector_rows(a->dq, a->dtype) || !vector_rows(a->dk, a->dtype) ||
+      !vector_rows(a->dv, a->dtype) || !a->dg.p || !a->dbeta.p)
+    return fail(BSG_E_INVALID_ARG, "bsg_delta_backward: inputs and gradients must be there, with 16-byte aligned rows of dim values");
+  const void* scratch[] = {a->kept_states, a->kept_w, a->work_states, a->work_w};
+  for (const void* p : scratch)
+    if (!p || (reinterpret_cast<uintptr_t>(p) & 15))
+      return fail(BSG_E_INVALID_ARG, "bsg_delta_backward: kept_* and work_* must be there, 16-byte aligned");
+  hipError_t e = bsg::launch_delta_backward(*a, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_delta_backward launch");
+}
+
+int32_t bsg_delta_step(const bsg_delta* a, void* stream) {
+  if (int32_t r = check_delta(a, "bsg_delta_step")) return r;
+  if (a->steps != 1 || a->lengths) return fail(BSG_E_INVALID_ARG, "bsg_delta_step: steps must be 1 and lengths NULL");
+  if (a->num_envs == 0) return BSG_OK;
+  if (!a->state || a->state != a->final_state || (reinterpret_cast<uintptr_t>(a->state) & 15))
+    return fail(BSG_E_INVALID_ARG, "bsg_delta_step: state and final_state must be one 16-byte aligned buffer");
+  if (!delta_inputs(a) || !vector_rows(a->out, a->dtype))
+    return fail(BSG_E_INVALID_ARG, "bsg_delta_step: q, k, v, g, beta and out must be there, with 16-byte aligned rows of q, k, v and out");
+  hipError_t e = bsg::launch_delta_step(*a, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_delta_step launch");
+}
+
+int32_t bsg_attention_forward(const bsg_attention* a, void* stream) {
+  if (int32_t r = check_attention(a, "bsg_attention_forward")) return r;
+  if (a->num_envs == 0 || a->steps == 0) return BSG_OK;
+  hipError_t e = bsg::launch_attention(with_begins(a), false, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_attention_forward launch");
+}
+
+int32_t bsg_attention_backward(const bsg_attention* a, void* stream) {
+  if (int32_t r = check_attention(a, "bsg_attention_backward")) return r;
+  if (a->num_envs == 0 || a->steps == 0) return BSG_OK;
+  if (!vector_rows(a->dout, a->dtype) || !vector_rows(a->dq, a->dtype) || !vector_rows(a->dk, a->dtype) || !vector_rows(a->dv, a->dtype))
+    return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: dout, dq, dk and dv must be there, with 16-byte aligned rows");
+  if (!a->lse || !a->delta) return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: null lse or delta");
+  hipError_t e = bsg::launch_attention(with_begins(a), true, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_attention_backward launch");
+}
+
+int64_t bsg_attention_step_bytes(const bsg_attention_act* a) {
+  if (!a) return fail(BSG_E_INVALID_ARG, "bsg_attention_step_bytes: null arguments");
+  if (a->slots < 1 || a->slots > 1 << 30) return fail(BSG_E_INVALID_ARG, "bsg_attention_step_bytes: slots must be in [1, 2^30]");
+  if (int32_t r = check_heads("bsg_attention_step_bytes", a->num_envs, a->heads_q, a->heads_k, a->dim, a->dtype, a->softcap, 1)) return r;
+  return a->num_envs == 0 ? 0 : bsg::attention_step_bytes(*a);
+}
+
+int32_t bsg_attention_step(const bsg_attention_act* a, void* stream) {
+  const int64_t need = bsg_attention_step_bytes(a);
+  if (need < 0) return (int32_t)need;
+  if (a->num_envs == 0) return BSG_OK;
+  const int32_t dt = a->dtype;
+  if (!vector_rows(a->q, dt) || !vector_rows(a->k, dt) || !vector_rows(a->v, dt) || !vector_rows(a->out, dt))
+    return fail(BSG_E_INVALID_ARG, "bsg_attention_step: q, k, v and out must be there, with 16-byte aligned rows");
+  if (!a->steps || !a->k_cache || !a->v_cache || ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15))
+    return fail(BSG_E_INVALID_ARG, "bsg_attention_step: steps and 16-byte aligned caches must be there");
+  if (need > 0 && (!a->work || a->work_bytes < need))
+    return fail(BSG_E_INVALID_ARG, "bsg_attention_step: work must hold %lld bytes", (long long)need);
+  hipError_t e = bsg::launch_attention_step(*a, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_attention_step launch");
+}
+
 int32_t bsg_set_stamps(bsg_ctx* c, void* buf) {
   if (!c) return fail(BSG_E_INVALID_ARG, "bsg_set_stamps: null ctx");
 #if defined(BSG_STAMPS) && BSG_STAMPS

@@ -344,6 +344,116 @@ int32_t bsg_policy_sac(const bsg_sac_actor* actor, const float* obs, int32_t num
                        int32_t obs_stride, const float* eps, double* actions, float* log_prob,
                        void* stream);
 
+/* ---- memory operators: the sequence layers of a policy with memory ----------------------
+ * A policy that sees noisy or partial states (the wind and uncertainty wrappers) carries what
+ * it saw through the steps of an episode.  Two such layers, each in the form that acts (one
+ * RL step of a batch, state or cache updated in place) and the form that learns (rollouts of
+ * several steps, with gradients): the gated delta rule and attention over the episode.  They
+ * replace nothing in the reference, whose actors are feed-forward (SB3's MultiInputPolicy); they
+ * stand beside bsg_policy_sac.
+ *
+ * A bsg_rows is a view [num_envs][steps][heads][dim] of device memory: element strides of the
+ * env, step and head axis, unit stride in the last.  Rows that are read or written in vectors
+ * (q, k, v, out and their gradients) are 16-byte aligned, pointer and strides alike.
+ * first[e][t] != 0: step t of env e is the first of an episode, nothing from before it is
+ * seen.  lengths[e] (0..steps, NULL = all): steps at or after it are padding: they are never
+ * read, and their outputs and gradients are written as zeros.  The values of the steps before
+ * it have to be finite where the output is to be: a non-finite value may reach every output of
+ * its env, but no other env's.
+ * All calls are asynchronous on `stream`, capturable, and use no memory but the caller's. */
+enum { BSG_F32 = 0, BSG_BF16 = 1 };
+typedef struct bsg_rows {
+  void* p;
+  int64_t env, step, head;   /* strides in elements */
+} bsg_rows;
+
+/* The gated delta rule, per env and value head, with a state S[dim_k][dim_v] (fp32):
+ *   S <- e^g S (0 at a first step);  w = v - S^T k;  S <- S + beta k w^T;  out = scale S^T q
+ * Query/key head h serves the value heads h r .. h r + r - 1, r = heads_v / heads_k.
+ * g <= 0 is the log of the decay (values below -1e5 act as -1e5: nothing is left).  The solve
+ * inside a chunk of steps is well conditioned for unit keys and beta in [0, 2].
+ * dims: 32, 64 or 128.  gates (g, beta, their gradients): dtype or fp32. */
+#define BSG_DELTA_CHUNK 64
+typedef struct bsg_delta {
+  int32_t num_envs, steps;
+  int32_t heads_k, heads_v, dim_k, dim_v;
+  int32_t dtype, gate_dtype; /* BSG_F32 / BSG_BF16 */
+  float scale;
+  int32_t reserved;
+  bsg_rows q, k, v, g, beta, out;
+  const uint8_t* first;      /* NULL: the rows continue the state throughout */
+  int64_t first_env, first_step;
+  const int32_t* lengths;    /* NULL: all steps */
+  const float* state;        /* [num_envs][heads_v][dim_k][dim_v] before the first step; NULL = 0 */
+  float* final_state;        /* the same after the last step; NULL = not wanted */
+  /* kept by the forward pass for the backward pass (both NULL: not kept), with
+   * chunks = ceil(steps / BSG_DELTA_CHUNK) */
+  float* kept_states;        /* [num_envs][heads_v][chunks][dim_k][dim_v] */
+  float* kept_w;             /* [num_envs][heads_v][chunks * BSG_DELTA_CHUNK][dim_v] */
+  /* backward only */
+  bsg_rows dout, dq, dk, dv, dg, dbeta;
+  const float* dfinal;       /* gradient of final_state; NULL = 0 */
+  float* dstate;             /* gradient of state; NULL = not wanted */
+  float* work_states;        /* scratch, as kept_states */
+  float* work_w;             /* scratch, as kept_w */
+} bsg_delta;
+int32_t bsg_delta_forward(const bsg_delta* a, void* stream);
+int32_t bsg_delta_backward(const bsg_delta* a, void* stream);
+/* One step of every env: steps = 1, `state` = `final_state` updated in place (it must not be
+ * NULL); a first step forgets it.  Reads q, k, v, g, beta, first; `lengths` must be NULL. */
+int32_t bsg_delta_step(const bsg_delta* a, void* stream);
+
+/* Attention of each step to the steps of its episode so far, per env and query head:
+ *   s_ij = scale q_i.k_j, capped to softcap tanh(s_ij / softcap) if softcap > 0, less
+ *   slopes[h] (i - j);  out_i = sum_j softmax_j(s_ij) v_j
+ * over j <= i of the same episode, and i - j < window if window > 0.  Key/value head h serves
+ * the query heads h r .. h r + r - 1, r = heads_q / heads_k.  dim: 32, 64 or 128. */
+typedef struct bsg_attention {
+  int32_t num_envs, steps;
+  int32_t heads_q, heads_k, dim;
+  int32_t dtype;
+  int32_t window;            /* 0 = the whole episode */
+  float scale, softcap;      /* softcap 0 = none */
+  int32_t reserved;
+  bsg_rows q, k, v, out;
+  const float* slopes;       /* [heads_q]; NULL = no bias */
+  const uint8_t* first;
+  int64_t first_env, first_step;
+  const int32_t* lengths;
+  int32_t* begins;           /* [num_envs][steps] scratch of the forward pass, read by the backward
+                                pass: the first step that each step sees; may be NULL if first
+                                is NULL and window is 0 */
+  float* lse;                /* [num_envs][heads_q][steps] kept for the backward pass; NULL = not */
+  /* backward only (out as the forward pass wrote it) */
+  bsg_rows dout, dq, dk, dv;
+  float* delta;              /* [num_envs][heads_q][steps] scratch */
+} bsg_attention;
+int32_t bsg_attention_forward(const bsg_attention* a, void* stream);
+int32_t bsg_attention_backward(const bsg_attention* a, void* stream);
+
+/* One acting step with a ring of the last `slots` steps' keys and values per env and head,
+ * k_cache / v_cache [num_envs][heads_k][slots][dim] (contiguous, dtype).  steps[e] counts the
+ * steps of the running episode before this one (first[e] != 0: it becomes 0); step n goes into
+ * slot n % slots, and the query attends to the steps that the ring holds, with s_ij as above.
+ * steps[e] is one more afterwards (it stays at its largest value).  Slots that hold no step
+ * of the episode are never read into a result.  work: bsg_attention_step_bytes() bytes. */
+typedef struct bsg_attention_act {
+  int32_t num_envs, slots;
+  int32_t heads_q, heads_k, dim;
+  int32_t dtype;
+  float scale, softcap;
+  bsg_rows q, k, v, out;     /* .step unused */
+  const float* slopes;
+  const uint8_t* first;      /* NULL: no env starts an episode */
+  int64_t first_env;
+  int32_t* steps;
+  void *k_cache, *v_cache;
+  void* work;
+  int64_t work_bytes;
+} bsg_attention_act;
+int64_t bsg_attention_step_bytes(const bsg_attention_act* a);
+int32_t bsg_attention_step(const bsg_attention_act* a, void* stream);
+
 /* ---- the multi-GPU learner-row all-gather (RCCL over xGMI) -----------------------------
  * Replaces: the reference's vectorisation is SubprocVecEnv (scripts/multi_processing_example
  * .py:51-53), one env per process feeding one learner; here every rank's shard of envs
