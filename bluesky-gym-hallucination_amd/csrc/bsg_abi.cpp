@@ -878,7 +878,8 @@ int32_t bsg_delta_forward(const bsg_delta* a, void* stream) {
   if (a->num_envs == 0) return BSG_OK;
   if (a->steps > 0 && (!delta_inputs(a) || !vector_rows(a->out, a->dtype)))
     return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: q, k, v, g, beta and out must be there, with 16-byte aligned rows of q, k, v and out");
-  if (!a->kept_states != !a->kept_w) return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: kept_states and kept_w go together");
+  if (!a->kept_states != !a->kept_w || ((reinterpret_cast<uintptr_t>(a->kept_states) | reinterpret_cast<uintptr_t>(a->kept_w)) & 15))
+    return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: kept_states and kept_w go together, 16-byte aligned");
   hipError_t e = bsg::launch_delta_forward(*a, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_delta_forward launch");
 }

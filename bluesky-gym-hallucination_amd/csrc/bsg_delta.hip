@@ -59,18 +59,66 @@ __device__ __forceinline__ int steps_of(const bsg_delta& a, int e) {
   return a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
 }
 
-// The gates of a chunk, one lane of a wave per step.
+// The gates of a chunk, one lane of a wave per step.  c is kept in units of log 2 (v_exp_f32 is a
+// power of two, and the product with log2 e is rounded in double).
 struct Gates {
   float hi[C], lo[C];              // c_i
   float in[C], out[C], beta[C];
   int episode[C];                  // episodes begun in the chunk up to i
-  float across;
+  float across, pad[3];
 };
-__device__ __forceinline__ void read_gates(Gates& s, const bsg_delta& a, int e, int h, int t0, int rows, int lane) {
-  const bool on = lane < rows;
-  double c = on ? (double)fmaxf(gate(a.g, a.gate_dtype, e, t0 + lane, h), LOWEST) : 0.0;
-  const bool f = on && a.first && a.first[e * a.first_env + (t0 + lane) * a.first_step] != 0;
-  const unsigned long long begun = __ballot(f);
+// The kernel's arguments, read anew: what is needed once a chunk or once a head is then not kept in
+// scalar registers all along (the compiler takes the address for a new one each time).
+__device__ __forceinline__ const bsg_delta& arguments() {
+  typedef const __attribute__((address_space(4))) bsg_delta* Args;
+  Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const bsg_delta*)p;
+}
+
+// An env's and head's rows along the steps.
+template <class T> struct Steps {
+  T* p;
+  int64_t step;
+  __device__ __forceinline__ T* at(int t) const { return p + t * step; }
+};
+template <class T> __device__ __forceinline__ Steps<T> steps_in(const bsg_rows& x, int e, int h) {
+  return {static_cast<T*>(x.p) + e * x.env + h * x.head, x.step};
+}
+struct GateSteps {
+  const char *g, *beta;
+  const uint8_t* first;
+  int64_t g_step, beta_step, first_step;   // in bytes
+  bool half;
+  __device__ __forceinline__ GateSteps(const bsg_delta& a, int e, int h) {
+    half = a.gate_dtype == BSG_BF16;
+    const int b = half ? 2 : 4;
+    g = static_cast<const char*>(a.g.p) + (e * a.g.env + h * a.g.head) * b;
+    beta = static_cast<const char*>(a.beta.p) + (e * a.beta.env + h * a.beta.head) * b;
+    first = a.first ? a.first + e * a.first_env : nullptr;
+    g_step = a.g.step * b, beta_step = a.beta.step * b, first_step = a.first_step;
+  }
+};
+// A lane's step as it lies in memory, not looked at before make_gates (the loads stay in flight).
+struct RawGates { uint32_t g, beta, first; };
+__device__ __forceinline__ RawGates load_gates(const GateSteps& s, int t0, int rows, int lane) {
+  RawGates r = {0, 0, 0};
+  if (lane < rows) {
+    const int t = t0 + lane;
+    if (s.half) {
+      r.g = *reinterpret_cast<const uint16_t*>(s.g + t * s.g_step);
+      r.beta = *reinterpret_cast<const uint16_t*>(s.beta + t * s.beta_step);
+    } else {
+      r.g = *reinterpret_cast<const uint32_t*>(s.g + t * s.g_step);
+      r.beta = *reinterpret_cast<const uint32_t*>(s.beta + t * s.beta_step);
+    }
+    if (s.first) r.first = s.first[t * s.first_step];
+  }
+  return r;
+}
+__device__ __forceinline__ void make_gates(Gates& s, const RawGates& raw, bool half, int lane) {
+  double c = (double)fmaxf(__uint_as_float(half ? raw.g << 16 : raw.g), LOWEST) * 1.4426950408889634074;
+  const unsigned long long begun = __ballot(raw.first != 0);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const double o = __shfl_up(c, d);
@@ -80,79 +128,191 @@ __device__ __forceinline__ void read_gates(Gates& s, const bsg_delta& a, int e, 
   const int ep = __popcll(begun & (~0ull >> (63 - lane))), all = __popcll(begun);
   s.hi[lane] = (float)c;
   s.lo[lane] = (float)(c - (double)(float)c);
-  s.in[lane] = ep == 0 ? expf((float)c) : 0.0f;
-  s.out[lane] = ep == all ? expf((float)(last - c)) : 0.0f;
-  s.beta[lane] = on ? gate(a.beta, a.gate_dtype, e, t0 + lane, h) : 0.0f;
+  s.in[lane] = ep == 0 ? __builtin_amdgcn_exp2f((float)c) : 0.0f;
+  s.out[lane] = ep == all ? __builtin_amdgcn_exp2f((float)(last - c)) : 0.0f;
+  s.beta[lane] = __uint_as_float(half ? raw.beta << 16 : raw.beta);
   s.episode[lane] = ep;
-  if (lane == 0) s.across = all == 0 ? expf((float)last) : 0.0f;
+  if (lane == 0) s.across = all == 0 ? __builtin_amdgcn_exp2f((float)last) : 0.0f;
 }
 __device__ __forceinline__ float decay(const Gates& s, int i, int j) {
-  return s.episode[i] == s.episode[j] ? expf((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j])) : 0.0f;
+  return s.episode[i] == s.episode[j] ? __builtin_amdgcn_exp2f((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j])) : 0.0f;
 }
 
-// What the passes along a rollout share of a chunk.  A workgroup of NW waves handles one env and
-// value head; wave w owns the 16 value columns 16 w .. 16 w + 15 and keeps their part of the state
-// in registers (as D tiles, whose rows are the key dimension), so the waves only meet over the
-// C x C matrices.
-template <class T, int DK>
+// A workgroup of NW waves handles one env and value head; wave w owns the 16 value columns
+// 16 w .. 16 w + 15 and keeps their part of the state in registers (as D tiles, whose rows are the
+// key dimension), so the waves only meet over the C x C matrices.
+template <class T, int DK, int NW>
 struct Chunk {
-  T k[C * pitch<T>(DK)], q[C * pitch<T>(DK)];
+  static constexpr int LD = pitch<T>(DK), VD = pitch<T>(16 * NW), PD = pitch<T>(C), parts = Parts<T, 2>::n;
+  T k[C * LD], q[C * LD];
+  T v[C * VD];                     // v (dout), then, column by column, out (v')
+  T p[parts][C * PD];              // P in parts of type T, zeros above its diagonal
   float n[C * AP];                 // minus the matrix of the system, below the diagonal
-  float p[C * AP];                 // P, its diagonal blocks filled with zeros above
   float inv[4 * 16 * IP];          // inverses of the system's diagonal blocks
-  Gates gates;
+  Gates gates[2];                  // of this chunk and the one that comes next
+  __device__ __forceinline__ WideOf<T, 2> p_row(int r, int k0, int g) const {
+    WideOf<T, 2> w;
+#pragma unroll
+    for (int i = 0; i < parts; ++i) w.p[i] = load_tile(&p[i][r * PD], k0, g);
+    return w;
+  }
+  __device__ __forceinline__ WideOf<T, 2> p_col(int m0, int k0, int lane) const {
+    WideOf<T, 2> w;
+#pragma unroll
+    for (int i = 0; i < parts; ++i) w.p[i] = load_col(p[i], PD, k0, m0, lane);
+    return w;
+  }
+};
+// Waves per SIMD that LDS leaves room for, two at most: what bounds the passes' registers.
+template <class T, int DK, int NW> constexpr int waves_per_simd() {
+  return NW == 2 ? 1 : NW == 8 || 2 * sizeof(Chunk<T, DK, NW>) <= 160 * 1024 ? 2 : 1;
+}
+
+// A C x N tile on its way from memory to LDS through registers: loaded while the chunk before it is
+// computed.  Rows behind `rows` (at least 1) become zeros; in their place the last one is read.
+template <class T, int N, int NT>
+struct Fetch {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  static constexpr int V = Vec<T>::n, ROW = N / V, n = (C * ROW + NT - 1) / NT;
+  u32x4 x[n];
+  __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int tid) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const int at = tid + i * NT, r = at / ROW, c = at % ROW * V;
+      x[i] = *reinterpret_cast<const u32x4*>(p + min(r, rows - 1) * stride + c);
+    }
+  }
+  __device__ __forceinline__ void store(T* s, int rows, int tid) const {
+    if (rows >= C) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) put(s, tid + i * NT, x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < n; ++i) put(s, tid + i * NT, (tid + i * NT) / ROW < rows ? x[i] : u32x4{0, 0, 0, 0});
+    }
+  }
+  static __device__ __forceinline__ void put(T* s, int at, const u32x4& v) {
+    const int r = at / ROW, c = at % ROW * V;
+    if (C * ROW % NT == 0 || r < C) *reinterpret_cast<u32x4*>(s + r * pitch<T>(N) + c) = v;
+  }
 };
 
-// N and P, then the inverses.  BACK: the system is (I + diag(beta) N)^T, else I + N diag(beta).
+// A wave's 16 columns of the C x 16 NW tile: from registers (D tiles) to LDS, and from there, in
+// 16-byte pieces, to the rows in memory.  Rows behind `rows` are padding: zeros, up to `all`.
+template <class T, int VD>
+__device__ __forceinline__ void put_columns(T* s, const f32x4* x, int w, int lane) {
+  const int m = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[(16 * b + 4 * g + r) * VD + 16 * w + m] = (T)x[b][r];
+}
+template <class T, int VD>
+__device__ __forceinline__ void write_columns(const T* s, T* to, int64_t stride, int rows, int all, int w, int lane) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  constexpr int V = Vec<T>::n, P = 16 / V;       // pieces to a row
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int r = (lane + 64 * i) / P, c = 16 * w + (lane + 64 * i) % P * V;
+    u32x4 x = *reinterpret_cast<const u32x4*>(s + r * VD + c);
+    if (r >= rows) x = u32x4{0, 0, 0, 0};
+    if (r < all) *reinterpret_cast<u32x4*>(to + r * stride + c) = x;
+  }
+}
+
+// lane j of each row of 16 lanes, to all of them
+template <int J> __device__ __forceinline__ float from_lane(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + J, 0xf, 0xf, false));
+}
+// x[c] of lane i, c <= J: minus n_iJ times row J of the inverse, which is done
+template <int J> __device__ __forceinline__ void eliminate(float (&x)[16], const float (&n)[16]) {
+  if constexpr (J < 15) {
+#pragma unroll
+    for (int c = 0; c <= J; ++c) x[c] = fmaf(from_lane<J>(x[c]), n[J], x[c]);
+    eliminate<J + 1>(x, n);
+  }
+}
+
+// The ten lower tiles of N and P (one decay serves both), then, after a barrier, the inverses by
+// wave NW - 1, which has the fewest tiles; the others go on to what does not need them.  An
+// inverse's row lies in a lane, and its substitution takes the rows before from their lanes.
+// BACK: the system is (I + diag(beta) N)^T, else I + N diag(beta).
 template <class T, int DK, int NW, bool BACK>
-__device__ __forceinline__ void solve_chunk(Chunk<T, DK>& s, float scale, int lane, int w) {
+__device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& s, const Gates& gates, float scale, int lane, int w) {
   constexpr int LD = pitch<T>(DK);
   const int m = lane & 15, g = lane >> 4;
-  // eight strips of 16 rows, N's in rising and P's in falling length, over the waves
-  for (int task = w; task < 8; task += NW) {
-    const bool isP = task >= 4;
-    const int b = isP ? 7 - task : task;
-    const T* rows = (isP ? s.q : s.k) + (16 * b + m) * LD;
-    Frag<T> af[DK / 32];
 #pragma unroll
-    for (int c = 0; c < DK / 32; ++c) af[c] = load_run(rows, 32 * c, g);
-    for (int u = 0; u <= b; ++u) {
-      f32x4 d = {0, 0, 0, 0};
+  for (int t0 = 0; t0 < 10; t0 += NW) {
+    const int t = t0 + w;
+    if (t >= 10) break;
+    const int b = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, u = t - b * (b + 1) / 2, j = 16 * u + m;
+    f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
 #pragma unroll
-      for (int c = 0; c < DK / 32; ++c) mma(d, af[c], load_run(s.k + (16 * u + m) * LD, 32 * c, g));
-      const int j = 16 * u + m;
+    for (int c = 0; c < DK / 32; ++c) {
+      const Frag<T> kj = load_run(s.k + j * LD, 32 * c, g);
+      mma(kk, load_run(s.k + (16 * b + m) * LD, 32 * c, g), kj);
+      mma(qk, load_run(s.q + (16 * b + m) * LD, 32 * c, g), kj);
+    }
+    const float bj = gates.beta[j];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * b + 4 * g + r;
-        const float f = decay(s.gates, i, j);
-        if (isP) s.p[i * AP + j] = j <= i ? scale * f * d[r] : 0.0f;
-        else s.n[i * AP + j] = j < i ? -s.gates.beta[BACK ? i : j] * f * d[r] : 0.0f;
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * b + 4 * g + r;
+      const float f = decay(gates, i, j);
+      s.n[i * AP + j] = j < i ? -(BACK ? gates.beta[i] : bj) * f * kk[r] : 0.0f;
+      float y = j <= i ? scale * f * qk[r] : 0.0f;
+#pragma unroll
+      for (int o = 0; o < Parts<T, 2>::n; ++o) {
+        const T z = (T)y;
+        s.p[o][i * Chunk<T, DK, NW>::PD + j] = z;
+        y -= (float)z;
       }
     }
   }
   __syncthreads();
-  if (w == 0) {                    // lane: block g, column m, by substitution down the rows
-    float x[16];
-    const float* nb = s.n + 16 * g * AP + 16 * g;
+  if (w == NW - 1) {               // lane: block g, row m
+    float x[16], n[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[i] = i == m ? 1.0f : 0.0f;
+    for (int j = 0; j < 16; j += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(&s.n[(16 * g + m) * AP + 16 * g + j]);
 #pragma unroll
-      for (int j = 0; j < i; ++j) x[i] = fmaf(nb[i * AP + j], x[j], x[i]);
-      s.inv[(16 * g + i) * IP + m] = x[i];
+      for (int o = 0; o < 4; ++o) n[j + o] = v[o];
     }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = j == m ? 1.0f : 0.0f;
+    eliminate<0>(x, n);
+#pragma unroll
+    for (int j = 0; j < 16; j += 4)
+      *reinterpret_cast<f32x4*>(&s.inv[(16 * g + m) * IP + j]) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
   }
+}
+// P's tiles above the diagonal that share a product step with one on it
+template <class T, int DK, int NW>
+__device__ __forceinline__ void clear_above(Chunk<T, DK, NW>& s, int tid) {
+  for (int i = tid; i < 2 * 256; i += 64 * NW) {
+    const int b = i / 256 * 32, r = i % 256 / 16, c = i % 16;
+#pragma unroll
+    for (int o = 0; o < Parts<T, 2>::n; ++o) s.p[o][(b + r) * Chunk<T, DK, NW>::PD + b + 16 + c] = (T)0.0f;
+  }
+}
+
+// the first two parts: enough for what ends in an output of type T
+__device__ __forceinline__ const Wide<float, 1>& front(const Wide<float, 1>& w) { return w; }
+__device__ __forceinline__ Wide<bf16, 2> front(const Wide<bf16, 3>& w) { return Wide<bf16, 2>{{w.p[0], w.p[1]}}; }
+
+// States and W (M) that only these kernels read lie as their D tiles do: 16 bytes a lane, wave by wave.
+template <int NW> __device__ __forceinline__ float* tiles(float* p, int64_t chunk, int tiles_per_wave, int w, int lane) {
+  return p + ((chunk * NW + w) * tiles_per_wave * 64 + lane) * 4;
 }
 
 // ---- forward -------------------------------------------------------------------------------
 template <class T, int DK, int NW>
-__global__ __launch_bounds__(64 * NW) void forward_kernel(bsg_delta a) {
-  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW;
-  __shared__ __align__(16) Chunk<T, DK> s;
+__global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void forward_kernel(bsg_delta a) {
+  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW, VD = pitch<T>(DV);
+  __shared__ __align__(16) Chunk<T, DK, NW> s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % a.heads_v, e = blockIdx.x / a.heads_v, hk = h / (a.heads_v / a.heads_k);
   const int n = steps_of(a, e), col = 16 * w + m;
-  const int chunks = (a.steps + C - 1) / C;
+  const int chunks = (a.steps + C - 1) / C, live = (n + C - 1) / C;
   const int64_t eh = (int64_t)e * a.heads_v + h;
 
   f32x4 S[DT];
@@ -162,33 +322,40 @@ __global__ __launch_bounds__(64 * NW) void forward_kernel(bsg_delta a) {
     for (int r = 0; r < 4; ++r)
       S[d][r] = a.state ? a.state[(eh * DK + 16 * d + 4 * g + r) * DV + col] : 0.0f;
 
-  for (int ch = 0; ch < chunks; ++ch) {
-    const int t0 = ch * C, rows = min(C, n - t0);
-    if (rows <= 0) {               // padding: zeros
-      for (int i = tid; i < min(C, a.steps - t0) * DV; i += 64 * NW) row_out<T>(a.out, e, t0 + i / DV, h)[i % DV] = (T)0.0f;
-      continue;
+  Fetch<T, DK, NT> fk, fq;
+  Fetch<T, DV, NT> fv;
+  RawGates raw = {0, 0, 0};
+  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), v = steps_in<const T>(a.v, e, h);
+  const Steps<T> out = steps_in<T>(a.out, e, h);
+  const GateSteps gate(a, e, h);
+  float *const ks = a.kept_states ? tiles<NW>(a.kept_states, eh * chunks, DT, w, lane) : nullptr;
+  float *const kw = a.kept_w ? tiles<NW>(a.kept_w, eh * chunks, 4, w, lane) : nullptr;
+  if (live > 0) {
+    fk.load(k.p, k.step, n, tid);
+    fq.load(q.p, q.step, n, tid);
+    fv.load(v.p, v.step, n, tid);
+    if (w == 0) make_gates(s.gates[0], load_gates(gate, 0, n, lane), gate.half, lane);
+    clear_above(s, tid);
+  }
+  for (int ch = 0; ch < live; ++ch) {
+    const int t0 = ch * C, rows = min(C, n - t0), t1 = t0 + C;
+    const Gates& gates = s.gates[ch & 1];
+    __syncthreads();               // the chunk before is done with LDS
+    fk.store(s.k, rows, tid);
+    fq.store(s.q, rows, tid);
+    fv.store(s.v, rows, tid);
+    if (t1 < n) {
+      fk.load(k.at(t1), k.step, n - t1, tid);
+      fq.load(q.at(t1), q.step, n - t1, tid);
+      fv.load(v.at(t1), v.step, n - t1, tid);
+      if (w == 0) raw = load_gates(gate, t1, n - t1, lane);
     }
-    f32x4 v[4];
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = 16 * b + 4 * g + r;
-        v[b][r] = t < rows ? (float)row<T>(a.v, e, t0 + t, h)[col] : 0.0f;
-      }
     __syncthreads();
-    stage<T, DK, C>(s.k, row<T>(a.k, e, t0, hk), a.k.step, rows, tid, 64 * NW);
-    stage<T, DK, C>(s.q, row<T>(a.q, e, t0, hk), a.q.step, rows, tid, 64 * NW);
-    if (w == 0) read_gates(s.gates, a, e, h, t0, rows, lane);
-    __syncthreads();
-    solve_chunk<T, DK, NW, false>(s, a.scale, lane, w);
+    solve_chunk<T, DK, NW, false>(s, gates, a.scale, lane, w);
 
-    if (a.kept_states) {
-      float* ks = a.kept_states + (eh * chunks + ch) * DK * DV + col;
+    if (ks) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) ks[(16 * d + 4 * g + r) * DV] = S[d][r];
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(ks + (int64_t)ch * DK * DV + 256 * d) = S[d];
     }
     // K S and Q S
     f32x4 x[4], o[4];
@@ -201,17 +368,17 @@ __global__ __launch_bounds__(64 * NW) void forward_kernel(bsg_delta a) {
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         mma<T>(x[b], load_tile(s.k + (16 * b + m) * LD, 32 * c, g), sw);
-        mma<T>(o[b], load_tile(s.q + (16 * b + m) * LD, 32 * c, g), sw);
+        mma<T>(o[b], load_tile(s.q + (16 * b + m) * LD, 32 * c, g), front(sw));
       }
     }
-    f32x4 beta[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const f32x4 in = *reinterpret_cast<const f32x4*>(&s.gates.in[16 * b + 4 * g]);
-      beta[b] = *reinterpret_cast<const f32x4*>(&s.gates.beta[16 * b + 4 * g]);
-      x[b] = v[b] - in * x[b];
+      const f32x4 in = *reinterpret_cast<const f32x4*>(&gates.in[16 * b + 4 * g]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[b][r] = (float)s.v[(16 * b + 4 * g + r) * VD + col] - in[r] * x[b][r];
       o[b] *= in * a.scale;
     }
+    if (w == 0 && t1 < n) make_gates(s.gates[(ch + 1) & 1], raw, gate.half, lane);
     __syncthreads();               // the inverses are there
     f32x4 W[4];
 #pragma unroll
@@ -222,40 +389,35 @@ __global__ __launch_bounds__(64 * NW) void forward_kernel(bsg_delta a) {
       W[b] = f32x4{0, 0, 0, 0};
       mma16(W[b], *reinterpret_cast<const f32x4*>(&s.inv[(16 * b + m) * IP + 4 * g]), x[b]);
     }
-    if (a.kept_w) {
-      float* kw = a.kept_w + (eh * chunks + ch) * C * DV + col;
+    if (kw) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) kw[(16 * b + 4 * g + r) * DV] = W[b][r];
+      for (int b = 0; b < 4; ++b) *reinterpret_cast<f32x4*>(kw + (int64_t)ch * C * DV + 256 * b) = W[b];
     }
 #pragma unroll
-    for (int b = 0; b < 4; ++b) W[b] *= beta[b];       // U
+    for (int b = 0; b < 4; ++b) W[b] *= *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);   // U
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+    for (int c = 0; c < 2; ++c) {
+      WideOf<T, 2> uw;
+      split(uw, join(W[2 * c], W[2 * c + 1]));
 #pragma unroll
-      for (int u = 0; u <= b; ++u)
-        mma16(o[b], *reinterpret_cast<const f32x4*>(&s.p[(16 * b + m) * AP + 16 * u + 4 * g]), W[u]);
+      for (int b = 2 * c; b < 4; ++b) mma<T>(o[b], s.p_row(16 * b + m, 32 * c, g), uw);
+    }
+    put_columns<T, VD>(s.v, o, w, lane);
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = 16 * b + 4 * g + r;
-        if (t0 + t < a.steps) row_out<T>(a.out, e, t0 + t, h)[col] = (T)(t < rows ? o[b][r] : 0.0f);
-      }
-#pragma unroll
-    for (int d = 0; d < DT; ++d) S[d] *= s.gates.across;
+    for (int d = 0; d < DT; ++d) S[d] *= gates.across;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       f32x4 u[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) u[i] = W[2 * c + i] * *reinterpret_cast<const f32x4*>(&s.gates.out[16 * (2 * c + i) + 4 * g]);
+      for (int i = 0; i < 2; ++i) u[i] = W[2 * c + i] * *reinterpret_cast<const f32x4*>(&gates.out[16 * (2 * c + i) + 4 * g]);
       WideOf<T, 3> uw;
       split(uw, join(u[0], u[1]));
 #pragma unroll
       for (int d = 0; d < DT; ++d) mma<T>(S[d], load_col(s.k, LD, 32 * c, 16 * d, lane), uw);
     }
+    write_columns<T, VD>(s.v, out.at(t0), out.step, rows, min(C, a.steps - t0), w, lane);
   }
+  for (int t = live * C + tid / DV; t < a.steps; t += NT / DV) out.at(t)[tid % DV] = (T)0.0f;   // padding
   if (a.final_state) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -268,13 +430,13 @@ __global__ __launch_bounds__(64 * NW) void forward_kernel(bsg_delta a) {
 // The gradient of the state, from the last chunk to the first, and with it M and v'.  Every
 // product's columns are value columns, so a wave works on its 16 alone, as in the forward pass.
 template <class T, int DK, int NW>
-__global__ __launch_bounds__(64 * NW) void backward_state_kernel(bsg_delta a) {
-  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW;
-  __shared__ __align__(16) Chunk<T, DK> s;
+__global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void backward_state_kernel(bsg_delta a) {
+  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW, VD = pitch<T>(DV);
+  __shared__ __align__(16) Chunk<T, DK, NW> s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % a.heads_v, e = blockIdx.x / a.heads_v, hk = h / (a.heads_v / a.heads_k);
   const int n = steps_of(a, e), col = 16 * w + m;
-  const int chunks = (a.steps + C - 1) / C;
+  const int chunks = (a.steps + C - 1) / C, live = (n + C - 1) / C;
   const int64_t eh = (int64_t)e * a.heads_v + h;
 
   f32x4 D[DT];
@@ -284,36 +446,47 @@ __global__ __launch_bounds__(64 * NW) void backward_state_kernel(bsg_delta a) {
     for (int r = 0; r < 4; ++r)
       D[d][r] = a.dfinal ? a.dfinal[(eh * DK + 16 * d + 4 * g + r) * DV + col] : 0.0f;
 
-  for (int ch = chunks - 1; ch >= 0; --ch) {
-    const int t0 = ch * C, rows = min(C, n - t0);
-    if (rows <= 0) {
-      for (int i = tid; i < min(C, a.steps - t0) * DV; i += 64 * NW) row_out<T>(a.dv, e, t0 + i / DV, h)[i % DV] = (T)0.0f;
-      continue;
+  Fetch<T, DK, NT> fk, fq;
+  Fetch<T, DV, NT> fv;
+  RawGates raw = {0, 0, 0};
+  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), dout = steps_in<const T>(a.dout, e, h);
+  const Steps<T> dv = steps_in<T>(a.dv, e, h);
+  const GateSteps gate(a, e, h);
+  float *const ws = tiles<NW>(a.work_states, eh * chunks, DT, w, lane), *const wm = tiles<NW>(a.work_w, eh * chunks, 4, w, lane);
+  if (live > 0) {
+    const int t0 = (live - 1) * C;
+    fk.load(k.at(t0), k.step, n - t0, tid);
+    fq.load(q.at(t0), q.step, n - t0, tid);
+    fv.load(dout.at(t0), dout.step, n - t0, tid);
+    if (w == 0) make_gates(s.gates[(live - 1) & 1], load_gates(gate, t0, n - t0, lane), gate.half, lane);
+    clear_above(s, tid);
+  }
+  for (int ch = live - 1; ch >= 0; --ch) {
+    const int t0 = ch * C, rows = min(C, n - t0), t1 = t0 - C;
+    const Gates& gates = s.gates[ch & 1];
+    __syncthreads();               // the chunk after is done with LDS
+    fk.store(s.k, rows, tid);
+    fq.store(s.q, rows, tid);
+    fv.store(s.v, rows, tid);
+    if (t1 >= 0) {
+      fk.load(k.at(t1), k.step, C, tid);
+      fq.load(q.at(t1), q.step, C, tid);
+      fv.load(dout.at(t1), dout.step, C, tid);
+      if (w == 0) raw = load_gates(gate, t1, C, lane);
     }
-    f32x4 go[4];
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = 16 * b + 4 * g + r;
-        go[b][r] = t < rows ? (float)row<T>(a.dout, e, t0 + t, h)[col] : 0.0f;
-      }
     __syncthreads();
-    stage<T, DK, C>(s.k, row<T>(a.k, e, t0, hk), a.k.step, rows, tid, 64 * NW);
-    stage<T, DK, C>(s.q, row<T>(a.q, e, t0, hk), a.q.step, rows, tid, 64 * NW);
-    if (w == 0) read_gates(s.gates, a, e, h, t0, rows, lane);
-    __syncthreads();
-    solve_chunk<T, DK, NW, true>(s, a.scale, lane, w);
+    solve_chunk<T, DK, NW, true>(s, gates, a.scale, lane, w);
 
-    float* ws = a.work_states + (eh * chunks + ch) * DK * DV + col;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) ws[(16 * d + 4 * g + r) * DV] = D[d][r];
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(ws + (int64_t)ch * DK * DV + 256 * d) = D[d];
 
-    f32x4 x[4];
+    f32x4 x[4], go[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
+    for (int b = 0; b < 4; ++b) {
+      x[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) go[b][r] = (float)s.v[(16 * b + 4 * g + r) * VD + col];
+    }
 #pragma unroll
     for (int c = 0; c < DK / 32; ++c) {
       WideOf<T, 3> dw;
@@ -322,14 +495,14 @@ __global__ __launch_bounds__(64 * NW) void backward_state_kernel(bsg_delta a) {
       for (int b = 0; b < 4; ++b) mma<T>(x[b], load_tile(s.k + (16 * b + m) * LD, 32 * c, g), dw);
     }
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      x[b] *= *reinterpret_cast<const f32x4*>(&s.gates.out[16 * b + 4 * g]);
+    for (int b = 0; b < 4; ++b) x[b] *= *reinterpret_cast<const f32x4*>(&gates.out[16 * b + 4 * g]);
 #pragma unroll
-      for (int u = b; u < 4; ++u) {
-        const float* p = &s.p[(16 * u + 4 * g) * AP + 16 * b + m];
-        mma16(x[b], f32x4{p[0], p[AP], p[2 * AP], p[3 * AP]}, go[u]);
-      }
+    for (int c = 0; c < 2; ++c) {
+      const Frag<T> gf = round_frag<T>(join(go[2 * c], go[2 * c + 1]));   // as it was read
+#pragma unroll
+      for (int b = 0; b < 2 * c + 2; ++b) mma<T>(x[b], s.p_col(16 * b, 32 * c, lane), gf);
     }
+    if (w == 0 && t1 >= 0) make_gates(s.gates[(ch + 1) & 1], raw, gate.half, lane);
     __syncthreads();               // the inverses are there
     f32x4 M[4];
 #pragma unroll
@@ -343,22 +516,20 @@ __global__ __launch_bounds__(64 * NW) void backward_state_kernel(bsg_delta a) {
       M[b] = f32x4{0, 0, 0, 0};
       mma16(M[b], f32x4{p[0], p[IP], p[2 * IP], p[3 * IP]}, x[b]);
     }
-    float* wm = a.work_w + (eh * chunks + ch) * C * DV + col;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const f32x4 beta = *reinterpret_cast<const f32x4*>(&s.gates.beta[16 * b + 4 * g]);
-      const f32x4 in = *reinterpret_cast<const f32x4*>(&s.gates.in[16 * b + 4 * g]);
+      *reinterpret_cast<f32x4*>(wm + (int64_t)ch * C * DV + 256 * b) = M[b];
+      M[b] *= *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);
+    }
+    put_columns<T, VD>(s.v, M, w, lane);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = 16 * b + 4 * g + r;
-        wm[t * DV] = M[b][r];
-        if (t0 + t < a.steps) row_out<T>(a.dv, e, t0 + t, h)[col] = (T)(t < rows ? beta[r] * M[b][r] : 0.0f);
-      }
-      M[b] *= beta * in * -1.0f;
+    for (int b = 0; b < 4; ++b) {
+      const f32x4 in = *reinterpret_cast<const f32x4*>(&gates.in[16 * b + 4 * g]);
+      M[b] *= -in;
       go[b] *= in * a.scale;
     }
 #pragma unroll
-    for (int d = 0; d < DT; ++d) D[d] *= s.gates.across;
+    for (int d = 0; d < DT; ++d) D[d] *= gates.across;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       WideOf<T, 3> lw, ow;
@@ -370,7 +541,9 @@ __global__ __launch_bounds__(64 * NW) void backward_state_kernel(bsg_delta a) {
         mma<T>(D[d], load_col(s.q, LD, 32 * c, 16 * d, lane), ow);
       }
     }
+    write_columns<T, VD>(s.v, dv.at(t0), dv.step, rows, min(C, a.steps - t0), w, lane);
   }
+  for (int t = live * C + tid / DV; t < a.steps; t += NT / DV) dv.at(t)[tid % DV] = (T)0.0f;   // padding
   if (a.dstate) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -383,20 +556,24 @@ __global__ __launch_bounds__(64 * NW) void backward_state_kernel(bsg_delta a) {
 // q', k', beta', g' of one chunk, env and key head, all chunks side by side: a wave owns 16 steps.
 // The matrices o'.w and m.w are needed by rows (for q', kr') and by columns (for kw'); both are
 // computed, each in the layout in which it is the B operand of what follows, which costs less than
-// a turn through LDS.  The value dimension is walked in slices of 32, the value heads that share
+// a turn through LDS, by different waves.  The value dimension is walked in slices of 32, the value heads that share
 // the key head one after the other, their q' and k' added up in registers.
 constexpr int SL = 32;
 template <class T, int R>
 struct WideRows {                  // an R x SL tile of fp32 values as operand parts of type T
   static constexpr int n = Parts<T, 2>::n, LD = pitch<T>(SL);
   T p[n][R * LD];
-  __device__ __forceinline__ void put(int r, int c, const f32x4& x) {
-    f32x4 rest = x;
+  // lane l's part of D tile d (rows) of column block b
+  __device__ __forceinline__ void put(int d, int b, int l, f32x4 x) {
+    T* at = &p[0][(16 * d + 4 * (l >> 4)) * LD + 16 * b + (l & 15)];
 #pragma unroll
-    for (int i = 0; i < n; ++i) {
-      store4(&p[i][r * LD + c], rest);
-      if (i + 1 < n) rest -= widen(*reinterpret_cast<const Half<T>*>(&p[i][r * LD + c]));
-    }
+    for (int i = 0; i < n; ++i, at += R * LD)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const T z = (T)x[r];
+        at[r * LD] = z;
+        x[r] -= (float)z;
+      }
   }
   __device__ __forceinline__ Wide<T, n> get(int r, int g) const {
     Wide<T, n> w;
@@ -414,174 +591,234 @@ template <class T, int N> __device__ __forceinline__ f32x8 whole(const Wide<T, N
 
 template <class T, int DK>
 struct Inside {
-  T k[C * pitch<T>(DK)], q[C * pitch<T>(DK)], go[C * pitch<T>(SL)];
-  WideRows<T, C> w, mu;
-  WideRows<T, DK> st, ds;
+  T k[C * pitch<T>(DK)], q[C * pitch<T>(DK)];
+  union {
+    struct {
+      T go[C * pitch<T>(SL)];
+      WideRows<T, C> w, mu;
+      WideRows<T, DK> st, ds;
+    };
+    float kw[C * (DK + 4)];        // at the end: kw', on its way to the waves that hold kr'
+  };
   Gates gates;
-  float dc[C], part[8];
+  float dc[2][C], part[8];
 };
 
-template <class T, int DK>
-__global__ __launch_bounds__(256) void backward_chunk_kernel(bsg_delta a) {
-  constexpr int LD = pitch<T>(DK), DT = DK / 16, GL = pitch<T>(SL);
+// Eight waves: 0..3 hold the 16 steps of tile w as they read the state (q', kr'), 4..7 those of tile
+// w - 4 as they write it (kw').
+template <class T, int DK, bool SHARED>
+__global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
+  constexpr int LD = pitch<T>(DK), DT = DK / 16, GL = pitch<T>(SL), NT = 512;
+  constexpr int NS = DK * SL / 4 / NT;           // f32x4 of a state's slice to a thread
+  static_assert(C * SL / 4 == NT, "one f32x4 of W and of M to a thread");
   __shared__ __align__(16) Inside<T, DK> s;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), tile = w & 3;
+  const bool reader = w < 4;
+  const bsg_delta& a = arguments();
   const int chunks = (a.steps + C - 1) / C, group = a.heads_v / a.heads_k, DV = a.dim_v;
+  const float scale = a.scale;
+  const bool half = a.gate_dtype == BSG_BF16;
   const int ch = blockIdx.x % chunks, ehk = blockIdx.x / chunks, hk = ehk % a.heads_k, e = ehk / a.heads_k;
   const int n = steps_of(a, e), t0 = ch * C, rows = min(C, n - t0), all = min(C, a.steps - t0);
-  const int own = 16 * w + m;
-  if (rows <= 0) {
-    for (int i = tid; i < all * DK; i += 256) {
-      row_out<T>(a.dq, e, t0 + i / DK, hk)[i % DK] = (T)0.0f;
-      row_out<T>(a.dk, e, t0 + i / DK, hk)[i % DK] = (T)0.0f;
-    }
-    for (int i = tid; i < all * group; i += 256) {
+  const int own = 16 * tile + m;
+  if (rows <= 0) {                 // padding
+    const Steps<T> dqs = steps_in<T>(a.dq, e, hk), dks = steps_in<T>(a.dk, e, hk);
+    for (int i = tid; i < all * DK; i += NT) dqs.at(t0 + i / DK)[i % DK] = dks.at(t0 + i / DK)[i % DK] = (T)0.0f;
+    for (int i = tid; i < all * group; i += NT) {
       gate_out(a.dg, a.gate_dtype, e, t0 + i / group, hk * group + i % group, 0.0f);
       gate_out(a.dbeta, a.gate_dtype, e, t0 + i / group, hk * group + i % group, 0.0f);
     }
     return;
   }
-  stage<T, DK, C>(s.k, row<T>(a.k, e, t0, hk), a.k.step, rows, tid, 256);
-  stage<T, DK, C>(s.q, row<T>(a.q, e, t0, hk), a.q.step, rows, tid, 256);
-  f32x4 dq[DT], dk[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d) dq[d] = dk[d] = f32x4{0, 0, 0, 0};
+  stage<T, DK, C>(s.k, row<T>(a.k, e, t0, hk), a.k.step, rows, tid, NT);
+  stage<T, DK, C>(s.q, row<T>(a.q, e, t0, hk), a.q.step, rows, tid, NT);
 
-  for (int h = hk * group; h < (hk + 1) * group; ++h) {
+  // one slice on its way from memory: the next is loaded while this one is computed
+  constexpr int GV = Vec<T>::n, GROW = SL / GV;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 fgo;
+  f32x4 fw, fm, fs[NS > 0 ? NS : 1], fd[NS > 0 ? NS : 1];
+  const auto fetch = [&](int h, int v0) {
+    const bsg_delta& a = arguments();
     const int64_t ehc = ((int64_t)e * a.heads_v + h) * chunks + ch;
-    f32x4 OWt[4], MWt[4], OW[4], MW[4], X1[DT], X2[DT], X3[DT];
+    const int64_t at = ehc * C * DV + v0 * C + tid * 4, as = ehc * DK * DV + v0 * DK + tid * 4;
+    if (tid < C * GROW)
+      fgo = *reinterpret_cast<const u32x4*>(row<T>(a.dout, e, t0 + min(tid / GROW, rows - 1), h) + v0 + tid % GROW * GV);
+    fw = *reinterpret_cast<const f32x4*>(a.kept_w + at);
+    fm = *reinterpret_cast<const f32x4*>(a.work_w + at);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) OWt[b] = MWt[b] = OW[b] = MW[b] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < (NS > 0 ? NS : 1); ++i)
+      if (NS > 0 || tid < DK * SL / 4) {
+        fs[i] = *reinterpret_cast<const f32x4*>(a.kept_states + as + i * 4 * NT);
+        fd[i] = *reinterpret_cast<const f32x4*>(a.work_states + as + i * 4 * NT);
+      }
+  };
+  fetch(hk * group, 0);
+
+  f32x4 sum1[DT], sum2[DT];        // over the value heads: q', kr' (readers); kw' (writers)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) X1[d] = X2[d] = X3[d] = f32x4{0, 0, 0, 0};
+  for (int d = 0; d < DT; ++d) sum1[d] = sum2[d] = f32x4{0, 0, 0, 0};
+  for (int h = hk * group, last = SHARED ? h + group - 1 : h; h <= last; ++h) {
+    // readers: o'.w and m.w by rows j, q' and kr'; writers: by rows i, kw'
+    f32x4 ow[4], mw[4], X1[DT], X2[DT];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) ow[b] = mw[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int d = 0; d < DT; ++d) X1[d] = X2[d] = f32x4{0, 0, 0, 0};
     float dbeta = 0.0f, sd = 0.0f;
+    RawGates raw = {0, 0, 0};
+    if (w == 0) raw = load_gates(GateSteps(arguments(), e, h), t0, rows, lane);
     for (int v0 = 0; v0 < DV; v0 += SL) {
-      __syncthreads();
-      if (v0 == 0 && w == 0) read_gates(s.gates, a, e, h, t0, rows, lane);
-      stage<T, SL, C>(s.go, row<T>(a.dout, e, t0, h) + v0, a.dout.step, rows, tid, 256);
-      for (int i = tid; i < C * SL / 4; i += 256) {
-        const int r = i / (SL / 4), c = i % (SL / 4) * 4;
-        const int64_t at = (ehc * C + r) * DV + v0 + c;
-        s.w.put(r, c, *reinterpret_cast<const f32x4*>(a.kept_w + at));
-        s.mu.put(r, c, *reinterpret_cast<const f32x4*>(a.work_w + at));
-      }
-      for (int i = tid; i < DK * SL / 4; i += 256) {
-        const int r = i / (SL / 4), c = i % (SL / 4) * 4;
-        const int64_t at = (ehc * DK + r) * DV + v0 + c;
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.kept_states + at);
-        const f32x4 y = *reinterpret_cast<const f32x4*>(a.work_states + at);
-        s.st.put(r, c, x);
-        s.ds.put(r, c, y);
+      __syncthreads();             // the slice before is done with
+      if (v0 == 0 && w == 0) make_gates(s.gates, raw, half, lane);
+      if (tid < C * GROW)
+        *reinterpret_cast<u32x4*>(&s.go[tid / GROW * GL + tid % GROW * GV]) = tid / GROW < rows ? fgo : u32x4{0, 0, 0, 0};
+      s.w.put(tid / 64 % 4, tid / 256, lane, fw);
+      s.mu.put(tid / 64 % 4, tid / 256, lane, fm);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sd = fmaf(x[j], y[j], sd);
-      }
-      __syncthreads();
-      const Frag<T> go = load_run(s.go + own * GL, 0, g);
-      const WideOf<T, 2> wf = s.w.get(own, g), mf = s.mu.get(own, g);
-      const f32x8 wx = whole(wf), mx = whole(mf);
+      for (int i = 0; i < (NS > 0 ? NS : 1); ++i)
+        if (NS > 0 || tid < DK * SL / 4) {
+          const int at = (tid + i * NT) / 64;
+          s.st.put(at % DT, at / DT, lane, fs[i]);
+          s.ds.put(at % DT, at / DT, lane, fd[i]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dbeta = fmaf(wx[j], mx[j], dbeta);
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        if (b <= w) {
-          const WideOf<T, 2> x = s.w.get(16 * b + m, g);
-          mma<T>(OWt[b], x, go);
-          mma<T>(MWt[b], x, mf);
+          for (int j = 0; j < 4; ++j) sd = fmaf(fs[i][j], fd[i][j], sd);
         }
-        if (b >= w) {
-          mma<T>(OW[b], load_run(s.go + (16 * b + m) * GL, 0, g), wf);
-          mma<T>(MW[b], s.mu.get(16 * b + m, g), wf);
-        }
-      }
+      if (v0 + SL < DV) fetch(h, v0 + SL);
+      else if (SHARED && h < last) fetch(h + 1, 0);
+      __syncthreads();
+      const WideOf<T, 2> wf = s.w.get(own, g);
+      if (reader) {
+        const Frag<T> go = load_run(s.go + own * GL, 0, g);
+        const WideOf<T, 2> mf = s.mu.get(own, g);
+        const f32x8 wx = whole(wf), mx = whole(mf);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const WideOf<T, 2> x = s.st.get(16 * d + m, g), y = s.ds.get(16 * d + m, g);
-        mma<T>(X1[d], x, go);
-        mma<T>(X2[d], x, mf);
-        mma<T>(X3[d], y, wf);
+        for (int j = 0; j < 8; ++j) dbeta = fmaf(wx[j], mx[j], dbeta);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (b <= tile) {
+            const WideOf<T, 2> x = s.w.get(16 * b + m, g);
+            mma<T>(ow[b], x, go);
+            mma<T>(mw[b], x, mf);
+          }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const WideOf<T, 2> x = s.st.get(16 * d + m, g);
+          mma<T>(X1[d], x, go);
+          mma<T>(X2[d], x, mf);
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (b >= tile) {
+            mma<T>(ow[b], load_run(s.go + (16 * b + m) * GL, 0, g), wf);
+            mma<T>(mw[b], s.mu.get(16 * b + m, g), wf);
+          }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) mma<T>(X1[d], s.ds.get(16 * d + m, g), wf);
       }
     }
     // scale by the gates of the wave's own step (its lane) and add the chunk's own terms
     const Gates& G = s.gates;
-    const float bi = G.beta[own], in = G.in[own], out = G.out[own];
-    float y = 0.0f;
+    const float bi = G.beta[own], in = G.in[own], out = G.out[own], across = G.across;
+    float y = 0.0f, dc = 0.0f;
+    if (reader) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        X1[d] *= scale * in;
+        X2[d] *= -bi * in;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (2 * c <= tile) {       // rows j of tiles 2c, 2c + 1 against the own step i
+          f32x4 f1[2], f2[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int j = 16 * (2 * c + u) + 4 * g + r;
+              const float f = j <= own ? decay(G, own, j) * G.beta[j] : 0.0f;
+              f1[u][r] = scale * f * ow[2 * c + u][r];
+              f2[u][r] = j < own ? -bi * f * mw[2 * c + u][r] : 0.0f;
+            }
+          WideOf<T, 2> w1, w2;
+          split(w1, join(f1[0], f1[1]));
+          split(w2, join(f2[0], f2[1]));
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const Frag<T> k = load_col(s.k, LD, 32 * c, 16 * d, lane);
+            mma<T>(X1[d], k, w1);
+            mma<T>(X2[d], k, w2);
+          }
+        }
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const f32x4 k = widen(*reinterpret_cast<const Half<T>*>(&s.k[own * LD + 16 * d + 4 * g]));
+        X1[d] *= out * bi;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y = fmaf(k[r], X1[d][r], y);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (2 * c + 1 >= tile) {   // rows i of tiles 2c, 2c + 1 against the own step j
+          f32x4 f1[2], f2[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int i = 16 * (2 * c + u) + 4 * g + r;
+              const float f = i >= own ? decay(G, i, own) * bi : 0.0f;
+              f1[u][r] = scale * f * ow[2 * c + u][r];
+              f2[u][r] = i > own ? -G.beta[i] * f * mw[2 * c + u][r] : 0.0f;
+            }
+          WideOf<T, 2> w1, w2;
+          split(w1, join(f1[0], f1[1]));
+          split(w2, join(f2[0], f2[1]));
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            mma<T>(X1[d], load_col(s.q, LD, 32 * c, 16 * d, lane), w1);
+            mma<T>(X1[d], load_col(s.k, LD, 32 * c, 16 * d, lane), w2);
+          }
+        }
+    }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const f32x4 k = widen(*reinterpret_cast<const Half<T>*>(&s.k[own * LD + 16 * d + 4 * g]));
-      X1[d] *= a.scale * in;
-      X2[d] *= -bi * in;
-      X3[d] *= out * bi;
+      if (reader) {
+        const f32x4 q = widen(*reinterpret_cast<const Half<T>*>(&s.q[own * LD + 16 * d + 4 * g]));
 #pragma unroll
-      for (int r = 0; r < 4; ++r) y = fmaf(k[r], X3[d][r], y);
-    }
+        for (int r = 0; r < 4; ++r) dc = fmaf(q[r], X1[d][r], fmaf(k[r], X2[d][r], dc));
+      } else {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      if (2 * c <= w) {            // rows j of tiles 2c, 2c + 1 against the own step i
-        f32x4 f1[2], f2[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = 16 * (2 * c + u) + 4 * g + r;
-            const float f = j <= own ? decay(G, own, j) * G.beta[j] : 0.0f;
-            f1[u][r] = a.scale * f * OWt[2 * c + u][r];
-            f2[u][r] = j < own ? -bi * f * MWt[2 * c + u][r] : 0.0f;
-          }
-        WideOf<T, 2> w1, w2;
-        split(w1, join(f1[0], f1[1]));
-        split(w2, join(f2[0], f2[1]));
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const Frag<T> k = load_col(s.k, LD, 32 * c, 16 * d, lane);
-          mma<T>(X1[d], k, w1);
-          mma<T>(X2[d], k, w2);
-        }
+        for (int r = 0; r < 4; ++r) dc = fmaf(-k[r], X1[d][r], dc);
       }
-      if (2 * c + 1 >= w) {        // rows i of tiles 2c, 2c + 1 against the own step j
-        f32x4 f1[2], f2[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = 16 * (2 * c + u) + 4 * g + r;
-            const float f = i >= own ? decay(G, i, own) * bi : 0.0f;
-            f1[u][r] = a.scale * f * OW[2 * c + u][r];
-            f2[u][r] = i > own ? -G.beta[i] * f * MW[2 * c + u][r] : 0.0f;
-          }
-        WideOf<T, 2> w1, w2;
-        split(w1, join(f1[0], f1[1]));
-        split(w2, join(f2[0], f2[1]));
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          mma<T>(X3[d], load_col(s.q, LD, 32 * c, 16 * d, lane), w1);
-          mma<T>(X3[d], load_col(s.k, LD, 32 * c, 16 * d, lane), w2);
-        }
+      if (SHARED) {
+        sum1[d] += X1[d];
+        sum2[d] += X2[d];
+      } else {
+        sum1[d] = X1[d];
+        sum2[d] = X2[d];
       }
-    }
-    float dc = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const f32x4 k = widen(*reinterpret_cast<const Half<T>*>(&s.k[own * LD + 16 * d + 4 * g]));
-      const f32x4 q = widen(*reinterpret_cast<const Half<T>*>(&s.q[own * LD + 16 * d + 4 * g]));
-#pragma unroll
-      for (int r = 0; r < 4; ++r) dc = fmaf(q[r], X1[d][r], fmaf(k[r], X2[d][r] - X3[d][r], dc));
-      dq[d] += X1[d];
-      dk[d] += X2[d] + X3[d];
     }
     dc = sum_groups(dc);
     dbeta = sum_groups(dbeta);
     // the chunk's last step: across <S, D> + sum_j k_j.(out_j D u_j)
-    y += G.across * sd;
+    y += across * sd;
 #pragma unroll
     for (int d = 32; d >= 1; d /= 2) y += __shfl_xor(y, d);
-    if (g == 0) s.dc[own] = dc;
+    if (g == 0) s.dc[reader ? 0 : 1][own] = dc;
     if (lane == 0) s.part[w] = y;
-    if (g == 0 && t0 + own < a.steps)
+    const bsg_delta& a = arguments();
+    if (reader && g == 0 && t0 + own < a.steps)
       gate_out(a.dbeta, a.gate_dtype, e, t0 + own, h, own < rows ? dbeta : 0.0f);
     __syncthreads();
     if (w == 0) {
-      float x = s.dc[lane];
-      if (lane == 63) x += (s.part[0] + s.part[1]) + (s.part[2] + s.part[3]);
+      float x = s.dc[0][lane] + s.dc[1][lane];
+      if (lane == 63)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x += s.part[i];
       const int ep = G.episode[lane], before = lane ? G.episode[lane - 1] : 0;
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) {
@@ -594,12 +831,19 @@ __global__ __launch_bounds__(256) void backward_chunk_kernel(bsg_delta a) {
         gate_out(a.dg, a.gate_dtype, e, t0 + lane, h, lane < rows && ep == before ? x : 0.0f);
     }
   }
-  if (t0 + own >= a.steps) return;
-  T *oq = row_out<T>(a.dq, e, t0 + own, hk), *ok = row_out<T>(a.dk, e, t0 + own, hk);
+  if (!reader) {                   // the last slice is done with: every wave has passed the barrier above
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&s.kw[own * (DK + 4) + 16 * d + 4 * g]) = sum1[d];
+  }
+  __syncthreads();
+  const bsg_delta& b = arguments();
+  if (!reader || t0 + own >= b.steps) return;
+  T *oq = row_out<T>(b.dq, e, t0 + own, hk), *ok = row_out<T>(b.dk, e, t0 + own, hk);
 #pragma unroll
   for (int d = 0; d < DT; ++d) {
-    store4(oq + 16 * d + 4 * g, own < rows ? dq[d] : f32x4{0, 0, 0, 0});
-    store4(ok + 16 * d + 4 * g, own < rows ? dk[d] : f32x4{0, 0, 0, 0});
+    const f32x4 kw = *reinterpret_cast<const f32x4*>(&s.kw[own * (DK + 4) + 16 * d + 4 * g]);
+    store4(oq + 16 * d + 4 * g, own < rows ? sum1[d] : f32x4{0, 0, 0, 0});
+    store4(ok + 16 * d + 4 * g, own < rows ? sum2[d] + kw : f32x4{0, 0, 0, 0});
   }
 }
 
@@ -672,7 +916,9 @@ hipError_t run(const bsg_delta& a, int what, hipStream_t st) {
   } else {
     backward_state_kernel<T, DK, NW><<<dim3(rows), dim3(64 * NW), 0, st>>>(a);
     const int chunks = (a.steps + C - 1) / C;
-    backward_chunk_kernel<T, DK><<<dim3((unsigned)(a.num_envs * a.heads_k * chunks)), dim3(256), 0, st>>>(a);
+    const dim3 grid((unsigned)(a.num_envs * a.heads_k * chunks));
+    if (a.heads_v > a.heads_k) backward_chunk_kernel<T, DK, true><<<grid, dim3(512), 0, st>>>(a);
+    else backward_chunk_kernel<T, DK, false><<<grid, dim3(512), 0, st>>>(a);
   }
   return hipGetLastError();
 }

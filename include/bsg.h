@@ -387,9 +387,9 @@ typedef struct bsg_delta {
   const float* state;        /* [num_envs][heads_v][dim_k][dim_v] before the first step; NULL = 0 */
   float* final_state;        /* the same after the last step; NULL = not wanted */
   /* kept by the forward pass for the backward pass (both NULL: not kept), with
-   * chunks = ceil(steps / BSG_DELTA_CHUNK) */
-  float* kept_states;        /* [num_envs][heads_v][chunks][dim_k][dim_v] */
-  float* kept_w;             /* [num_envs][heads_v][chunks * BSG_DELTA_CHUNK][dim_v] */
+   * chunks = ceil(steps / BSG_DELTA_CHUNK); the order of their values is the library's */
+  float* kept_states;        /* [num_envs][heads_v][chunks] x dim_k x dim_v */
+  float* kept_w;             /* [num_envs][heads_v][chunks] x BSG_DELTA_CHUNK x dim_v */
   /* backward only */
   bsg_rows dout, dq, dk, dv, dg, dbeta;
   const float* dfinal;       /* gradient of final_state; NULL = 0 */
