@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("BSG_LIBRARY", os.path.join(_HERE, "_lib", "libbsg.so"))
@@ -97,7 +98,7 @@ EXPORTED_SYMBOLS = (
     "bsg_comm_all_reduce", "bsg_set_params", "bsg_trajectory_bytes", "bsg_set_trajectory",
     "bsg_trajectory_info", "bsg_delta_forward", "bsg_delta_backward", "bsg_delta_step",
     "bsg_attention_forward", "bsg_attention_backward", "bsg_attention_step_bytes",
-    "bsg_attention_step",
+    "bsg_attention_step", "bsg_attention_parts_bytes",
 )
 TRAJ_SYNC = 1                # include/bsg.h BSG_TRAJ_SYNC
 # include/bsg.h BSG_MP_*: MergeEnv-v0's module constants (merge_env.py:13-46), in this order,
@@ -127,6 +128,7 @@ class BsgSacActor(C.Structure):
 
 F32, BF16 = 0, 1             # include/bsg.h BSG_F32, BSG_BF16
 DELTA_CHUNK = 64             # BSG_DELTA_CHUNK
+ATTENTION_TILE = 64          # steps up to which bsg_attention.out_rest is not wanted
 
 
 class BsgRows(C.Structure):
@@ -146,14 +148,21 @@ class BsgDelta(C.Structure):
         [(n, C.c_void_p) for n in ("dfinal", "dstate", "work_states", "work_w")]
 
 
+class BsgDeltaAct(C.Structure):
+    """include/bsg.h bsg_delta_act."""
+    _fields_ = [(n, C.c_int32) for n in ("num_envs", "heads_k", "heads_v", "dim_k", "dim_v", "dtype", "gate_dtype")] + \
+        [("scale", C.c_float)] + [(n, BsgRows) for n in ("q", "k", "v", "g", "beta", "out")] + \
+        [("first", C.c_void_p), ("first_env", C.c_int64), ("state", C.c_void_p)]
+
+
 class BsgAttention(C.Structure):
     """include/bsg.h bsg_attention."""
     _fields_ = [(n, C.c_int32) for n in ("num_envs", "steps", "heads_q", "heads_k", "dim", "dtype", "window")] + \
         [("scale", C.c_float), ("softcap", C.c_float), ("reserved", C.c_int32)] + \
         [(n, BsgRows) for n in ("q", "k", "v", "out")] + \
         [("slopes", C.c_void_p), ("first", C.c_void_p), ("first_env", C.c_int64), ("first_step", C.c_int64)] + \
-        [(n, C.c_void_p) for n in ("lengths", "begins", "lse")] + \
-        [(n, BsgRows) for n in ("dout", "dq", "dk", "dv")] + [("delta", C.c_void_p)]
+        [(n, C.c_void_p) for n in ("lengths", "begins", "lse", "out_rest")] + \
+        [(n, BsgRows) for n in ("dout", "dq", "dk", "dv")] + [("delta", C.c_void_p), ("parts", C.c_void_p)]
 
 
 class BsgAttentionAct(C.Structure):
@@ -163,6 +172,21 @@ class BsgAttentionAct(C.Structure):
         [(n, BsgRows) for n in ("q", "k", "v", "out")] + \
         [("slopes", C.c_void_p), ("first", C.c_void_p), ("first_env", C.c_int64)] + \
         [(n, C.c_void_p) for n in ("steps", "k_cache", "v_cache", "work")] + [("work_bytes", C.c_int64)]
+
+
+def packer(cls):
+    """struct.Struct of a C structure's fields in their order (nested ones in place; pointers as
+    integers, 0 = NULL): building an argument block from a list of numbers costs a tenth of setting
+    the ctypes fields one by one, which an acting step of a few envs would feel."""
+    codes = {C.c_int32: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "Q"}
+
+    def flat(c):
+        return "".join(codes[t] if t in codes else flat(t) for _, t in c._fields_)
+
+    p = struct.Struct("@" + flat(cls))
+    if p.size != C.sizeof(cls):
+        raise AssertionError(f"{cls.__name__}: packed size {p.size} != {C.sizeof(cls)}")
+    return p.pack
 
 
 _lib = None
@@ -253,13 +277,14 @@ def load_library(path: str | None = None):
     lib.bsg_step_gather.restype = C.c_int32
     lib.bsg_step_gather.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                     C.c_void_p, C.c_int32, C.c_void_p]
-    for fn, args in (("bsg_delta_forward", BsgDelta), ("bsg_delta_backward", BsgDelta),
-                     ("bsg_delta_step", BsgDelta), ("bsg_attention_forward", BsgAttention),
-                     ("bsg_attention_backward", BsgAttention), ("bsg_attention_step", BsgAttentionAct)):
+    # argument blocks: ctypes structures by reference, or their packed bytes
+    for fn in ("bsg_delta_forward", "bsg_delta_backward", "bsg_delta_step", "bsg_attention_forward",
+               "bsg_attention_backward", "bsg_attention_step"):
         getattr(lib, fn).restype = C.c_int32
-        getattr(lib, fn).argtypes = [C.POINTER(args), C.c_void_p]
-    lib.bsg_attention_step_bytes.restype = C.c_int64
-    lib.bsg_attention_step_bytes.argtypes = [C.POINTER(BsgAttentionAct)]
+        getattr(lib, fn).argtypes = [C.c_void_p, C.c_void_p]
+    for fn in ("bsg_attention_parts_bytes", "bsg_attention_step_bytes"):
+        getattr(lib, fn).restype = C.c_int64
+        getattr(lib, fn).argtypes = [C.c_void_p]
     if lib.bsg_abi_version() != ABI_VERSION:
         raise BsgError(f"libbsg ABI {lib.bsg_abi_version()} != expected {ABI_VERSION}")
     if path is None:

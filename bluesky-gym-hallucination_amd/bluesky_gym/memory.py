@@ -53,31 +53,38 @@ def _tensors(who, ref, **named):
             raise ValueError(f"{who}: {n} is on {x.device}, q is on {dev}")
 
 
-def _shape(who, name, x, *shape, dtype=None):
-    if tuple(x.shape) != shape:
+def _shape(who, name, x, shape, dtypes=None):
+    if x.shape != shape:
         raise ValueError(f"{who}: {name} has shape {tuple(x.shape)}, expected {shape}")
-    if dtype is not None and x.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
-        raise ValueError(f"{who}: {name} has dtype {x.dtype}, expected {dtype}")
+    if dtypes is not None and x.dtype not in dtypes:
+        raise ValueError(f"{who}: {name} has dtype {x.dtype}, expected one of {dtypes}")
 
 
-def _heads(who, q, k, v, dims, rank):
+_FP32, _INT32, _FLAGS = (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
+
+
+def _heads(who, q, k, v, rank, **dims):
     """Type and shape of q, k, v; returns the dtype code."""
     if q.dim() != rank or k.dim() != rank or v.dim() != rank:
         raise ValueError(f"{who}: q, k and v must have {rank} axes")
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    t = q.dtype
+    if t not in _DTYPES or k.dtype != t or v.dtype != t:
         raise ValueError(f"{who}: q, k and v must share one dtype, float32 or bfloat16 "
-                         f"(got {q.dtype}, {k.dtype}, {v.dtype})")
+                         f"(got {t}, {k.dtype}, {v.dtype})")
     for n, d in dims.items():
         if d not in HEAD_DIMS:
             raise ValueError(f"{who}: {n} must be 32, 64 or 128 (got {d})")
-    return _DTYPES[q.dtype]
+    return _DTYPES[t]
 
 
 def _aligned(x):
     """Whether the kernels can read or write x's rows in 16-byte vectors."""
+    if x.data_ptr() % 16:
+        return False
+    if x.is_contiguous():
+        return True
     b = x.element_size()
-    return x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and \
-        all(n == 1 or s * b % 16 == 0 for n, s in zip(x.shape[:-1], x.stride()[:-1]))
+    return x.stride(-1) == 1 and all(n == 1 or s * b % 16 == 0 for n, s in zip(x.shape[:-1], x.stride()[:-1]))
 
 
 def _vectors(x):
@@ -90,36 +97,43 @@ def _empty_like(x):
     return y if _aligned(y) else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
-def _rows(x, heads_last=False):
-    """x [E, T, H(, D)] (rollouts) or [E, H(, D)] (a step) as a bsg_rows."""
-    s = [0 if n == 1 else st for n, st in zip(x.shape, x.stride())]
-    if not heads_last:
-        s = s[:-1]
-    return nat.BsgRows(x.data_ptr(), s[0], s[1] if len(s) == 3 else 0, s[-1])
+def _rows(x):
+    """A bsg_rows: a rollout's [E, T, H, D], a gate's [E, T, H].  The strides of axes of one are
+    not looked at."""
+    E, T, H = x.shape[:3]
+    s = x.stride()
+    return x.data_ptr(), s[0] if E > 1 else 0, s[1] if T > 1 else 0, s[2] if H > 1 else 0
+
+
+def _step_rows(x):
+    """A bsg_rows of one step: [E, H, D] or a gate's [E, H]."""
+    s = x.stride()
+    return x.data_ptr(), s[0] if x.shape[0] > 1 else 0, 0, s[1] if x.shape[1] > 1 else 0
+
+
+_NO_ROWS = (0, 0, 0, 0)
 
 
 def _ptr(x):
-    return None if x is None else x.data_ptr()
+    return 0 if x is None else x.data_ptr()
 
 
-def _flags(who, first, shape):
-    if first is not None:
-        _shape(who, "first", first, *shape, dtype=(torch.bool, torch.uint8))
+def _flag_rows(first):
+    return (0, 0, 0) if first is None else (first.data_ptr(), first.stride(0), first.stride(1))
 
 
 def _numbers(who, scale, dim, softcap=0.0, window=0):
-    scale = dim ** -0.5 if scale is None else float(scale)
     if not 0.0 <= softcap < float("inf"):
         raise ValueError(f"{who}: softcap must be finite and >= 0 (0 = none), got {softcap}")
     if window < 0:
         raise ValueError(f"{who}: window must be >= 0 (0 = the whole episode), got {window}")
-    return scale
+    return dim ** -0.5 if scale is None else float(scale)
 
 
 def _slopes(who, slopes, heads):
     if slopes is None:
         return None
-    _shape(who, "slopes", slopes, heads, dtype=torch.float32)
+    _shape(who, "slopes", slopes, (heads,), _FP32)
     if slopes.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{who}: slopes are constants; they get no gradient")
     return slopes.contiguous()
@@ -130,39 +144,51 @@ def _no_grad(who, *xs):
         raise ValueError(f"{who} has no gradient: act under torch.no_grad()")
 
 
-def _call(fn, args, dev):
-    with torch.cuda.device(dev):               # the launch goes to the tensors' device
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        nat.check(getattr(nat.load_library(), fn)(C.byref(args), stream), fn)
+def _out(who, out, like):
+    if out is None:
+        return _empty_like(like)
+    _shape(who, "out", out, like.shape, (like.dtype,))
+    if not _aligned(out):
+        raise ValueError(f"{who}: out must have contiguous, 16-byte aligned rows")
+    return out
+
+
+def _call(fn, block, dev):
+    """The launch goes to the tensors' device, on its current stream."""
+    call = getattr(nat.load_library(), fn)
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        nat.check(call(block, stream), fn)
+    else:
+        with torch.cuda.device(dev):
+            nat.check(call(block, stream), fn)
 
 
 # ---- the gated delta rule -------------------------------------------------------------------
 
-def _delta_args(dtype, scale, q, k, v, g, beta, first):
-    a = nat.BsgDelta()
-    a.num_envs, a.steps = (v.shape[0], v.shape[1]) if v.dim() == 4 else (v.shape[0], 1)
-    a.heads_k, a.heads_v, a.dim_k, a.dim_v = q.shape[-2], v.shape[-2], q.shape[-1], v.shape[-1]
-    a.dtype, a.gate_dtype, a.scale = dtype, _DTYPES[g.dtype], scale
-    a.q, a.k, a.v = _rows(q), _rows(k), _rows(v)
-    a.g, a.beta = _rows(g, True), _rows(beta, True)
-    if first is not None:
-        a.first, a.first_env = first.data_ptr(), first.stride(0)
-        a.first_step = first.stride(1) if first.dim() == 2 else 0
-    return a
+_pack_delta, _pack_delta_act = nat.packer(nat.BsgDelta), nat.packer(nat.BsgDeltaAct)
+
+
+def _delta_inputs(dtype, scale, q, k, v, g, beta, out, first, lengths):
+    """The leading fields of bsg_delta, up to lengths."""
+    E, T, H, Dv = v.shape
+    return (E, T, q.shape[2], H, q.shape[3], Dv, dtype, _DTYPES[g.dtype], scale, 0, *_rows(q), *_rows(k),
+            *_rows(v), *_rows(g), *_rows(beta), *out, *_flag_rows(first), _ptr(lengths))
 
 
 def _delta_check(who, q, k, v, g, beta, state, first, lead):
-    E, Hk, Dk, H, Dv = q.shape[0], q.shape[-2], q.shape[-1], v.shape[-2], v.shape[-1]
-    _shape(who, "k", k, *lead, Hk, Dk)
-    _shape(who, "q", q, *lead, Hk, Dk)
+    Hk, Dk = q.shape[-2:]
+    H, Dv = v.shape[-2:]
+    _shape(who, "q", q, (*lead, Hk, Dk))
+    _shape(who, "k", k, (*lead, Hk, Dk))
     if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"{who}: {H} value heads do not share {Hk} key heads evenly")
-    gates = (torch.float32, q.dtype)
-    _shape(who, "g", g, *lead, H, dtype=gates)
-    _shape(who, "beta", beta, *lead, H, dtype=(g.dtype,))
+    _shape(who, "g", g, (*lead, H), (torch.float32, q.dtype))
+    _shape(who, "beta", beta, (*lead, H), (g.dtype,))
     if state is not None:
-        _shape(who, "state", state, E, H, Dk, Dv, dtype=torch.float32)
-    _flags(who, first, lead)
+        _shape(who, "state", state, (lead[0], H, Dk, Dv), _FP32)
+    if first is not None:
+        _shape(who, "first", first, lead, _FLAGS)
 
 
 class _DeltaRule(torch.autograd.Function):
@@ -172,19 +198,18 @@ class _DeltaRule(torch.autograd.Function):
         state = None if state is None else state.contiguous()
         E, T, H, Dv = v.shape
         Dk, dev = q.shape[-1], v.device
-        a = _delta_args(dtype, scale, q, k, v, g, beta, first)
         out = _empty_like(v)
         final = torch.empty((E, H, Dk, Dv), dtype=torch.float32, device=dev)
-        a.out, a.lengths, a.state, a.final_state = _rows(out), _ptr(lengths), _ptr(state), final.data_ptr()
-        kept = ()
+        states = w = None
         if keep:
             n = -(-T // nat.DELTA_CHUNK)
-            kept = (torch.empty((E, H, n, Dk, Dv), dtype=torch.float32, device=dev),
-                    torch.empty((E, H, n * nat.DELTA_CHUNK, Dv), dtype=torch.float32, device=dev))
-            a.kept_states, a.kept_w = kept[0].data_ptr(), kept[1].data_ptr()
-        _call("bsg_delta_forward", a, dev)
+            states = torch.empty((E, H, n, Dk, Dv), dtype=torch.float32, device=dev)
+            w = torch.empty((E, H, n * nat.DELTA_CHUNK, Dv), dtype=torch.float32, device=dev)
+        _call("bsg_delta_forward", _pack_delta(
+            *_delta_inputs(dtype, scale, q, k, v, g, beta, _rows(out), first, lengths), _ptr(state), final.data_ptr(),
+            _ptr(states), _ptr(w), *_NO_ROWS * 6, 0, 0, 0, 0), dev)
         if keep:
-            ctx.save_for_backward(q, k, v, g, beta, first, lengths, *kept)
+            ctx.save_for_backward(q, k, v, g, beta, first, lengths, states, w)
             ctx.rest = scale, dtype
             ctx.set_materialize_grads(False)
         return out, final
@@ -202,12 +227,10 @@ class _DeltaRule(torch.autograd.Function):
         if ctx.needs_input_grad[5]:
             dstate = torch.empty((v.shape[0], v.shape[2], q.shape[-1], v.shape[-1]), dtype=torch.float32, device=v.device)
         ws, ww = torch.empty_like(states), torch.empty_like(w)
-        a = _delta_args(dtype, scale, q, k, v, g, beta, first)
-        a.lengths, a.kept_states, a.kept_w = _ptr(lengths), states.data_ptr(), w.data_ptr()
-        a.dout, a.dq, a.dk, a.dv = _rows(dout), _rows(dq), _rows(dk), _rows(dv)
-        a.dg, a.dbeta = _rows(dg, True), _rows(db, True)
-        a.dfinal, a.dstate, a.work_states, a.work_w = _ptr(dfinal), _ptr(dstate), ws.data_ptr(), ww.data_ptr()
-        _call("bsg_delta_backward", a, v.device)
+        _call("bsg_delta_backward", _pack_delta(
+            *_delta_inputs(dtype, scale, q, k, v, g, beta, _NO_ROWS, first, lengths), 0, 0, states.data_ptr(),
+            w.data_ptr(), *_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv), *_rows(dg), *_rows(db), _ptr(dfinal),
+            _ptr(dstate), ws.data_ptr(), ww.data_ptr()), v.device)
         return dq, dk, dv, dg, db, dstate, None, None, None, None, None
 
 
@@ -224,11 +247,11 @@ def gated_delta_rule(q, k, v, g, beta, state=None, first=None, lengths=None, *, 
     Returns ``out`` [E, T, Hv, Dv] and the state after the last step, fp32.  Differentiable once in
     q, k, v, g, beta and state."""
     who = "gated_delta_rule"
-    dtype = _heads(who, q, k, v, {"Dk": q.shape[-1], "Dv": v.shape[-1]}, 4)
+    dtype = _heads(who, q, k, v, 4, Dk=q.shape[-1], Dv=v.shape[-1])
     E, T, H, Dv = v.shape
     _delta_check(who, q, k, v, g, beta, state, first, (E, T))
     if lengths is not None:
-        _shape(who, "lengths", lengths, E, dtype=torch.int32)
+        _shape(who, "lengths", lengths, (E,), _INT32)
         lengths = lengths.contiguous()
     _tensors(who, q, k=k, v=v, g=g, beta=beta, state=state, first=first, lengths=lengths)
     scale = _numbers(who, scale, q.shape[-1])
@@ -248,8 +271,8 @@ def gated_delta_step(q, k, v, g, beta, state, first=None, *, scale=None, out=Non
     holds).  Returns out [E, Hv, Dv] (``out=`` to write into a given tensor).  No gradient: a
     learner replays the steps through :func:`gated_delta_rule`."""
     who = "gated_delta_step"
-    dtype = _heads(who, q, k, v, {"Dk": q.shape[-1], "Dv": v.shape[-1]}, 3)
-    E = v.shape[0]
+    dtype = _heads(who, q, k, v, 3, Dk=q.shape[-1], Dv=v.shape[-1])
+    E, H, Dv = v.shape
     if state is None:
         raise ValueError(f"{who}: state is updated in place and must be given")
     _delta_check(who, q, k, v, g, beta, state, first, (E,))
@@ -261,64 +284,62 @@ def gated_delta_step(q, k, v, g, beta, state, first=None, *, scale=None, out=Non
     if E == 0:
         return out
     q, k, v = _vectors(q), _vectors(k), _vectors(v)
-    a = _delta_args(dtype, _numbers(who, scale, q.shape[-1]), q, k, v, g, beta, first)
-    a.out, a.state, a.final_state = _rows(out), state.data_ptr(), state.data_ptr()
-    _call("bsg_delta_step", a, v.device)
-    return out
-
-
-def _out(who, out, like):
-    if out is None:
-        return _empty_like(like)
-    _shape(who, "out", out, *like.shape, dtype=like.dtype)
-    if not _aligned(out):
-        raise ValueError(f"{who}: out must have contiguous, 16-byte aligned rows")
+    _call("bsg_delta_step", _pack_delta_act(
+        E, q.shape[1], H, q.shape[2], Dv, dtype, _DTYPES[g.dtype], _numbers(who, scale, q.shape[2]), *_step_rows(q),
+        *_step_rows(k), *_step_rows(v), *_step_rows(g), *_step_rows(beta), *_step_rows(out), _ptr(first),
+        0 if first is None else first.stride(0), state.data_ptr()), v.device)
     return out
 
 
 # ---- attention over the episode -------------------------------------------------------------
 
-def _attention_args(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, out):
-    a = nat.BsgAttention()
-    a.num_envs, a.steps, a.heads_q, a.dim = q.shape
-    a.heads_k, a.dtype = k.shape[2], dtype
-    a.scale, a.softcap, a.window = numbers
-    a.q, a.k, a.v, a.out = _rows(q), _rows(k), _rows(v), _rows(out)
-    a.slopes, a.lengths, a.begins, a.lse = _ptr(slopes), _ptr(lengths), _ptr(begins), _ptr(lse)
-    if first is not None:
-        a.first, a.first_env, a.first_step = first.data_ptr(), first.stride(0), first.stride(1)
-    return a
+_pack_attention, _pack_attention_act = nat.packer(nat.BsgAttention), nat.packer(nat.BsgAttentionAct)
+
+
+def _attention_block(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, rest, out, grads=_NO_ROWS * 4, delta=0, parts=0):
+    E, T, H, D = q.shape
+    scale, softcap, window = numbers
+    return _pack_attention(E, T, H, k.shape[2], D, dtype, window, scale, softcap, 0, *_rows(q), *_rows(k), *_rows(v),
+                           *_rows(out), _ptr(slopes), *_flag_rows(first), _ptr(lengths), _ptr(begins), _ptr(lse),
+                           _ptr(rest), *grads, delta, parts)
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, first, lengths, slopes, numbers, dtype, keep):
         q, k, v = _vectors(q), _vectors(k), _vectors(v)
-        E, T, H, _ = q.shape
+        E, T, H, D = q.shape
         dev = q.device
         out = _empty_like(q)
-        begins = lse = None
+        begins = lse = rest = None
         if first is not None or numbers[2] > 0:
             begins = torch.empty((E, T), dtype=torch.int32, device=dev)
         if keep:
             lse = torch.empty((E, H, T), dtype=torch.float32, device=dev)
+            if dtype == nat.BF16 and T > nat.ATTENTION_TILE:
+                rest = torch.empty((E, H, T, D), dtype=q.dtype, device=dev)
         _call("bsg_attention_forward",
-              _attention_args(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, out), dev)
+              _attention_block(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, rest, out), dev)
         if keep:
-            ctx.save_for_backward(q, k, v, first, lengths, slopes, begins, lse, out)
+            ctx.save_for_backward(q, k, v, slopes, first, lengths, begins, lse, rest, out)   # as _attention_block takes them
             ctx.rest = numbers, dtype
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, first, lengths, slopes, begins, lse, out = ctx.saved_tensors
+        *saved, out = ctx.saved_tensors
+        q, k, v, lse = saved[0], saved[1], saved[2], saved[7]
         numbers, dtype = ctx.rest
         dout = _vectors(dout)
         dq, dk, dv, delta = _empty_like(q), _empty_like(k), _empty_like(v), torch.empty_like(lse)
-        a = _attention_args(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, out)
-        a.dout, a.dq, a.dk, a.dv, a.delta = _rows(dout), _rows(dq), _rows(dk), _rows(dv), delta.data_ptr()
-        _call("bsg_attention_backward", a, q.device)
+        grads = (*_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv))
+        block, parts = _attention_block(dtype, numbers, *saved, out, grads, delta.data_ptr()), None
+        need = nat.load_library().bsg_attention_parts_bytes(block)
+        if need > 0:
+            parts = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+            block = _attention_block(dtype, numbers, *saved, out, grads, delta.data_ptr(), parts.data_ptr())
+        _call("bsg_attention_backward", block, q.device)
         return dq, dk, dv, None, None, None, None, None, None
 
 
@@ -333,16 +354,17 @@ def episode_attention(q, k, v, first=None, lengths=None, *, scale=None, softcap=
     the number of last steps that are seen (0 = all of the episode).  scale: D ** -0.5 by default.
     Returns out [E, T, Hq, D].  Differentiable once in q, k and v."""
     who = "episode_attention"
-    dtype = _heads(who, q, k, v, {"the head dim": q.shape[-1]}, 4)
+    dtype = _heads(who, q, k, v, 4, D=q.shape[-1])
     E, T, H, D = q.shape
     Hk = k.shape[2]
-    _shape(who, "k", k, E, T, Hk, D)
-    _shape(who, "v", v, E, T, Hk, D)
+    _shape(who, "k", k, (E, T, Hk, D))
+    _shape(who, "v", v, (E, T, Hk, D))
     if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"{who}: {H} query heads do not share {Hk} key heads evenly")
-    _flags(who, first, (E, T))
+    if first is not None:
+        _shape(who, "first", first, (E, T), _FLAGS)
     if lengths is not None:
-        _shape(who, "lengths", lengths, E, dtype=torch.int32)
+        _shape(who, "lengths", lengths, (E,), _INT32)
         lengths = lengths.contiguous()
     _tensors(who, q, k=k, v=v, first=first, lengths=lengths, slopes=slopes)
     scale = _numbers(who, scale, D, softcap, window)
@@ -366,20 +388,21 @@ def episode_attention_step(q, k, v, k_cache, v_cache, steps, first=None, *, scal
     holds no step of the episode is not looked at, whatever it holds.  Returns out [E, Hq, D]
     (``out=`` to write into a given tensor).  No gradient."""
     who = "episode_attention_step"
-    dtype = _heads(who, q, k, v, {"the head dim": q.shape[-1]}, 3)
+    dtype = _heads(who, q, k, v, 3, D=q.shape[-1])
     E, H, D = q.shape
     Hk = k.shape[1]
-    _shape(who, "k", k, E, Hk, D)
-    _shape(who, "v", v, E, Hk, D)
+    _shape(who, "k", k, (E, Hk, D))
+    _shape(who, "v", v, (E, Hk, D))
     if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"{who}: {H} query heads do not share {Hk} key heads evenly")
     if k_cache.dim() != 4 or k_cache.shape[2] < 1:
         raise ValueError(f"{who}: k_cache must be [E, Hkv, slots, D] with at least one slot")
     S = k_cache.shape[2]
-    _shape(who, "k_cache", k_cache, E, Hk, S, D, dtype=q.dtype)
-    _shape(who, "v_cache", v_cache, E, Hk, S, D, dtype=q.dtype)
-    _shape(who, "steps", steps, E, dtype=torch.int32)
-    _flags(who, first, (E,))
+    _shape(who, "k_cache", k_cache, (E, Hk, S, D), (q.dtype,))
+    _shape(who, "v_cache", v_cache, (E, Hk, S, D), (q.dtype,))
+    _shape(who, "steps", steps, (E,), _INT32)
+    if first is not None:
+        _shape(who, "first", first, (E,), _FLAGS)
     _tensors(who, q, k=k, v=v, k_cache=k_cache, v_cache=v_cache, steps=steps, first=first, slopes=slopes, out=out)
     _no_grad(who, q, k, v, k_cache, v_cache)
     for n, x in (("k_cache", k_cache), ("v_cache", v_cache), ("steps", steps)):
@@ -391,16 +414,13 @@ def episode_attention_step(q, k, v, k_cache, v_cache, steps, first=None, *, scal
     if E == 0:
         return out
     q, k, v = _vectors(q), _vectors(k), _vectors(v)
-    a = nat.BsgAttentionAct()
-    a.num_envs, a.slots, a.heads_q, a.heads_k, a.dim, a.dtype = E, S, H, Hk, D, dtype
-    a.scale, a.softcap = scale, softcap
-    a.q, a.k, a.v, a.out = _rows(q), _rows(k), _rows(v), _rows(out)
-    a.slopes, a.steps, a.k_cache, a.v_cache = _ptr(slopes), steps.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    if first is not None:
-        a.first, a.first_env = first.data_ptr(), first.stride(0)
-    need = nat.load_library().bsg_attention_step_bytes(C.byref(a))
+    fields = (E, S, H, Hk, D, dtype, scale, softcap, *_step_rows(q), *_step_rows(k), *_step_rows(v), *_step_rows(out),
+              _ptr(slopes), _ptr(first), 0 if first is None else first.stride(0), steps.data_ptr(), k_cache.data_ptr(),
+              v_cache.data_ptr())
+    block, work = _pack_attention_act(*fields, 0, 0), None
+    need = nat.load_library().bsg_attention_step_bytes(block)
     if need > 0:
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.work, a.work_bytes = work.data_ptr(), need
-    _call("bsg_attention_step", a, q.device)
+        block = _pack_attention_act(*fields, work.data_ptr(), need)
+    _call("bsg_attention_step", block, q.device)
     return out

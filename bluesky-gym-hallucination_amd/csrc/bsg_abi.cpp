@@ -812,6 +812,8 @@ int32_t bsg_policy_sac(const bsg_sac_actor* w, const float* obs, int32_t num_env
   return BSG_OK;
 }
 
+}  // extern "C"
+
 // ---- memory operators ----------------------------------------------------------------------
 namespace {
 
@@ -824,21 +826,20 @@ bool vector_rows(const bsg_rows& r, int dtype) {
          !((r.step * bytes) & 15) && !((r.head * bytes) & 15);
 }
 
-int32_t check_delta(const bsg_delta* a, const char* who) {
-  if (!a) return fail(BSG_E_INVALID_ARG, "%s: null arguments", who);
-  if (a->num_envs < 0 || a->steps < 0) return fail(BSG_E_INVALID_ARG, "%s: num_envs or steps < 0", who);
+template <class A> int32_t check_delta(const A* a, int steps, const char* who) {
+  if (a->num_envs < 0 || steps < 0) return fail(BSG_E_INVALID_ARG, "%s: num_envs or steps < 0", who);
   if (a->heads_k < 1 || a->heads_v < 1 || a->heads_v % a->heads_k)
     return fail(BSG_E_INVALID_ARG, "%s: heads_v (%d) must be a multiple of heads_k (%d)", who, a->heads_v, a->heads_k);
   if (!head_dim(a->dim_k) || !head_dim(a->dim_v))
     return fail(BSG_E_INVALID_ARG, "%s: dim_k and dim_v must be 32, 64 or 128 (got %d, %d)", who, a->dim_k, a->dim_v);
   if ((a->dtype != BSG_F32 && a->dtype != BSG_BF16) || (a->gate_dtype != BSG_F32 && a->gate_dtype != a->dtype))
     return fail(BSG_E_INVALID_ARG, "%s: dtype must be BSG_F32 or BSG_BF16, gate_dtype that or BSG_F32", who);
-  const int64_t chunks = ((int64_t)a->steps + BSG_DELTA_CHUNK - 1) / BSG_DELTA_CHUNK;
+  const int64_t chunks = ((int64_t)steps + BSG_DELTA_CHUNK - 1) / BSG_DELTA_CHUNK;
   if ((int64_t)a->num_envs * a->heads_v * (chunks > 4 ? chunks : 4) > 0x7fffffffll)
     return fail(BSG_E_INVALID_ARG, "%s: num_envs x heads_v x chunks exceeds 2^31 - 1", who);
   return BSG_OK;
 }
-bool delta_inputs(const bsg_delta* a) {
+template <class A> bool delta_inputs(const A* a) {
   return vector_rows(a->q, a->dtype) && vector_rows(a->k, a->dtype) && vector_rows(a->v, a->dtype) && a->g.p && a->beta.p;
 }
 
@@ -860,6 +861,7 @@ int32_t check_attention(const bsg_attention* a, const char* who) {
   if (a->num_envs == 0 || a->steps == 0) return BSG_OK;
   if (!vector_rows(a->q, a->dtype) || !vector_rows(a->k, a->dtype) || !vector_rows(a->v, a->dtype) || !vector_rows(a->out, a->dtype))
     return fail(BSG_E_INVALID_ARG, "%s: q, k, v and out must be there, with 16-byte aligned rows", who);
+  if (reinterpret_cast<uintptr_t>(a->out_rest) & 15) return fail(BSG_E_INVALID_ARG, "%s: out_rest must be 16-byte aligned", who);
   if ((a->first || a->window > 0) && !a->begins)
     return fail(BSG_E_INVALID_ARG, "%s: first or window without begins", who);
   return BSG_OK;
@@ -873,8 +875,11 @@ bsg_attention with_begins(const bsg_attention* a) {
 
 }  // namespace
 
+extern "C" {
+
 int32_t bsg_delta_forward(const bsg_delta* a, void* stream) {
-  if (int32_t r = check_delta(a, "bsg_delta_forward")) return r;
+  if (!a) return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: null arguments");
+  if (int32_t r = check_delta(a, a->steps, "bsg_delta_forward")) return r;
   if (a->num_envs == 0) return BSG_OK;
   if (a->steps > 0 && (!delta_inputs(a) || !vector_rows(a->out, a->dtype)))
     return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: q, k, v, g, beta and out must be there, with 16-byte aligned rows of q, k, v and out");
@@ -885,7 +890,8 @@ int32_t bsg_delta_forward(const bsg_delta* a, void* stream) {
 }
 
 int32_t bsg_delta_backward(const bsg_delta* a, void* stream) {
-  if (int32_t r = check_delta(a, "bsg_delta_backward")) return r;
+  if (!a) return fail(BSG_E_INVALID_ARG, "bsg_delta_backward: null arguments");
+  if (int32_t r = check_delta(a, a->steps, "bsg_delta_backward")) return r;
   if (a->num_envs == 0 || a->steps == 0) return BSG_OK;
   if (!delta_inputs(a) || !vector_rows(a->dout, a->dtype) || !vector_rows(a->dq, a->dtype) || !vector_rows(a->dk, a->dtype) ||
       !vector_rows(a->dv, a->dtype) || !a->dg.p || !a->dbeta.p)
@@ -898,12 +904,12 @@ int32_t bsg_delta_backward(const bsg_delta* a, void* stream) {
   return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_delta_backward launch");
 }
 
-int32_t bsg_delta_step(const bsg_delta* a, void* stream) {
-  if (int32_t r = check_delta(a, "bsg_delta_step")) return r;
-  if (a->steps != 1 || a->lengths) return fail(BSG_E_INVALID_ARG, "bsg_delta_step: steps must be 1 and lengths NULL");
+int32_t bsg_delta_step(const bsg_delta_act* a, void* stream) {
+  if (!a) return fail(BSG_E_INVALID_ARG, "bsg_delta_step: null arguments");
+  if (int32_t r = check_delta(a, 1, "bsg_delta_step")) return r;
   if (a->num_envs == 0) return BSG_OK;
-  if (!a->state || a->state != a->final_state || (reinterpret_cast<uintptr_t>(a->state) & 15))
-    return fail(BSG_E_INVALID_ARG, "bsg_delta_step: state and final_state must be one 16-byte aligned buffer");
+  if (!a->state || (reinterpret_cast<uintptr_t>(a->state) & 15))
+    return fail(BSG_E_INVALID_ARG, "bsg_delta_step: state must be there, 16-byte aligned");
   if (!delta_inputs(a) || !vector_rows(a->out, a->dtype))
     return fail(BSG_E_INVALID_ARG, "bsg_delta_step: q, k, v, g, beta and out must be there, with 16-byte aligned rows of q, k, v and out");
   hipError_t e = bsg::launch_delta_step(*a, static_cast<hipStream_t>(stream));
@@ -917,12 +923,22 @@ int32_t bsg_attention_forward(const bsg_attention* a, void* stream) {
   return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_attention_forward launch");
 }
 
+int64_t bsg_attention_parts_bytes(const bsg_attention* a) {
+  if (int32_t r = check_attention(a, "bsg_attention_parts_bytes")) return r;
+  if (!bsg::attention_wants_parts(*a)) return 0;
+  return (int64_t)a->num_envs * a->heads_q * a->steps * 2 * a->dim * 4;
+}
+
 int32_t bsg_attention_backward(const bsg_attention* a, void* stream) {
   if (int32_t r = check_attention(a, "bsg_attention_backward")) return r;
   if (a->num_envs == 0 || a->steps == 0) return BSG_OK;
   if (!vector_rows(a->dout, a->dtype) || !vector_rows(a->dq, a->dtype) || !vector_rows(a->dk, a->dtype) || !vector_rows(a->dv, a->dtype))
     return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: dout, dq, dk and dv must be there, with 16-byte aligned rows");
   if (!a->lse || !a->delta) return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: null lse or delta");
+  if (a->dtype == BSG_BF16 && a->steps > 64 && !a->out_rest)
+    return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: null out_rest");
+  if (bsg::attention_wants_parts(*a) != (a->parts != nullptr) || (reinterpret_cast<uintptr_t>(a->parts) & 15))
+    return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: parts must be there, 16-byte aligned, where bsg_attention_parts_bytes is not 0");
   hipError_t e = bsg::launch_attention(with_begins(a), true, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_attention_backward launch");
 }

@@ -14,6 +14,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "bsg_internal.h"
 #include "bsg_mma.h"
 
@@ -51,16 +53,20 @@ __device__ __forceinline__ Score score_of(float scale, float softcap, const floa
   s.slope = slopes ? slopes[h] * LOG2E : 0.0f;
   return s;
 }
-// the score in base 2; with a cap, `y` is the tanh (its derivative is 1 - y^2)
-template <class T, bool CAP>
-__device__ __forceinline__ float score(const Score& s, float dot, int ago, float& y) {
-  float x = dot * s.mul;
+// The score in base 2, `ago` steps back; with a cap, `y` is the tanh (its derivative is 1 - y^2).
+template <class T, bool CAP, bool BIAS>
+__device__ __forceinline__ float score(const Score& s, float dot, float ago, float& y) {
   if (CAP) {
-    y = cap_tanh<T>(x);
-    x = y * s.cap;
+    y = cap_tanh<T>(dot * s.mul);
+    const float x = y * s.cap;
+    return BIAS ? fmaf(-s.slope, ago, x) : x;
   }
-  return x - s.slope * (float)ago;
+  return BIAS ? fmaf(dot, s.mul, -s.slope * ago) : dot * s.mul;
 }
+
+// Workgroups go to the eight XCDs in turn; each takes one contiguous eighth of the tiles, so that
+// the tiles of a head, which read the same rows, share an L2.
+__device__ __forceinline__ int swizzled(int b, int all) { return all % 8 ? b : b % 8 * (all / 8) + b / 8; }
 
 // begins[e][t]: one workgroup per env walks its steps, 256 at a time; the last first step at or
 // before t is the highest set bit of the wave's ballot up to its lane, or of an earlier wave's.
@@ -90,269 +96,597 @@ __global__ __launch_bounds__(256) void begins_kernel(const uint8_t* first, int64
 }
 
 // ---- forward -------------------------------------------------------------------------------
-// A workgroup of four waves takes 64 queries of one head, a wave 16 of them, and walks the keys in
-// tiles of 64 staged in LDS.  Scores are computed transposed (keys x queries), so a lane holds one
-// query: its running maximum and sum are in-lane but for two shuffles, and the probabilities lie in
-// registers as the B operand of out^T[dim][query] += V^T[dim][key] P^T[key][query].
-template <class T, int D, bool CAP>
+// A workgroup of four waves takes 64 QW queries of one head, a wave 16 QW of them, and walks the
+// keys in tiles of 64, fetched one tile ahead through registers and shared in LDS.  Scores are
+// computed transposed (keys x queries), so a lane holds one query: its running maximum and sum are
+// in-lane but for two lane swaps, and the probabilities lie in registers as the B operand of
+// out^T[dim][query] += V^T[dim][key] P^T[key][query].  QW = 2 halves the LDS reads per product;
+// fp32 operands, which the matrix cores take at a sixteenth of the rate, have no use for it.
+// Masks are only applied in tiles that an edge crosses.
+template <class T, int D, int QW, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) void forward_kernel(bsg_attention a) {
-  constexpr int LD = pitch<T>(D);
+  constexpr int LD = pitch<T>(D), KT = TILE / 16;
   __shared__ __align__(16) T sK[TILE * LD];
   __shared__ __align__(16) T sV[TILE * LD];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int nt = (a.steps + TILE - 1) / TILE;
-  const int q0 = (nt - 1 - (int)(blockIdx.x % nt)) * TILE;       // the longest ranges first
-  const int eh = blockIdx.x / nt, h = eh % a.heads_q, e = eh / a.heads_q;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW), id = swizzled(blockIdx.x, gridDim.x);
+  const int q0 = (nt - 1 - id % nt) * TILE * QW;                 // the longest ranges first
+  const int eh = id / nt, h = eh % a.heads_q, e = eh / a.heads_q;
   const int hk = h / (a.heads_q / a.heads_k);
   const int n = a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
-  const int qi = q0 + 16 * w + m;
-  const bool live = qi < n;
+  const int qw = q0 + 16 * QW * w;                               // the wave's first query
   const Score sc = score_of(a.scale, a.softcap, a.slopes, h);
-
-  Frag<T> qf[D / 32];
-#pragma unroll
-  for (int s = 0; s < D / 32; ++s) qf[s] = Frag<T>{};
-  if (live) {
-    const T* qr = row<T>(a.q, e, qi, h);
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) qf[s] = load_run(qr, 32 * s, g);
-  }
   const int32_t* begins = a.begins ? a.begins + (int64_t)e * a.steps : nullptr;
-  const int begin = begins && live ? begins[qi] : 0;
-  const int kend = min(q0 + TILE, n);
-  const int kbeg = begins && q0 < n ? begins[q0] / TILE * TILE : 0;
 
-  f32x4 o[D / 16];
+  Frag<T> qf[QW][D / 32];
+  int qi[QW], begin[QW];
 #pragma unroll
-  for (int d = 0; d < D / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
-  float mx = -INFINITY, sum = 0.0f;
+  for (int i = 0; i < QW; ++i) {
+    qi[i] = qw + 16 * i + m;
+    // a query behind the last step reads the last one's row and is not written
+    const int at = max(min(qi[i], n - 1), 0);
+    const T* qr = row<T>(a.q, e, at, h);
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) qf[i][s] = load_run(qr, 32 * s, g);
+    begin[i] = begins ? begins[at] : 0;
+  }
+  const int kend = min(q0 + TILE * QW, n), kbeg = begins && q0 < n ? begins[q0] / TILE * TILE : 0;
+  // what the wave's queries see: from the first one's begin; all of them from the last one's
+  const int see_any = begins && qw < n ? begins[qw] : 0;
+  const int see_all = begins && qw < n ? begins[min(qw + 16 * QW, n) - 1] : 0;
+
+  f32x4 o[QW][D / 16];
+  float mx[QW], sum[QW];
+#pragma unroll
+  for (int i = 0; i < QW; ++i) {
+    mx[i] = -INFINITY;
+    sum[i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) o[i][d] = f32x4{0, 0, 0, 0};
+  }
+  const auto tile = [&](int k0, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    f32x4 s[QW][KT];
+    float top[QW];
+#pragma unroll
+    for (int i = 0; i < QW; ++i) top[i] = mx[i];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      if (MASK && k0 + 16 * t > qw + 16 * QW - 1) {              // behind the wave's last query
+#pragma unroll
+        for (int i = 0; i < QW; ++i) s[i][t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i < QW; ++i) s[i][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const Frag<T> kf = load_run(sK + (16 * t + m) * LD, 32 * c, g);
+#pragma unroll
+        for (int i = 0; i < QW; ++i) mma(s[i][t], kf, qf[i][c]);
+      }
+#pragma unroll
+      for (int i = 0; i < QW; ++i) {
+        const float ago = (float)(qi[i] - k0 - 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float y;
+          s[i][t][r] = score<T, CAP, BIAS>(sc, s[i][t][r], ago - (float)(16 * t + r), y);
+          if (MASK) {
+            const int j = k0 + 16 * t + 4 * g + r;
+            s[i][t][r] = j <= qi[i] && j >= begin[i] ? s[i][t][r] : -INFINITY;
+          }
+          top[i] = fmaxf(top[i], s[i][t][r]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < QW; ++i) {
+      top[i] = max_groups(top[i]);
+      // a query whose keys all lie in other tiles has nothing yet: exp2(-inf - 0) = 0
+      const float base = MASK && top[i] == -INFINITY ? 0.0f : top[i];
+      const float old = __builtin_amdgcn_exp2f(mx[i] - base);
+      mx[i] = top[i];
+      sum[i] *= old;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[i][t][r] = __builtin_amdgcn_exp2f(s[i][t][r] - base);
+          sum[i] += s[i][t][r];
+        }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) o[i][d] *= old;
+    }
+#pragma unroll
+    for (int c = 0; c < KT / 2; ++c) {
+      if (MASK && k0 + 32 * c > qw + 16 * QW - 1) continue;
+      Frag<T> pf[QW];
+#pragma unroll
+      for (int i = 0; i < QW; ++i) pf[i] = round_frag<T>(join(s[i][2 * c], s[i][2 * c + 1]));
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const Frag<T> vf = load_col(sV, LD, 32 * c, 16 * d, lane);
+#pragma unroll
+        for (int i = 0; i < QW; ++i) mma(o[i][d], vf, pf[i]);
+      }
+    }
+  };
+  Fetch<T, TILE, D, 256> fk, fv;
+  if (kbeg < kend) {
+    fk.load(row<T>(a.k, e, kbeg, hk), a.k.step, kend - kbeg, tid);
+    fv.load(row<T>(a.v, e, kbeg, hk), a.v.step, kend - kbeg, tid);
+  }
   for (int k0 = kbeg; k0 < kend; k0 += TILE) {
     __syncthreads();
-    stage<T, D, TILE>(sK, row<T>(a.k, e, k0, hk), a.k.step, kend - k0, tid, 256);
-    stage<T, D, TILE>(sV, row<T>(a.v, e, k0, hk), a.v.step, kend - k0, tid, 256);
+    fk.store(sK, kend - k0, tid);
+    fv.store(sV, kend - k0, tid);
+    if (k0 + TILE < kend) {
+      fk.load(row<T>(a.k, e, k0 + TILE, hk), a.k.step, kend - k0 - TILE, tid);
+      fv.load(row<T>(a.v, e, k0 + TILE, hk), a.v.step, kend - k0 - TILE, tid);
+    }
     __syncthreads();
-    f32x4 s[TILE / 16];
-    float top = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < TILE / 16; ++t) {
-      s[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) mma(s[t], load_run(sK + (16 * t + m) * LD, 32 * c, g), qf[c]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = k0 + 16 * t + 4 * g + r;
-        float y;
-        const float x = score<T, CAP>(sc, s[t][r], qi - j, y);
-        s[t][r] = live && j <= qi && j >= begin ? x : -INFINITY;
-        top = fmaxf(top, s[t][r]);
-      }
-    }
-    top = fmaxf(mx, max_groups(top));
-    // a query whose keys all lie in other tiles has nothing yet: exp2(-inf - 0) = 0
-    const float base = top == -INFINITY ? 0.0f : top;
-    const float old = __builtin_amdgcn_exp2f(mx - base);
-    mx = top;
-    float part = 0.0f;
-#pragma unroll
-    for (int t = 0; t < TILE / 16; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - base);
-        part += s[t][r];
-      }
-    sum = sum * old + part;
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) o[d] *= old;
-#pragma unroll
-    for (int c = 0; c < TILE / 32; ++c) {
-      const Frag<T> pf = round_frag<T>(join(s[2 * c], s[2 * c + 1]));
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) mma(o[d], load_col(sV, LD, 32 * c, 16 * d, lane), pf);
-    }
+    if (qw >= n || k0 > qw + 16 * QW - 1 || k0 + TILE <= see_any) continue;
+    if (k0 + TILE - 1 <= qw && k0 >= see_all) tile(k0, std::false_type());
+    else tile(k0, std::true_type());
   }
-  sum = sum_groups(sum);
-  if (qi >= a.steps) return;
-  const float inv = live ? 1.0f / sum : 0.0f;
-  T* out = row_out<T>(a.out, e, qi, h);
 #pragma unroll
-  for (int d = 0; d < D / 16; ++d) store4(out + 16 * d + 4 * g, live ? o[d] * inv : f32x4{0, 0, 0, 0});
-  if (a.lse && g == 0 && live) a.lse[((int64_t)e * a.heads_q + h) * a.steps + qi] = mx + log2f(sum);
+  for (int i = 0; i < QW; ++i) {
+    if (qi[i] >= a.steps) continue;
+    const bool live = qi[i] < n;
+    const float all = sum_groups(sum[i]), inv = live ? 1.0f / all : 0.0f;
+    const int64_t at = ((int64_t)e * a.heads_q + h) * a.steps + qi[i];
+    T* out = row_out<T>(a.out, e, qi[i], h);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      const f32x4 x = live ? o[i][d] * inv : f32x4{0, 0, 0, 0};
+      store4(out + 16 * d + 4 * g, x);
+      if (sizeof(T) == 2 && a.out_rest) {                        // what the rounding left
+        f32x4 rest;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) rest[r] = x[r] - (float)(T)x[r];
+        store4(static_cast<T*>(a.out_rest) + at * D + 16 * d + 4 * g, rest);
+      }
+    }
+    if (a.lse && g == 0 && live) a.lse[at] = mx[i] + log2f(all);
+  }
 }
 
 // ---- backward ------------------------------------------------------------------------------
-// dq: as the forward pass, with dp^T = V dout^T next to the scores and dq^T += K^T ds^T.  It also
-// writes delta_i = dout_i.out_i for the pass over keys.
-template <class T, int D, bool CAP>
-__global__ __launch_bounds__(256) void backward_q_kernel(bsg_attention a) {
-  constexpr int LD = pitch<T>(D);
-  __shared__ __align__(16) T sK[TILE * LD];
-  __shared__ __align__(16) T sV[TILE * LD];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int nt = (a.steps + TILE - 1) / TILE;
-  const int q0 = (nt - 1 - (int)(blockIdx.x % nt)) * TILE;
-  const int eh = blockIdx.x / nt, h = eh % a.heads_q, e = eh / a.heads_q;
-  const int hk = h / (a.heads_q / a.heads_k);
-  const int n = a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
-  const int qi = q0 + 16 * w + m;
-  const bool live = qi < n;
-  const Score sc = score_of(a.scale, a.softcap, a.slopes, h);
-  const int64_t at = ((int64_t)e * a.heads_q + h) * a.steps + qi;
-
-  Frag<T> qf[D / 32], df[D / 32];
-  float delta = 0.0f;
+// p and ds of 16 keys (rows 4g + r, from key j0) and a lane's query, or of 16 queries and a lane's
+// key (SWAP: i0 and `at` change places).
+template <class T, bool CAP, bool BIAS>
+__device__ __forceinline__ void p_and_ds(const Score& sc, float ago, const f32x4& step, const f32x4& lse,
+                                         const f32x4& delta, const f32x4& s, const f32x4& dp, f32x4& p, f32x4& ds) {
 #pragma unroll
-  for (int s = 0; s < D / 32; ++s) qf[s] = df[s] = Frag<T>{};
-  if (live) {
-    const T *qr = row<T>(a.q, e, qi, h), *dr = row<T>(a.dout, e, qi, h), *orow = row<T>(a.out, e, qi, h);
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      qf[s] = load_run(qr, 32 * s, g);
-      df[s] = load_run(dr, 32 * s, g);
-      const f32x8 x = widen(df[s]), y = widen(load_run(orow, 32 * s, g));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) delta = fmaf(x[j], y[j], delta);
-    }
+  for (int r = 0; r < 4; ++r) {
+    float y = 0.0f;
+    const float x = score<T, CAP, BIAS>(sc, s[r], ago + step[r], y);
+    p[r] = __builtin_amdgcn_exp2f(x - lse[r]);
+    ds[r] = p[r] * (dp[r] - delta[r]);
+    if (CAP) ds[r] *= fmaf(-y, y, 1.0f);
   }
-  delta = sum_groups(delta);
-  if (live && g == 0) a.delta[at] = delta;
-  const float lse = live ? a.lse[at] : 0.0f;
-  const int32_t* begins = a.begins ? a.begins + (int64_t)e * a.steps : nullptr;
-  const int begin = begins && live ? begins[qi] : 0;
-  const int kend = min(q0 + TILE, n);
-  const int kbeg = begins && q0 < n ? begins[q0] / TILE * TILE : 0;
-
-  f32x4 dq[D / 16];
-#pragma unroll
-  for (int d = 0; d < D / 16; ++d) dq[d] = f32x4{0, 0, 0, 0};
-  for (int k0 = kbeg; k0 < kend; k0 += TILE) {
-    __syncthreads();
-    stage<T, D, TILE>(sK, row<T>(a.k, e, k0, hk), a.k.step, kend - k0, tid, 256);
-    stage<T, D, TILE>(sV, row<T>(a.v, e, k0, hk), a.v.step, kend - k0, tid, 256);
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < TILE / 32; ++c) {
-      f32x4 ds[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int t = 2 * c + u;
-        f32x4 s = {0, 0, 0, 0}, dp = {0, 0, 0, 0};
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-          mma(s, load_run(sK + (16 * t + m) * LD, 32 * x, g), qf[x]);
-          mma(dp, load_run(sV + (16 * t + m) * LD, 32 * x, g), df[x]);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = k0 + 16 * t + 4 * g + r;
-          float y = 0.0f;
-          const float x = score<T, CAP>(sc, s[r], qi - j, y);
-          const float p = __builtin_amdgcn_exp2f(x - lse);
-          float v = p * (dp[r] - delta);
-          if (CAP) v *= 1.0f - y * y;
-          ds[u][r] = live && j <= qi && j >= begin ? v : 0.0f;
-        }
-      }
-      const Frag<T> f = round_frag<T>(join(ds[0], ds[1]));
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) mma(dq[d], load_col(sK, LD, 32 * c, 16 * d, lane), f);
-    }
-  }
-  if (qi >= a.steps) return;
-  T* out = row_out<T>(a.dq, e, qi, h);
-#pragma unroll
-  for (int d = 0; d < D / 16; ++d) store4(out + 16 * d + 4 * g, live ? dq[d] * a.scale : f32x4{0, 0, 0, 0});
 }
 
-// dk, dv: a wave holds 16 keys and walks the queries that see them, of every query head that
-// shares the key's head, so nothing is added across workgroups.
-template <class T, int D, bool CAP>
-__global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
-  constexpr int LD = pitch<T>(D);
-  __shared__ __align__(16) T sQ[TILE * LD];
-  __shared__ __align__(16) T sD[TILE * LD];
-  __shared__ __align__(16) float sLse[TILE], sDelta[TILE];
-  __shared__ __align__(16) int sBegin[TILE];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int nt = (a.steps + TILE - 1) / TILE;
-  const int k0 = (int)(blockIdx.x % nt) * TILE;                  // the longest ranges first
-  const int eh = blockIdx.x / nt, hk = eh % a.heads_k, e = eh / a.heads_k;
-  const int group = a.heads_q / a.heads_k;
+// Rollouts of one tile (64 steps): one workgroup per env and key head computes all three
+// gradients, rows of each head fetched once.  A wave first holds 16 queries (dq, and delta from
+// the whole row of p and dp, so that the rounded out is not needed), then 16 keys, whose dk and dv
+// it adds up over the query heads that share them.
+template <class T, int D>
+struct Short { T k[TILE * pitch<T>(D)], v[TILE * pitch<T>(D)], q[TILE * pitch<T>(D)], go[TILE * pitch<T>(D)]; float lse[TILE], delta[TILE]; int begin[TILE]; };
+template <class T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) void backward_short_kernel(bsg_attention a) {
+  constexpr int LD = pitch<T>(D), KT = TILE / 16;
+  __shared__ __align__(16) Short<T, D> x;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hk = blockIdx.x % a.heads_k, e = blockIdx.x / a.heads_k, group = a.heads_q / a.heads_k;
   const int n = a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
-  const int kj = k0 + 16 * w + m;
-  const int32_t* begins = a.begins ? a.begins + (int64_t)e * a.steps : nullptr;
-
-  Frag<T> kf[D / 32], vf[D / 32];
-#pragma unroll
-  for (int s = 0; s < D / 32; ++s) kf[s] = vf[s] = Frag<T>{};
-  if (kj < n) {
-    const T *kr = row<T>(a.k, e, kj, hk), *vr = row<T>(a.v, e, kj, hk);
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      kf[s] = load_run(kr, 32 * s, g);
-      vf[s] = load_run(vr, 32 * s, g);
-    }
-  }
+  const int own = 16 * w + m;
+  const bool live = own < n;
+  stage<T, D, TILE>(x.k, row<T>(a.k, e, 0, hk), a.k.step, n, tid, 256);
+  stage<T, D, TILE>(x.v, row<T>(a.v, e, 0, hk), a.v.step, n, tid, 256);
+  // a query behind the last step sees no key: its range begins after every key
+  if (tid < TILE) x.begin[tid] = tid < n ? (a.begins ? a.begins[(int64_t)e * a.steps + tid] : 0) : 0x7fffffff;
   f32x4 dk[D / 16], dv[D / 16];
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) dk[d] = dv[d] = f32x4{0, 0, 0, 0};
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
     const Score sc = score_of(a.scale, a.softcap, a.slopes, h);
-    const int64_t at = ((int64_t)e * a.heads_q + h) * a.steps;
-    for (int q0 = k0; q0 < n; q0 += TILE) {
-      if (begins && begins[q0] > k0 + TILE - 1) break;
-      __syncthreads();
-      stage<T, D, TILE>(sQ, row<T>(a.q, e, q0, h), a.q.step, n - q0, tid, 256);
-      stage<T, D, TILE>(sD, row<T>(a.dout, e, q0, h), a.dout.step, n - q0, tid, 256);
-      if (tid < TILE) {
-        const bool on = q0 + tid < n;
-        sLse[tid] = on ? a.lse[at + q0 + tid] : 0.0f;
-        sDelta[tid] = on ? a.delta[at + q0 + tid] : 0.0f;
-        // a query behind the last step sees no key: its range begins after every key
-        sBegin[tid] = on ? (begins ? begins[q0 + tid] : 0) : 0x7fffffff;
-      }
-      __syncthreads();
+    __syncthreads();               // the head before is done with
+    stage<T, D, TILE>(x.q, row<T>(a.q, e, 0, h), a.q.step, n, tid, 256);
+    stage<T, D, TILE>(x.go, row<T>(a.dout, e, 0, h), a.dout.step, n, tid, 256);
+    if (tid < TILE) x.lse[tid] = tid < n ? a.lse[((int64_t)e * a.heads_q + h) * a.steps + tid] : 0.0f;
+    __syncthreads();
+    f32x4 dq[D / 16];
 #pragma unroll
-      for (int c = 0; c < TILE / 32; ++c) {
-        f32x4 ps[2], ds[2];
+    for (int d = 0; d < D / 16; ++d) dq[d] = f32x4{0, 0, 0, 0};
+    if (16 * w < n) {              // the wave's 16 queries
+      f32x4 p[KT], dp[KT], ds[KT];
+      const float lse = x.lse[own];
+      const int begin = x.begin[own];
+      float delta = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int t = 2 * c + u;
-          f32x4 s = {0, 0, 0, 0}, dp = {0, 0, 0, 0};
+      for (int t = 0; t < KT; ++t) {
+        p[t] = dp[t] = ds[t] = f32x4{0, 0, 0, 0};
+        if (t <= w) {
+          f32x4 s = {0, 0, 0, 0};
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            mma(s, load_run(sQ + (16 * t + m) * LD, 32 * x, g), kf[x]);
-            mma(dp, load_run(sD + (16 * t + m) * LD, 32 * x, g), vf[x]);
+          for (int c = 0; c < D / 32; ++c) {
+            mma(s, load_run(x.k + (16 * t + m) * LD, 32 * c, g), load_run(x.q + own * LD, 32 * c, g));
+            mma(dp[t], load_run(x.v + (16 * t + m) * LD, 32 * c, g), load_run(x.go + own * LD, 32 * c, g));
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int l = 16 * t + 4 * g + r, i = q0 + l;
+            const int j = 16 * t + 4 * g + r;
             float y = 0.0f;
-            const float x = score<T, CAP>(sc, s[r], i - kj, y);
-            const float p = __builtin_amdgcn_exp2f(x - sLse[l]);
-            const bool on = kj <= i && kj >= sBegin[l];
-            float v = p * (dp[r] - sDelta[l]);
-            if (CAP) v *= 1.0f - y * y;
-            ps[u][r] = on ? p : 0.0f;
-            ds[u][r] = on ? v : 0.0f;
+            const float z = score<T, CAP, BIAS>(sc, s[r], (float)(own - j), y);
+            const bool on = j <= own && j >= begin;
+            p[t][r] = on ? __builtin_amdgcn_exp2f(z - lse) : 0.0f;
+            ds[t][r] = CAP ? p[t][r] * fmaf(-y, y, 1.0f) : p[t][r];
+            delta = fmaf(p[t][r], dp[t][r], delta);
           }
         }
-        const Frag<T> pf = round_frag<T>(join(ps[0], ps[1])), f = round_frag<T>(join(ds[0], ds[1]));
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          mma(dv[d], load_col(sD, LD, 32 * c, 16 * d, lane), pf);
-          mma(dk[d], load_col(sQ, LD, 32 * c, 16 * d, lane), f);
-        }
       }
+      delta = sum_groups(delta);
+      if (g == 0) x.delta[own] = delta;
+#pragma unroll
+      for (int c = 0; c < KT / 2; ++c)
+        if (2 * c <= w) {
+          const Frag<T> f = round_frag<T>(join(ds[2 * c] * (dp[2 * c] - delta), ds[2 * c + 1] * (dp[2 * c + 1] - delta)));
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) mma(dq[d], load_col(x.k, LD, 32 * c, 16 * d, lane), f);
+        }
+    }
+    if (own < a.steps) {
+      T* out = row_out<T>(a.dq, e, own, h);
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) store4(out + 16 * d + 4 * g, live ? dq[d] * a.scale : f32x4{0, 0, 0, 0});
+    }
+    __syncthreads();               // delta is there
+    if (16 * w < n) {              // the wave's 16 keys
+#pragma unroll
+      for (int c = 0; c < KT / 2; ++c)
+        if (2 * c + 1 >= w && 32 * c < n) {
+          f32x4 p[2], ds[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int t = 2 * c + u;
+            f32x4 s = {0, 0, 0, 0}, dp = {0, 0, 0, 0};
+            p[u] = ds[u] = f32x4{0, 0, 0, 0};
+            if (t < w || 16 * t >= n) continue;
+#pragma unroll
+            for (int z = 0; z < D / 32; ++z) {
+              mma(s, load_run(x.q + (16 * t + m) * LD, 32 * z, g), load_run(x.k + own * LD, 32 * z, g));
+              mma(dp, load_run(x.go + (16 * t + m) * LD, 32 * z, g), load_run(x.v + own * LD, 32 * z, g));
+            }
+            const f32x4 lse = *reinterpret_cast<const f32x4*>(&x.lse[16 * t + 4 * g]);
+            const f32x4 delta = *reinterpret_cast<const f32x4*>(&x.delta[16 * t + 4 * g]);
+            p_and_ds<T, CAP, BIAS>(sc, (float)(16 * t + 4 * g - own), f32x4{0, 1, 2, 3}, lse, delta, s, dp, p[u], ds[u]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int i = 16 * t + 4 * g + r;
+              const bool on = own <= i && own >= x.begin[i];
+              p[u][r] = on ? p[u][r] : 0.0f;
+              ds[u][r] = on ? ds[u][r] : 0.0f;
+            }
+          }
+          const Frag<T> pf = round_frag<T>(join(p[0], p[1])), f = round_frag<T>(join(ds[0], ds[1]));
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            mma(dv[d], load_col(x.go, LD, 32 * c, 16 * d, lane), pf);
+            mma(dk[d], load_col(x.q, LD, 32 * c, 16 * d, lane), f);
+          }
+        }
     }
   }
-  if (kj >= a.steps) return;
-  const bool live = kj < n;
-  T *ok = row_out<T>(a.dk, e, kj, hk), *ov = row_out<T>(a.dv, e, kj, hk);
+  if (own >= a.steps) return;
+  T *ok = row_out<T>(a.dk, e, own, hk), *ov = row_out<T>(a.dv, e, own, hk);
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) {
     store4(ok + 16 * d + 4 * g, live ? dk[d] * a.scale : f32x4{0, 0, 0, 0});
     store4(ov + 16 * d + 4 * g, live ? dv[d] : f32x4{0, 0, 0, 0});
   }
+}
+
+// Longer rollouts.  dq: as the forward pass, with dp^T = V dout^T next to the scores and
+// dq^T += K^T ds^T.  It also writes delta_i = dout_i.out_i for the pass over keys; out is taken
+// with what its rounding left, else delta would carry that rounding into every ds of the row.
+template <class T, int D, int QW, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) void backward_q_kernel(bsg_attention a) {
+  constexpr int LD = pitch<T>(D), KT = TILE / 16;
+  __shared__ __align__(16) T sK[TILE * LD];
+  __shared__ __align__(16) T sV[TILE * LD];
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW), id = swizzled(blockIdx.x, gridDim.x);
+  const int q0 = (nt - 1 - id % nt) * TILE * QW;
+  const int eh = id / nt, h = eh % a.heads_q, e = eh / a.heads_q;
+  const int hk = h / (a.heads_q / a.heads_k);
+  const int n = a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
+  const int qw = q0 + 16 * QW * w;
+  const Score sc = score_of(a.scale, a.softcap, a.slopes, h);
+  const int64_t base = ((int64_t)e * a.heads_q + h) * a.steps;
+  const int32_t* begins = a.begins ? a.begins + (int64_t)e * a.steps : nullptr;
+
+  Frag<T> qf[QW][D / 32], df[QW][D / 32];
+  float delta[QW], lse[QW];
+  int qi[QW], begin[QW];
+#pragma unroll
+  for (int i = 0; i < QW; ++i) {
+    qi[i] = qw + 16 * i + m;
+    const int at = max(min(qi[i], n - 1), 0);      // a query behind the last step: the last one's row
+    const T *qr = row<T>(a.q, e, at, h), *dr = row<T>(a.dout, e, at, h), *orow = row<T>(a.out, e, at, h);
+    const T* rest = static_cast<const T*>(a.out_rest) + (base + at) * D;
+    float x = 0.0f;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      qf[i][s] = load_run(qr, 32 * s, g);
+      df[i][s] = load_run(dr, 32 * s, g);
+      const f32x8 u = widen(df[i][s]);
+      f32x8 v = widen(load_run(orow, 32 * s, g));
+      if (sizeof(T) == 2) v += widen(load_run(rest, 32 * s, g));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x = fmaf(u[j], v[j], x);
+    }
+    delta[i] = sum_groups(x);
+    if (g == 0 && qi[i] < n) a.delta[base + qi[i]] = delta[i];
+    lse[i] = n > 0 ? a.lse[base + at] : 0.0f;
+    begin[i] = begins ? begins[at] : 0;
+  }
+  const int kend = min(q0 + TILE * QW, n), kbeg = begins && q0 < n ? begins[q0] / TILE * TILE : 0;
+  const int see_any = begins && qw < n ? begins[qw] : 0;
+  const int see_all = begins && qw < n ? begins[min(qw + 16 * QW, n) - 1] : 0;
+
+  f32x4 dq[QW][D / 16];
+#pragma unroll
+  for (int i = 0; i < QW; ++i)
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) dq[i][d] = f32x4{0, 0, 0, 0};
+  const auto tile = [&](int k0, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+#pragma unroll
+    for (int c = 0; c < KT / 2; ++c) {
+      if (MASK && k0 + 32 * c > qw + 16 * QW - 1) continue;
+      f32x4 ds[QW][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t = 2 * c + u;
+        f32x4 s[QW], dp[QW];
+#pragma unroll
+        for (int i = 0; i < QW; ++i) s[i] = dp[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+          const Frag<T> kf = load_run(sK + (16 * t + m) * LD, 32 * x, g), vf = load_run(sV + (16 * t + m) * LD, 32 * x, g);
+#pragma unroll
+          for (int i = 0; i < QW; ++i) {
+            mma(s[i], kf, qf[i][x]);
+            mma(dp[i], vf, df[i][x]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < QW; ++i) {
+          f32x4 p;
+          const f32x4 l = {lse[i], lse[i], lse[i], lse[i]}, dl = {delta[i], delta[i], delta[i], delta[i]};
+          p_and_ds<T, CAP, BIAS>(sc, (float)(qi[i] - k0 - 4 * g) - (float)(16 * t), f32x4{0, -1, -2, -3}, l, dl, s[i], dp[i], p, ds[i][u]);
+          if (MASK)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int j = k0 + 16 * t + 4 * g + r;
+              ds[i][u][r] = j <= qi[i] && j >= begin[i] ? ds[i][u][r] : 0.0f;
+            }
+        }
+      }
+      Frag<T> f[QW];
+#pragma unroll
+      for (int i = 0; i < QW; ++i) f[i] = round_frag<T>(join(ds[i][0], ds[i][1]));
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const Frag<T> kf = load_col(sK, LD, 32 * c, 16 * d, lane);
+#pragma unroll
+        for (int i = 0; i < QW; ++i) mma(dq[i][d], kf, f[i]);
+      }
+    }
+  };
+  Fetch<T, TILE, D, 256> fk, fv;
+  if (kbeg < kend) {
+    fk.load(row<T>(a.k, e, kbeg, hk), a.k.step, kend - kbeg, tid);
+    fv.load(row<T>(a.v, e, kbeg, hk), a.v.step, kend - kbeg, tid);
+  }
+  for (int k0 = kbeg; k0 < kend; k0 += TILE) {
+    __syncthreads();
+    fk.store(sK, kend - k0, tid);
+    fv.store(sV, kend - k0, tid);
+    if (k0 + TILE < kend) {
+      fk.load(row<T>(a.k, e, k0 + TILE, hk), a.k.step, kend - k0 - TILE, tid);
+      fv.load(row<T>(a.v, e, k0 + TILE, hk), a.v.step, kend - k0 - TILE, tid);
+    }
+    __syncthreads();
+    if (qw >= n || k0 > qw + 16 * QW - 1 || k0 + TILE <= see_any) continue;
+    if (k0 + TILE - 1 <= qw && k0 >= see_all) tile(k0, std::false_type());
+    else tile(k0, std::true_type());
+  }
+#pragma unroll
+  for (int i = 0; i < QW; ++i) {
+    if (qi[i] >= a.steps) continue;
+    const bool live = qi[i] < n;
+    T* out = row_out<T>(a.dq, e, qi[i], h);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) store4(out + 16 * d + 4 * g, live ? dq[i][d] * a.scale : f32x4{0, 0, 0, 0});
+  }
+}
+
+// dk, dv: a wave holds 16 QW keys and walks the queries that see them, in tiles of 64 fetched one
+// ahead.  A workgroup does so for every query head that shares the key's head, so that nothing is
+// added across workgroups; or, where that leaves CUs idle (`parts`), for one of them, into fp32
+// partial sums that add_parts_kernel adds.
+template <class T, int D, int QW, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
+  constexpr int LD = pitch<T>(D), QT = TILE / 16;
+  __shared__ __align__(16) T sQ[TILE * LD];
+  __shared__ __align__(16) T sD[TILE * LD];
+  __shared__ __align__(16) float sLse[TILE], sDelta[TILE];
+  __shared__ __align__(16) int sBegin[TILE];
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW), id = swizzled(blockIdx.x, gridDim.x);
+  const int k0 = id % nt * TILE * QW;                            // the longest ranges first
+  const int group = a.heads_q / a.heads_k, eh = id / nt;
+  const bool split = a.parts != nullptr;
+  const int h0 = split ? eh % a.heads_q : eh % a.heads_k * group, h1 = split ? h0 + 1 : h0 + group;
+  const int hk = h0 / group, e = split ? eh / a.heads_q : eh / a.heads_k;
+  const int n = a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
+  const int kw = k0 + 16 * QW * w;                               // the wave's first key
+  const int32_t* begins = a.begins ? a.begins + (int64_t)e * a.steps : nullptr;
+
+  Frag<T> kf[QW][D / 32], vf[QW][D / 32];
+  f32x4 dk[QW][D / 16], dv[QW][D / 16];
+  int kj[QW];
+#pragma unroll
+  for (int i = 0; i < QW; ++i) {
+    kj[i] = kw + 16 * i + m;
+    const int at = max(min(kj[i], n - 1), 0);
+    const T *kr = row<T>(a.k, e, at, hk), *vr = row<T>(a.v, e, at, hk);
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      kf[i][s] = load_run(kr, 32 * s, g);
+      vf[i][s] = load_run(vr, 32 * s, g);
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) dk[i][d] = dv[i][d] = f32x4{0, 0, 0, 0};
+  }
+  // the queries that see one of the keys end where the next episode (window) begins
+  int qend = n;
+  if (begins)
+    for (int q = k0 + TILE; q < n; q += TILE)
+      if (begins[q] > k0 + TILE * QW - 1) {
+        qend = q;
+        break;
+      }
+
+  Fetch<T, TILE, D, 256> fq, fd;
+  float flse = 0.0f, fdelta = 0.0f;
+  int fbegin = 0;
+  const auto fetch = [&](int h, int q0) {
+    fq.load(row<T>(a.q, e, q0, h), a.q.step, n - q0, tid);
+    fd.load(row<T>(a.dout, e, q0, h), a.dout.step, n - q0, tid);
+    const int64_t at = ((int64_t)e * a.heads_q + h) * a.steps;
+    const int q = min(q0 + tid % TILE, n - 1);
+    flse = a.lse[at + q];
+    fdelta = a.delta[at + q];
+    fbegin = begins ? begins[q] : 0;
+  };
+  if (k0 < qend) fetch(h0, k0);
+  for (int h = h0; h < h1; ++h) {
+    const Score sc = score_of(a.scale, a.softcap, a.slopes, h);
+    const auto tile = [&](int q0, auto masked) {
+      constexpr bool MASK = decltype(masked)::value;
+#pragma unroll
+      for (int c = 0; c < QT / 2; ++c) {
+        if (MASK && q0 + 32 * c + 31 < kw) continue;             // before the wave's first key
+        f32x4 ps[QW][2], ds[QW][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int t = 2 * c + u;
+          f32x4 s[QW], dp[QW];
+#pragma unroll
+          for (int i = 0; i < QW; ++i) s[i] = dp[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            const Frag<T> qf = load_run(sQ + (16 * t + m) * LD, 32 * x, g), df = load_run(sD + (16 * t + m) * LD, 32 * x, g);
+#pragma unroll
+            for (int i = 0; i < QW; ++i) {
+              mma(s[i], qf, kf[i][x]);
+              mma(dp[i], df, vf[i][x]);
+            }
+          }
+          const f32x4 lse = *reinterpret_cast<const f32x4*>(&sLse[16 * t + 4 * g]);
+          const f32x4 delta = *reinterpret_cast<const f32x4*>(&sDelta[16 * t + 4 * g]);
+#pragma unroll
+          for (int i = 0; i < QW; ++i) {
+            p_and_ds<T, CAP, BIAS>(sc, (float)(q0 + 4 * g - kj[i]) + (float)(16 * t), f32x4{0, 1, 2, 3}, lse, delta, s[i], dp[i], ps[i][u], ds[i][u]);
+            if (MASK)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int l = 16 * t + 4 * g + r;
+                const bool on = kj[i] <= q0 + l && kj[i] >= sBegin[l];
+                ps[i][u][r] = on ? ps[i][u][r] : 0.0f;
+                ds[i][u][r] = on ? ds[i][u][r] : 0.0f;
+              }
+          }
+        }
+        Frag<T> pf[QW], f[QW];
+#pragma unroll
+        for (int i = 0; i < QW; ++i) {
+          pf[i] = round_frag<T>(join(ps[i][0], ps[i][1]));
+          f[i] = round_frag<T>(join(ds[i][0], ds[i][1]));
+        }
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          const Frag<T> dc = load_col(sD, LD, 32 * c, 16 * d, lane), qc = load_col(sQ, LD, 32 * c, 16 * d, lane);
+#pragma unroll
+          for (int i = 0; i < QW; ++i) {
+            mma(dv[i][d], dc, pf[i]);
+            mma(dk[i][d], qc, f[i]);
+          }
+        }
+      }
+    };
+    for (int q0 = k0; q0 < qend; q0 += TILE) {
+      __syncthreads();
+      fq.store(sQ, n - q0, tid);
+      fd.store(sD, n - q0, tid);
+      if (tid < TILE) {
+        sLse[tid] = flse;
+        sDelta[tid] = fdelta;
+        // a query behind the last step sees no key: its range begins after every key
+        sBegin[tid] = q0 + tid < n ? fbegin : 0x7fffffff;
+      }
+      if (q0 + TILE < qend) fetch(h, q0 + TILE);
+      else if (h + 1 < h1) fetch(h + 1, k0);
+      __syncthreads();
+      if (kw >= n || q0 + TILE - 1 < kw || sBegin[0] > kw + 16 * QW - 1) continue;
+      // every query of the tile sees every key of the wave
+      if (kw + 16 * QW - 1 <= q0 && sBegin[TILE - 1] <= kw) tile(q0, std::false_type());
+      else tile(q0, std::true_type());
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < QW; ++i) {
+    if (kj[i] >= a.steps) continue;
+    const bool live = kj[i] < n;
+    if (split) {
+      float* to = a.parts + (((int64_t)e * a.heads_q + h0) * a.steps + kj[i]) * 2 * D;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        store4(to + 16 * d + 4 * g, live ? dk[i][d] * a.scale : f32x4{0, 0, 0, 0});
+        store4(to + D + 16 * d + 4 * g, live ? dv[i][d] : f32x4{0, 0, 0, 0});
+      }
+    } else {
+      T *ok = row_out<T>(a.dk, e, kj[i], hk), *ov = row_out<T>(a.dv, e, kj[i], hk);
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        store4(ok + 16 * d + 4 * g, live ? dk[i][d] * a.scale : f32x4{0, 0, 0, 0});
+        store4(ov + 16 * d + 4 * g, live ? dv[i][d] : f32x4{0, 0, 0, 0});
+      }
+    }
+  }
+}
+// one thread per four values of a key's dk and dv: the query heads' parts in their order
+template <class T, int D>
+__global__ __launch_bounds__(256) void add_parts_kernel(bsg_attention a, int64_t all) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= all) return;
+  const int c = (int)(i % (D / 2)) * 4, group = a.heads_q / a.heads_k;
+  const int t = (int)(i / (D / 2) % a.steps);
+  const int64_t eh = i / (D / 2) / a.steps;
+  const int hk = (int)(eh % a.heads_k), e = (int)(eh / a.heads_k);
+  f32x4 x = {0, 0, 0, 0};
+  for (int h = hk * group; h < (hk + 1) * group; ++h)
+    x += *reinterpret_cast<const f32x4*>(a.parts + (((int64_t)e * a.heads_q + h) * a.steps + t) * 2 * D + c);
+  if (c < D) store4(row_out<T>(a.dk, e, t, hk) + c, x);
+  else store4(row_out<T>(a.dv, e, t, hk) + c - D, x);
 }
 
 // ---- acting --------------------------------------------------------------------------------
@@ -448,7 +782,7 @@ struct Act {
 #pragma unroll
           for (int j = 0; j < EPL; ++j) dot = fmaf(q[i][j], kx[u][j], dot);
           float y;
-          s[u][i] = score<T, CAP>(sc[i], sum_lanes<LPR>(dot), ago[u], y);
+          s[u][i] = score<T, CAP, true>(sc[i], sum_lanes<LPR>(dot), (float)ago[u], y);
           s[u][i] = on[u] ? s[u][i] : -INFINITY;
         }
       // what a masked slot holds is not even multiplied by zero: it may be anything
@@ -485,7 +819,7 @@ struct Act {
         float dot = 0.0f, y;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) dot = fmaf(q[i][j], kx[j], dot);
-        const float s = score<T, CAP>(sc[i], sum_lanes<LPR>(dot), 0, y);
+        const float s = score<T, CAP, true>(sc[i], sum_lanes<LPR>(dot), 0.0f, y);
         const float top = fmaxf(x.mx[i], s);
         const float old = __builtin_amdgcn_exp2f(x.mx[i] - top), p = __builtin_amdgcn_exp2f(s - top);
         x.mx[i] = top;
@@ -694,25 +1028,44 @@ hipError_t act(const bsg_attention_act& a, hipStream_t st) {
   return cap ? act<T, D, 1, true>(a, p, st) : act<T, D, 1, false>(a, p, st);
 }
 
-template <class T, int D, bool CAP>
+// Queries (keys) per wave: 32 for bf16 rollouts of more than one tile, else 16.
+template <class T> bool two_tiles(const bsg_attention& a) { return sizeof(T) == 2 && a.steps > 512; }
+
+template <class T, int D, int QW, bool CAP, bool BIAS>
 hipError_t forward(const bsg_attention& a, hipStream_t st) {
-  const int nt = (a.steps + TILE - 1) / TILE;
-  if (a.begins && (a.first || a.window > 0))
+  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW);
+  if (a.begins)
     begins_kernel<<<dim3(a.num_envs), dim3(256), 0, st>>>(a.first, a.first_env, a.first_step, a.steps, a.window, a.begins);
-  forward_kernel<T, D, CAP><<<dim3(a.num_envs * a.heads_q * nt), dim3(256), 0, st>>>(a);
+  forward_kernel<T, D, QW, CAP, BIAS><<<dim3(a.num_envs * a.heads_q * nt), dim3(256), 0, st>>>(a);
   return hipGetLastError();
 }
-template <class T, int D, bool CAP>
+template <class T, int D, int QW, bool CAP, bool BIAS>
 hipError_t backward(const bsg_attention& a, hipStream_t st) {
-  const int nt = (a.steps + TILE - 1) / TILE;
-  backward_q_kernel<T, D, CAP><<<dim3(a.num_envs * a.heads_q * nt), dim3(256), 0, st>>>(a);
-  backward_kv_kernel<T, D, CAP><<<dim3(a.num_envs * a.heads_k * nt), dim3(256), 0, st>>>(a);
+  if (a.steps <= TILE) {
+    backward_short_kernel<T, D, CAP, BIAS><<<dim3(a.num_envs * a.heads_k), dim3(256), 0, st>>>(a);
+    return hipGetLastError();
+  }
+  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW);
+  backward_q_kernel<T, D, QW, CAP, BIAS><<<dim3(a.num_envs * a.heads_q * nt), dim3(256), 0, st>>>(a);
+  constexpr int KW = D == 128 ? 1 : QW;
+  const int heads = a.parts ? a.heads_q : a.heads_k, kt = (a.steps + TILE * KW - 1) / (TILE * KW);
+  backward_kv_kernel<T, D, KW, CAP, BIAS><<<dim3(a.num_envs * heads * kt), dim3(256), 0, st>>>(a);
+  if (a.parts) {
+    const int64_t all = (int64_t)a.num_envs * a.heads_k * a.steps * (D / 2);
+    add_parts_kernel<T, D><<<dim3((unsigned)((all + 255) / 256)), dim3(256), 0, st>>>(a, all);
+  }
   return hipGetLastError();
+}
+template <class T, int D, bool CAP, bool BIAS>
+hipError_t learn(const bsg_attention& a, bool back, hipStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (two_tiles<T>(a)) return back ? backward<T, D, 2, CAP, BIAS>(a, st) : forward<T, D, 2, CAP, BIAS>(a, st);
+  return back ? backward<T, D, 1, CAP, BIAS>(a, st) : forward<T, D, 1, CAP, BIAS>(a, st);
 }
 template <class T, int D>
 hipError_t learn(const bsg_attention& a, bool back, hipStream_t st) {
-  if (a.softcap > 0.0f) return back ? backward<T, D, true>(a, st) : forward<T, D, true>(a, st);
-  return back ? backward<T, D, false>(a, st) : forward<T, D, false>(a, st);
+  if (a.softcap > 0.0f) return a.slopes ? learn<T, D, true, true>(a, back, st) : learn<T, D, true, false>(a, back, st);
+  return a.slopes ? learn<T, D, false, true>(a, back, st) : learn<T, D, false, false>(a, back, st);
 }
 template <class T>
 hipError_t learn(const bsg_attention& a, bool back, hipStream_t st) {
@@ -733,6 +1086,12 @@ hipError_t launch_attention(const bsg_attention& a, bool back, hipStream_t st) {
 }
 hipError_t launch_attention_step(const bsg_attention_act& a, hipStream_t st) {
   return a.dtype == BSG_BF16 ? act<mma::bf16>(a, st) : act<float>(a, st);
+}
+// Parts by query head are wanted where key tiles alone give fewer than four workgroups to a CU.
+bool attention_wants_parts(const bsg_attention& a) {
+  if (a.heads_q == a.heads_k || a.steps <= TILE) return false;
+  const int rows = a.dtype == BSG_BF16 && two_tiles<mma::bf16>(a) ? 2 * TILE : TILE;
+  return (int64_t)a.num_envs * a.heads_k * ((a.steps + rows - 1) / rows) < 1024;
 }
 int64_t attention_step_bytes(const bsg_attention_act& a) {
   const Plan p = plan_of(a);

@@ -168,35 +168,6 @@ template <class T, int DK, int NW> constexpr int waves_per_simd() {
   return NW == 2 ? 1 : NW == 8 || 2 * sizeof(Chunk<T, DK, NW>) <= 160 * 1024 ? 2 : 1;
 }
 
-// A C x N tile on its way from memory to LDS through registers: loaded while the chunk before it is
-// computed.  Rows behind `rows` (at least 1) become zeros; in their place the last one is read.
-template <class T, int N, int NT>
-struct Fetch {
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  static constexpr int V = Vec<T>::n, ROW = N / V, n = (C * ROW + NT - 1) / NT;
-  u32x4 x[n];
-  __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int tid) {
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const int at = tid + i * NT, r = at / ROW, c = at % ROW * V;
-      x[i] = *reinterpret_cast<const u32x4*>(p + min(r, rows - 1) * stride + c);
-    }
-  }
-  __device__ __forceinline__ void store(T* s, int rows, int tid) const {
-    if (rows >= C) {
-#pragma unroll
-      for (int i = 0; i < n; ++i) put(s, tid + i * NT, x[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < n; ++i) put(s, tid + i * NT, (tid + i * NT) / ROW < rows ? x[i] : u32x4{0, 0, 0, 0});
-    }
-  }
-  static __device__ __forceinline__ void put(T* s, int at, const u32x4& v) {
-    const int r = at / ROW, c = at % ROW * V;
-    if (C * ROW % NT == 0 || r < C) *reinterpret_cast<u32x4*>(s + r * pitch<T>(N) + c) = v;
-  }
-};
-
 // A wave's 16 columns of the C x 16 NW tile: from registers (D tiles) to LDS, and from there, in
 // 16-byte pieces, to the rows in memory.  Rows behind `rows` are padding: zeros, up to `all`.
 template <class T, int VD>
@@ -322,8 +293,8 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void forwar
     for (int r = 0; r < 4; ++r)
       S[d][r] = a.state ? a.state[(eh * DK + 16 * d + 4 * g + r) * DV + col] : 0.0f;
 
-  Fetch<T, DK, NT> fk, fq;
-  Fetch<T, DV, NT> fv;
+  Fetch<T, C, DK, NT> fk, fq;
+  Fetch<T, C, DV, NT> fv;
   RawGates raw = {0, 0, 0};
   const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), v = steps_in<const T>(a.v, e, h);
   const Steps<T> out = steps_in<T>(a.out, e, h);
@@ -446,8 +417,8 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void backwa
     for (int r = 0; r < 4; ++r)
       D[d][r] = a.dfinal ? a.dfinal[(eh * DK + 16 * d + 4 * g + r) * DV + col] : 0.0f;
 
-  Fetch<T, DK, NT> fk, fq;
-  Fetch<T, DV, NT> fv;
+  Fetch<T, C, DK, NT> fk, fq;
+  Fetch<T, C, DV, NT> fv;
   RawGates raw = {0, 0, 0};
   const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), dout = steps_in<const T>(a.dout, e, h);
   const Steps<T> dv = steps_in<T>(a.dv, e, h);
@@ -852,7 +823,7 @@ __global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
 // both sums over it (S^T k and S^T q) in one pass, then the update.  Lanes hold four columns;
 // S'^T q = (S + k u^T)^T q = S^T q + (k.q) u.
 template <class T, int DK, int DV>
-__global__ __launch_bounds__(256) void step_kernel(bsg_delta a, int64_t waves) {
+__global__ __launch_bounds__(256) void step_kernel(bsg_delta_act a, int64_t waves) {
   constexpr int COLS = DV == 32 || DK == 128 ? 32 : 64, L = COLS / 4, RG = 64 / L, N = DK / RG, SLICES = DV / COLS;
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (id >= waves) return;
@@ -861,7 +832,7 @@ __global__ __launch_bounds__(256) void step_kernel(bsg_delta a, int64_t waves) {
   const int c0 = (int)(id % SLICES) * COLS + lane % L * 4;
   const int h = (int)(eh % a.heads_v), e = (int)(eh / a.heads_v), hk = h / (a.heads_v / a.heads_k);
   const bool first = a.first && a.first[e * a.first_env] != 0;
-  float* st = a.final_state + eh * DK * DV + c0;
+  float* st = a.state + eh * DK * DV + c0;
   f32x4 S[N];
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -902,36 +873,37 @@ __global__ __launch_bounds__(256) void step_kernel(bsg_delta a, int64_t waves) {
   if (rg == 0) store4(row_out<T>(a.out, e, 0, h) + c0, (sq + u * kq) * a.scale);
 }
 
-enum { FORWARD, BACKWARD, STEP };
 
 template <class T, int DK, int NW>
-hipError_t run(const bsg_delta& a, int what, hipStream_t st) {
-  const unsigned rows = (unsigned)(a.num_envs * a.heads_v);
-  if (what == STEP) {
-    constexpr int DV = 16 * NW, slices = DV / (DV == 32 || DK == 128 ? 32 : 64);
-    const int64_t waves = (int64_t)rows * slices;
-    step_kernel<T, DK, DV><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st>>>(a, waves);
-  } else if (what == FORWARD) {
-    forward_kernel<T, DK, NW><<<dim3(rows), dim3(64 * NW), 0, st>>>(a);
+hipError_t run(const bsg_delta_act& a, bool, hipStream_t st) {
+  constexpr int DV = 16 * NW, slices = DV / (DV == 32 || DK == 128 ? 32 : 64);
+  const int64_t waves = (int64_t)a.num_envs * a.heads_v * slices;
+  step_kernel<T, DK, DV><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st>>>(a, waves);
+  return hipGetLastError();
+}
+template <class T, int DK, int NW>
+hipError_t run(const bsg_delta& a, bool back, hipStream_t st) {
+  const dim3 rows((unsigned)(a.num_envs * a.heads_v));
+  if (back) {
+    backward_state_kernel<T, DK, NW><<<rows, dim3(64 * NW), 0, st>>>(a);
+    const dim3 chunks((unsigned)(a.num_envs * a.heads_k * ((a.steps + C - 1) / C)));
+    if (a.heads_v > a.heads_k) backward_chunk_kernel<T, DK, true><<<chunks, dim3(512), 0, st>>>(a);
+    else backward_chunk_kernel<T, DK, false><<<chunks, dim3(512), 0, st>>>(a);
   } else {
-    backward_state_kernel<T, DK, NW><<<dim3(rows), dim3(64 * NW), 0, st>>>(a);
-    const int chunks = (a.steps + C - 1) / C;
-    const dim3 grid((unsigned)(a.num_envs * a.heads_k * chunks));
-    if (a.heads_v > a.heads_k) backward_chunk_kernel<T, DK, true><<<grid, dim3(512), 0, st>>>(a);
-    else backward_chunk_kernel<T, DK, false><<<grid, dim3(512), 0, st>>>(a);
+    forward_kernel<T, DK, NW><<<rows, dim3(64 * NW), 0, st>>>(a);
   }
   return hipGetLastError();
 }
-template <class T, int DK>
-hipError_t run(const bsg_delta& a, int what, hipStream_t st) {
-  return a.dim_v == 32 ? run<T, DK, 2>(a, what, st) : a.dim_v == 64 ? run<T, DK, 4>(a, what, st) : run<T, DK, 8>(a, what, st);
+template <class T, int DK, class A>
+hipError_t run(const A& a, bool back, hipStream_t st) {
+  return a.dim_v == 32 ? run<T, DK, 2>(a, back, st) : a.dim_v == 64 ? run<T, DK, 4>(a, back, st) : run<T, DK, 8>(a, back, st);
 }
-template <class T>
-hipError_t run(const bsg_delta& a, int what, hipStream_t st) {
-  return a.dim_k == 32 ? run<T, 32>(a, what, st) : a.dim_k == 64 ? run<T, 64>(a, what, st) : run<T, 128>(a, what, st);
+template <class T, class A>
+hipError_t run(const A& a, bool back, hipStream_t st) {
+  return a.dim_k == 32 ? run<T, 32>(a, back, st) : a.dim_k == 64 ? run<T, 64>(a, back, st) : run<T, 128>(a, back, st);
 }
-hipError_t run(const bsg_delta& a, int what, hipStream_t st) {
-  return a.dtype == BSG_BF16 ? run<bf16>(a, what, st) : run<float>(a, what, st);
+template <class A> hipError_t run(const A& a, bool back, hipStream_t st) {
+  return a.dtype == BSG_BF16 ? run<bf16>(a, back, st) : run<float>(a, back, st);
 }
 
 }  // namespace
@@ -939,8 +911,8 @@ hipError_t run(const bsg_delta& a, int what, hipStream_t st) {
 namespace bsg {
 
 // Shapes, strides and pointers are validated by the bsg_delta_* entry points (bsg_abi.cpp).
-hipError_t launch_delta_forward(const bsg_delta& a, hipStream_t st) { return run(a, FORWARD, st); }
-hipError_t launch_delta_backward(const bsg_delta& a, hipStream_t st) { return run(a, BACKWARD, st); }
-hipError_t launch_delta_step(const bsg_delta& a, hipStream_t st) { return run(a, STEP, st); }
+hipError_t launch_delta_forward(const bsg_delta& a, hipStream_t st) { return run(a, false, st); }
+hipError_t launch_delta_backward(const bsg_delta& a, hipStream_t st) { return run(a, true, st); }
+hipError_t launch_delta_step(const bsg_delta_act& a, hipStream_t st) { return run(a, false, st); }
 
 }  // namespace bsg

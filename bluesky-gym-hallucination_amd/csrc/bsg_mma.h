@@ -160,14 +160,18 @@ __device__ __forceinline__ void store4(T* p, const f32x4& x) {   // 4 T's, align
 template <class T> struct Vec { static constexpr int n = 16 / (int)sizeof(T); };
 template <class T> __host__ __device__ constexpr int pitch(int n) { return n + Vec<T>::n; }
 
-// sum / max over the four lane groups (the rows of a D tile)
+// sum / max over the four lane groups (the rows of a D tile): lanes 16 and 32 apart trade places
 __device__ __forceinline__ float sum_groups(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 __device__ __forceinline__ float max_groups(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // Copies `rows` rows of `n` T's (16-byte aligned, `stride` apart) into an LDS tile of `all`
@@ -183,6 +187,35 @@ __device__ __forceinline__ void stage(T* s, const T* p, int64_t stride, int rows
     *reinterpret_cast<u32x4*>(s + r * pitch<T>(N) + c) = x;
   }
 }
+
+// An R x N tile on its way from memory to LDS through registers: loaded while the one before it is
+// computed.  Rows behind `rows` (at least 1) become zeros; in their place the last one is read.
+template <class T, int R, int N, int NT>
+struct Fetch {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  static constexpr int V = Vec<T>::n, ROW = N / V, n = (R * ROW + NT - 1) / NT;
+  u32x4 x[n];
+  __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int tid) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const int at = tid + i * NT, r = at / ROW, c = at % ROW * V;
+      x[i] = *reinterpret_cast<const u32x4*>(p + min(r, rows - 1) * stride + c);
+    }
+  }
+  __device__ __forceinline__ void store(T* s, int rows, int tid) const {
+    if (rows >= R) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) put(s, tid + i * NT, x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < n; ++i) put(s, tid + i * NT, (tid + i * NT) / ROW < rows ? x[i] : u32x4{0, 0, 0, 0});
+    }
+  }
+  static __device__ __forceinline__ void put(T* s, int at, const u32x4& v) {
+    const int r = at / ROW, c = at % ROW * V;
+    if (R * ROW % NT == 0 || r < R) *reinterpret_cast<u32x4*>(s + r * pitch<T>(N) + c) = v;
+  }
+};
 
 }  // namespace mma
 }  // namespace bsg

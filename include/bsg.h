@@ -399,9 +399,19 @@ typedef struct bsg_delta {
 } bsg_delta;
 int32_t bsg_delta_forward(const bsg_delta* a, void* stream);
 int32_t bsg_delta_backward(const bsg_delta* a, void* stream);
-/* One step of every env: steps = 1, `state` = `final_state` updated in place (it must not be
- * NULL); a first step forgets it.  Reads q, k, v, g, beta, first; `lengths` must be NULL. */
-int32_t bsg_delta_step(const bsg_delta* a, void* stream);
+/* One step of every env, with the state updated in place; a first step forgets it, whatever it
+ * holds. */
+typedef struct bsg_delta_act {
+  int32_t num_envs;
+  int32_t heads_k, heads_v, dim_k, dim_v;
+  int32_t dtype, gate_dtype;
+  float scale;
+  bsg_rows q, k, v, g, beta, out;   /* .step unused */
+  const uint8_t* first;      /* NULL: no env starts an episode */
+  int64_t first_env;
+  float* state;              /* [num_envs][heads_v][dim_k][dim_v] */
+} bsg_delta_act;
+int32_t bsg_delta_step(const bsg_delta_act* a, void* stream);
 
 /* Attention of each step to the steps of its episode so far, per env and query head:
  *   s_ij = scale q_i.k_j, capped to softcap tanh(s_ij / softcap) if softcap > 0, less
@@ -423,11 +433,16 @@ typedef struct bsg_attention {
   int32_t* begins;           /* [num_envs][steps] scratch of the forward pass, read by the backward
                                 pass: the first step that each step sees; may be NULL if first
                                 is NULL and window is 0 */
-  float* lse;                /* [num_envs][heads_q][steps] kept for the backward pass; NULL = not */
+  /* kept by the forward pass for the backward pass (NULL: not kept) */
+  float* lse;                /* [num_envs][heads_q][steps] */
+  void* out_rest;            /* [num_envs][heads_q][steps][dim] dtype: what rounding left of out; read
+                                and wanted for BSG_BF16 and more than 64 steps only */
   /* backward only (out as the forward pass wrote it) */
   bsg_rows dout, dq, dk, dv;
   float* delta;              /* [num_envs][heads_q][steps] scratch */
+  float* parts;              /* scratch of bsg_attention_parts_bytes() bytes, NULL if that is 0 */
 } bsg_attention;
+int64_t bsg_attention_parts_bytes(const bsg_attention* a);
 int32_t bsg_attention_forward(const bsg_attention* a, void* stream);
 int32_t bsg_attention_backward(const bsg_attention* a, void* stream);
 

@@ -16,7 +16,7 @@ REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def test_struct_layouts_match_c(tmp_path):
-    structs = {"bsg_rows": nat.BsgRows, "bsg_delta": nat.BsgDelta, "bsg_attention": nat.BsgAttention,
+    structs = {"bsg_rows": nat.BsgRows, "bsg_delta": nat.BsgDelta, "bsg_delta_act": nat.BsgDeltaAct, "bsg_attention": nat.BsgAttention,
                "bsg_attention_act": nat.BsgAttentionAct}
     lines = []
     for name, cls in structs.items():
@@ -51,6 +51,14 @@ def delta_args(**kw):
     return a
 
 
+def step_args(**kw):
+    a = nat.BsgDeltaAct(num_envs=2, heads_k=1, heads_v=1, dim_k=64, dim_v=64, scale=1.0, q=rows(), k=rows(), v=rows(), g=rows(),
+                        beta=rows(), out=rows(), state=P)
+    for n, x in kw.items():
+        setattr(a, n, x)
+    return a
+
+
 def attention_args(**kw):
     a = nat.BsgAttention(num_envs=2, steps=3, heads_q=2, heads_k=1, dim=64, scale=1.0, q=rows(), k=rows(), v=rows(),
                          out=rows(), dout=rows(), dq=rows(), dk=rows(), dv=rows(), lse=P, delta=P)
@@ -78,8 +86,8 @@ def test_delta_entry_points_refuse(kw):
     lib = nat.load_library()
     assert lib.bsg_delta_forward(C.byref(delta_args(**kw)), None) == INVALID
     assert lib.bsg_delta_backward(C.byref(delta_args(**kw)), None) == INVALID
-    step = dict(steps=1, state=P, final_state=P)
-    assert lib.bsg_delta_step(C.byref(delta_args(**{**step, **kw})), None) == INVALID
+    if "steps" not in kw:
+        assert lib.bsg_delta_step(C.byref(step_args(**kw)), None) == INVALID
     assert lib.bsg_last_error()
 
 
@@ -88,11 +96,11 @@ def test_delta_entry_points_refuse(kw):
     ("bsg_delta_backward", dict(dq=rows(0))), ("bsg_delta_backward", dict(dv=rows(step=1))),
     ("bsg_delta_backward", dict(dbeta=rows(0))), ("bsg_delta_backward", dict(work_states=None)),
     ("bsg_delta_backward", dict(kept_w=P + 4)),
-    ("bsg_delta_step", dict(steps=2, state=P, final_state=P)), ("bsg_delta_step", dict(steps=1)),
-    ("bsg_delta_step", dict(steps=1, state=P, final_state=2 * P)), ("bsg_delta_step", dict(steps=1, state=P + 4, final_state=P + 4)),
-    ("bsg_delta_step", dict(steps=1, state=P, final_state=P, lengths=P))], ids=str)
+    ("bsg_delta_forward", dict(kept_states=P + 4)), ("bsg_delta_step", dict(state=None)), ("bsg_delta_step", dict(state=P + 4)),
+    ("bsg_delta_step", dict(out=rows(P + 2)))], ids=str)
 def test_delta_calls_refuse(fn, kw):
-    assert getattr(nat.load_library(), fn)(C.byref(delta_args(**kw)), None) == INVALID
+    args = step_args if fn == "bsg_delta_step" else delta_args
+    assert getattr(nat.load_library(), fn)(C.byref(args(**kw)), None) == INVALID
 
 
 @pytest.mark.parametrize("kw", [
@@ -105,7 +113,9 @@ def test_attention_entry_points_refuse(kw):
     assert lib.bsg_attention_backward(C.byref(attention_args(**kw)), None) == INVALID
 
 
-@pytest.mark.parametrize("kw", [dict(lse=None), dict(delta=None), dict(dout=rows(0)), dict(dk=rows(P + 4))], ids=str)
+@pytest.mark.parametrize("kw", [dict(lse=None), dict(delta=None), dict(dout=rows(0)), dict(dk=rows(P + 4)), dict(parts=P),
+                                dict(steps=300), dict(steps=300, parts=P + 4), dict(steps=300, parts=P, dtype=1),
+                                dict(out_rest=P + 2)], ids=str)
 def test_attention_backward_refuses(kw):
     assert nat.load_library().bsg_attention_backward(C.byref(attention_args(**kw)), None) == INVALID
 
@@ -116,6 +126,31 @@ def test_attention_backward_refuses(kw):
     dict(work_bytes=16)], ids=str)
 def test_attention_step_refuses(kw):
     assert nat.load_library().bsg_attention_step(C.byref(act_args(**kw)), None) == INVALID
+
+
+def test_packed_blocks_are_the_structures():
+    """The byte blocks that bluesky_gym.memory passes are the ctypes structures."""
+    for cls in (nat.BsgDelta, nat.BsgDeltaAct, nat.BsgAttention, nat.BsgAttentionAct):
+        flat = []
+        for n, t in cls._fields_:
+            flat += [len(flat) + i + 1 for i in range(4)] if t is nat.BsgRows else [len(flat) + 1]
+        a = cls.from_buffer_copy(nat.packer(cls)(*flat))
+        i = 0
+        for n, t in cls._fields_:
+            x = getattr(a, n)
+            got = [x.p, x.env, x.step, x.head] if t is nat.BsgRows else [x]
+            assert got == flat[i:i + len(got)], (cls.__name__, n)
+            i += len(got)
+
+
+def test_parts_are_wanted_where_key_tiles_are_few():
+    """By query head where shared key heads leave CUs idle, from bsg_attention_parts_bytes alone."""
+    lib = nat.load_library()
+    need = lambda **kw: lib.bsg_attention_parts_bytes(C.byref(attention_args(**kw)))  # noqa: E731
+    assert need() == 0 and need(steps=64) == 0 and need(steps=65, heads_q=1) == 0
+    assert need(steps=65) == 2 * 2 * 65 * 2 * 64 * 4
+    assert need(steps=65, num_envs=4096) == 0
+    assert need(steps=-1) == INVALID
 
 
 def test_empty_calls_do_nothing_and_null_arguments_are_refused():
