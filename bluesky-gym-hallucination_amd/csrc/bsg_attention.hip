@@ -270,14 +270,19 @@ __device__ __forceinline__ void p_and_ds(const Score& sc, float ago, const f32x4
 }
 
 // Rollouts of one tile (64 steps): one workgroup per env and key head computes all three
-// gradients, rows of each head fetched once.  A wave first holds 16 queries (dq, and delta from
-// the whole row of p and dp, so that the rounded out is not needed), then 16 keys, whose dk and dv
-// it adds up over the query heads that share them.
+// gradients from p and ds computed once.  A wave holds 16 queries for p, ds and dq (and delta, from
+// the whole row of p and dp, so that the rounded out is not needed); p and ds then go to LDS, where V
+// and K were, and the wave takes 16 keys, whose dk and dv it adds up over the query heads that share
+// them.
 template <class T, int D>
-struct Short { T k[TILE * pitch<T>(D)], v[TILE * pitch<T>(D)], q[TILE * pitch<T>(D)], go[TILE * pitch<T>(D)]; float lse[TILE], delta[TILE]; int begin[TILE]; };
+struct Short {
+  static constexpr int N = D > TILE ? D : TILE, LD = pitch<T>(D), PD = pitch<T>(TILE);
+  T q[TILE * LD], go[TILE * LD];
+  T k[TILE * pitch<T>(N)], v[TILE * pitch<T>(N)];                // then ds and p, [query][key]
+};
 template <class T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) void backward_short_kernel(bsg_attention a) {
-  constexpr int LD = pitch<T>(D), KT = TILE / 16;
+  constexpr int LD = pitch<T>(D), PD = pitch<T>(TILE), KT = TILE / 16;
   __shared__ __align__(16) Short<T, D> x;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -285,33 +290,40 @@ __global__ __launch_bounds__(256) void backward_short_kernel(bsg_attention a) {
   const int n = a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
   const int own = 16 * w + m;
   const bool live = own < n;
-  stage<T, D, TILE>(x.k, row<T>(a.k, e, 0, hk), a.k.step, n, tid, 256);
-  stage<T, D, TILE>(x.v, row<T>(a.v, e, 0, hk), a.v.step, n, tid, 256);
-  // a query behind the last step sees no key: its range begins after every key
-  if (tid < TILE) x.begin[tid] = tid < n ? (a.begins ? a.begins[(int64_t)e * a.steps + tid] : 0) : 0x7fffffff;
+  const int begin = live && a.begins ? a.begins[(int64_t)e * a.steps + own] : 0;
   f32x4 dk[D / 16], dv[D / 16];
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) dk[d] = dv[d] = f32x4{0, 0, 0, 0};
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
     const Score sc = score_of(a.scale, a.softcap, a.slopes, h);
+    const float lse = live ? a.lse[((int64_t)e * a.heads_q + h) * a.steps + own] : 0.0f;
+    Fetch<T, TILE, D, 256> fk, fv, fq, fd;
+    if (n > 0) {
+      fk.load(row<T>(a.k, e, 0, hk), a.k.step, n, tid);
+      fq.load(row<T>(a.q, e, 0, h), a.q.step, n, tid);
+      fv.load(row<T>(a.v, e, 0, hk), a.v.step, n, tid);
+      fd.load(row<T>(a.dout, e, 0, h), a.dout.step, n, tid);
+    }
     __syncthreads();               // the head before is done with
-    stage<T, D, TILE>(x.q, row<T>(a.q, e, 0, h), a.q.step, n, tid, 256);
-    stage<T, D, TILE>(x.go, row<T>(a.dout, e, 0, h), a.dout.step, n, tid, 256);
-    if (tid < TILE) x.lse[tid] = tid < n ? a.lse[((int64_t)e * a.heads_q + h) * a.steps + tid] : 0.0f;
+    if (n > 0) {
+      fk.store(x.k, n, tid);
+      fq.store(x.q, n, tid);
+      fv.store(x.v, n, tid);
+      fd.store(x.go, n, tid);
+    }
     __syncthreads();
-    f32x4 dq[D / 16];
+    // rows of keys, a lane's query; the tiles of keys behind the wave's queries stay zero
+    f32x4 p[KT], ds[KT], dq[D / 16];
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) dq[d] = f32x4{0, 0, 0, 0};
-    if (16 * w < n) {              // the wave's 16 queries
-      f32x4 p[KT], dp[KT], ds[KT];
-      const float lse = x.lse[own];
-      const int begin = x.begin[own];
+    for (int t = 0; t < KT; ++t) p[t] = ds[t] = f32x4{0, 0, 0, 0};
+    if (16 * w < n) {
+      f32x4 dp[KT];
       float delta = 0.0f;
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        p[t] = dp[t] = ds[t] = f32x4{0, 0, 0, 0};
+      for (int t = 0; t < KT; ++t)
         if (t <= w) {
           f32x4 s = {0, 0, 0, 0};
+          dp[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             mma(s, load_run(x.k + (16 * t + m) * LD, 32 * c, g), load_run(x.q + own * LD, 32 * c, g));
@@ -322,64 +334,51 @@ __global__ __launch_bounds__(256) void backward_short_kernel(bsg_attention a) {
             const int j = 16 * t + 4 * g + r;
             float y = 0.0f;
             const float z = score<T, CAP, BIAS>(sc, s[r], (float)(own - j), y);
-            const bool on = j <= own && j >= begin;
+            const bool on = live && j <= own && j >= begin;
             p[t][r] = on ? __builtin_amdgcn_exp2f(z - lse) : 0.0f;
             ds[t][r] = CAP ? p[t][r] * fmaf(-y, y, 1.0f) : p[t][r];
             delta = fmaf(p[t][r], dp[t][r], delta);
           }
         }
-      }
       delta = sum_groups(delta);
-      if (g == 0) x.delta[own] = delta;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+        if (t <= w) ds[t] *= dp[t] - delta;
+    }
+    __syncthreads();               // V is done with: p takes its place
+#pragma unroll
+    for (int t = 0; t < KT; ++t) store4(x.v + own * PD + 16 * t + 4 * g, p[t]);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) dq[d] = f32x4{0, 0, 0, 0};
+    if (16 * w < n) {
 #pragma unroll
       for (int c = 0; c < KT / 2; ++c)
         if (2 * c <= w) {
-          const Frag<T> f = round_frag<T>(join(ds[2 * c] * (dp[2 * c] - delta), ds[2 * c + 1] * (dp[2 * c + 1] - delta)));
+          const Frag<T> f = round_frag<T>(join(ds[2 * c], ds[2 * c + 1]));
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) mma(dq[d], load_col(x.k, LD, 32 * c, 16 * d, lane), f);
         }
     }
+    __syncthreads();               // K is done with: ds takes its place
+#pragma unroll
+    for (int t = 0; t < KT; ++t) store4(x.k + own * PD + 16 * t + 4 * g, ds[t]);
     if (own < a.steps) {
       T* out = row_out<T>(a.dq, e, own, h);
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) store4(out + 16 * d + 4 * g, live ? dq[d] * a.scale : f32x4{0, 0, 0, 0});
     }
-    __syncthreads();               // delta is there
-    if (16 * w < n) {              // the wave's 16 keys
+    __syncthreads();
+    // a lane's key: the queries from the wave's tile on
 #pragma unroll
-      for (int c = 0; c < KT / 2; ++c)
-        if (2 * c + 1 >= w && 32 * c < n) {
-          f32x4 p[2], ds[2];
+    for (int c = 0; c < KT / 2; ++c)
+      if (2 * c + 1 >= w && 32 * c < n) {
+        const Frag<T> pf = load_col(x.v, PD, 32 * c, 16 * w, lane), f = load_col(x.k, PD, 32 * c, 16 * w, lane);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int t = 2 * c + u;
-            f32x4 s = {0, 0, 0, 0}, dp = {0, 0, 0, 0};
-            p[u] = ds[u] = f32x4{0, 0, 0, 0};
-            if (t < w || 16 * t >= n) continue;
-#pragma unroll
-            for (int z = 0; z < D / 32; ++z) {
-              mma(s, load_run(x.q + (16 * t + m) * LD, 32 * z, g), load_run(x.k + own * LD, 32 * z, g));
-              mma(dp, load_run(x.go + (16 * t + m) * LD, 32 * z, g), load_run(x.v + own * LD, 32 * z, g));
-            }
-            const f32x4 lse = *reinterpret_cast<const f32x4*>(&x.lse[16 * t + 4 * g]);
-            const f32x4 delta = *reinterpret_cast<const f32x4*>(&x.delta[16 * t + 4 * g]);
-            p_and_ds<T, CAP, BIAS>(sc, (float)(16 * t + 4 * g - own), f32x4{0, 1, 2, 3}, lse, delta, s, dp, p[u], ds[u]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int i = 16 * t + 4 * g + r;
-              const bool on = own <= i && own >= x.begin[i];
-              p[u][r] = on ? p[u][r] : 0.0f;
-              ds[u][r] = on ? ds[u][r] : 0.0f;
-            }
-          }
-          const Frag<T> pf = round_frag<T>(join(p[0], p[1])), f = round_frag<T>(join(ds[0], ds[1]));
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            mma(dv[d], load_col(x.go, LD, 32 * c, 16 * d, lane), pf);
-            mma(dk[d], load_col(x.q, LD, 32 * c, 16 * d, lane), f);
-          }
+        for (int d = 0; d < D / 16; ++d) {
+          mma(dv[d], load_col(x.go, LD, 32 * c, 16 * d, lane), pf);
+          mma(dk[d], load_col(x.q, LD, 32 * c, 16 * d, lane), f);
         }
-    }
+      }
   }
   if (own >= a.steps) return;
   T *ok = row_out<T>(a.dk, e, own, hk), *ov = row_out<T>(a.dv, e, own, hk);
@@ -914,10 +913,10 @@ __global__ __launch_bounds__(256) void act_env_kernel(bsg_attention_act a, int w
   if (threadIdx.x == 0) a.steps[e] = steps_after(n);
 }
 
-// Long rings and few envs: `splits` workgroups of four waves share an item's slots and leave
-// their maximum, sum and output in the workspace; a second launch joins them.
+// Long rings and few envs: `splits` workgroups of four waves share the slots that an item holds, in
+// even parts, and leave their maximum, sum and output in the workspace; a second launch joins them.
 template <class T, int D, int G, bool CAP>
-__global__ __launch_bounds__(256) void act_split_kernel(bsg_attention_act a, int splits, int span, int subs) {
+__global__ __launch_bounds__(256) void act_split_kernel(bsg_attention_act a, int splits, int subs) {
   typedef Act<T, D, G, CAP> A;
   constexpr int EPL = A::EPL;
   __shared__ float sm[4][G], ss[4][G], sa[4][G][D];
@@ -926,7 +925,7 @@ __global__ __launch_bounds__(256) void act_split_kernel(bsg_attention_act a, int
   const int items = a.heads_k * subs, item = ei % items, e = ei / items;
   const int group = a.heads_q / a.heads_k;
   const int hk = item / subs, sub = item % subs, h0 = hk * group + sub * G, heads = min(G, group - sub * G);
-  const int n = steps_before(a, e), all = min(n, a.slots);
+  const int n = steps_before(a, e), all = min(n, a.slots), span = (all + splits - 1) / splits;
   const int lo = min(split * span, all), hi = min(lo + span, all);
   Seen<G, EPL> x;
   A::see(x, a, e, hk, h0, heads, n, lo, hi, w, 4, split == 0 && w == 0, lane);
@@ -962,37 +961,46 @@ __global__ __launch_bounds__(256) void act_split_kernel(bsg_attention_act a, int
   }
 }
 
+// A workgroup per env and query head: a split's weight per thread, then the values by rows of D threads.
+constexpr int MAX_SPLITS = 256;
 template <class T, int D>
 __global__ __launch_bounds__(256) void act_join_kernel(bsg_attention_act a, int splits) {
-  __shared__ float sacc[256], sbase[256];
-  const int h = blockIdx.x % a.heads_q, e = blockIdx.x / a.heads_q;
+  __shared__ float weight[MAX_SPLITS], acc[256], top4[4], sum4[4];
+  const int h = blockIdx.x % a.heads_q, e = blockIdx.x / a.heads_q, tid = threadIdx.x;
   const float* p = static_cast<const float*>(a.work) + ((int64_t)e * a.heads_q + h) * splits * (D + 2);
+  const float mx = tid < splits ? p[tid * (D + 2) + D] : -INFINITY, sm = tid < splits ? p[tid * (D + 2) + D + 1] : 0.0f;
+  float top = mx;
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (tid % 64 == 0) top4[tid / 64] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));   // split 0 saw the step itself
+  const float f = __builtin_amdgcn_exp2f(mx - top);
+  weight[tid] = f;
+  float sum = sm * f;
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) sum += __shfl_xor(sum, d);
+  if (tid % 64 == 0) sum4[tid / 64] = sum;
+  __syncthreads();
   constexpr int P = 256 / D;                     // threads that share a value's splits
-  const int c = threadIdx.x % D, part = threadIdx.x / D;
-  float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, p[s * (D + 2) + D]);   // split 0 saw the step itself
-  float sum = 0.0f, acc = 0.0f;
-  for (int s = part; s < splits; s += P) {
-    const float f = __builtin_amdgcn_exp2f(p[s * (D + 2) + D] - top);
-    sum += p[s * (D + 2) + D + 1] * f;
-    acc += p[s * (D + 2) + c] * f;
-  }
-  sacc[threadIdx.x] = acc;
-  sbase[threadIdx.x] = sum;
+  const int c = tid % D, part = tid / D;
+  float x = 0.0f;
+#pragma unroll 8
+  for (int s = part; s < splits; s += P) x = fmaf(p[s * (D + 2) + c], weight[s], x);
+  acc[tid] = x;
   __syncthreads();
   if (part == 0) {
-    for (int i = 1; i < P; ++i) {
-      acc += sacc[i * D + c];
-      sum += sbase[i * D + c];
-    }
-    row_out<T>(a.out, e, 0, h)[c] = (T)(acc / sum);
+#pragma unroll
+    for (int i = 1; i < P; ++i) x += acc[i * D + c];
+    row_out<T>(a.out, e, 0, h)[c] = (T)(x / ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])));
   }
-  if (h == 0 && threadIdx.x == 0) a.steps[e] = steps_after(steps_before(a, e));
+  if (h == 0 && tid == 0) a.steps[e] = steps_after(steps_before(a, e));
 }
 
-// How an acting step is split: enough workgroups of four waves for every CU to hold four, none
-// with fewer than 256 slots.  One workgroup per env (no second launch) where that is one split.
-struct Plan { int g, subs, wpi, splits, span; };
+// How an acting step is split: two workgroups of four waves to a CU, which is what its registers
+// hold (one more makes a second round of a few), none with fewer than 256 slots of a full ring.  One
+// workgroup per env (no second launch) where that is one split.
+struct Plan { int g, subs, wpi, splits; };
 Plan plan_of(const bsg_attention_act& a) {
   Plan p;
   const int group = a.heads_q / a.heads_k;
@@ -1000,11 +1008,11 @@ Plan plan_of(const bsg_attention_act& a) {
   p.subs = (group + p.g - 1) / p.g;
   const int64_t items = (int64_t)a.heads_k * p.subs;
   p.wpi = items == 1 ? 4 : items == 2 ? 2 : 1;
-  const int64_t want = (1024 + a.num_envs * items - 1) / (a.num_envs * items);
+  const int64_t want = 512 / (a.num_envs * items);
   const int64_t most = a.slots / 256;
   p.splits = (int)(want < most ? want : most);
+  if (p.splits > MAX_SPLITS) p.splits = MAX_SPLITS;
   if (p.splits < 2) p.splits = 1;
-  p.span = (a.slots + p.splits - 1) / p.splits;
   return p;
 }
 
@@ -1014,7 +1022,7 @@ hipError_t act(const bsg_attention_act& a, const Plan& p, hipStream_t st) {
     act_env_kernel<T, D, G, CAP><<<dim3(a.num_envs), dim3(256), 0, st>>>(a, p.wpi, p.subs);
   } else {
     act_split_kernel<T, D, G, CAP><<<dim3(a.num_envs * a.heads_k * p.subs * p.splits), dim3(256), 0, st>>>(
-        a, p.splits, p.span, p.subs);
+        a, p.splits, p.subs);
     act_join_kernel<T, D><<<dim3(a.num_envs * a.heads_q), dim3(256), 0, st>>>(a, p.splits);
   }
   return hipGetLastError();

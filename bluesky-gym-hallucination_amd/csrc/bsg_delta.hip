@@ -602,8 +602,13 @@ __global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
     }
     return;
   }
-  stage<T, DK, C>(s.k, row<T>(a.k, e, t0, hk), a.k.step, rows, tid, NT);
-  stage<T, DK, C>(s.q, row<T>(a.q, e, t0, hk), a.q.step, rows, tid, NT);
+  {
+    Fetch<T, C, DK, NT> fk, fq;
+    fk.load(row<T>(a.k, e, t0, hk), a.k.step, rows, tid);
+    fq.load(row<T>(a.q, e, t0, hk), a.q.step, rows, tid);
+    fk.store(s.k, rows, tid);
+    fq.store(s.q, rows, tid);
+  }
 
   // one slice on its way from memory: the next is loaded while this one is computed
   constexpr int GV = Vec<T>::n, GROW = SL / GV;

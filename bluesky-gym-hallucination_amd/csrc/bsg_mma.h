@@ -174,20 +174,6 @@ __device__ __forceinline__ float max_groups(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Copies `rows` rows of `n` T's (16-byte aligned, `stride` apart) into an LDS tile of `all`
-// rows; the rows behind `rows` become zeros.  All `nt` threads of the workgroup call it.
-template <class T, int N, int ALL>
-__device__ __forceinline__ void stage(T* s, const T* p, int64_t stride, int rows, int tid, int nt) {
-  constexpr int V = Vec<T>::n, C = N / V;
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  for (int i = tid; i < ALL * C; i += nt) {
-    const int r = i / C, c = i % C * V;
-    u32x4 x = {0, 0, 0, 0};
-    if (r < rows) x = *reinterpret_cast<const u32x4*>(p + r * stride + c);
-    *reinterpret_cast<u32x4*>(s + r * pitch<T>(N) + c) = x;
-  }
-}
-
 // An R x N tile on its way from memory to LDS through registers: loaded while the one before it is
 // computed.  Rows behind `rows` (at least 1) become zeros; in their place the last one is read.
 template <class T, int R, int N, int NT>
