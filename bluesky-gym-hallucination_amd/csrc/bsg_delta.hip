@@ -134,8 +134,22 @@ __device__ __forceinline__ void make_gates(Gates& s, const RawGates& raw, bool h
   s.episode[lane] = ep;
   if (lane == 0) s.across = all == 0 ? __builtin_amdgcn_exp2f((float)last) : 0.0f;
 }
-__device__ __forceinline__ float decay(const Gates& s, int i, int j) {
-  return s.episode[i] == s.episode[j] ? __builtin_amdgcn_exp2f((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j])) : 0.0f;
+// G_ij of four rows i = row..row + 3 and the step j (FROM: of the rows j and the step i), for i >= j;
+// no branch: another episode's exponent is lowered until nothing is left.
+struct Step { float hi, lo; int episode; };
+__device__ __forceinline__ Step step_of(const Gates& s, int i) { return {s.hi[i], s.lo[i], s.episode[i]}; }
+template <bool FROM>
+__device__ __forceinline__ f32x4 decays(const Gates& s, int row, const Step& o) {
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
+  const f32x4 hi = *reinterpret_cast<const f32x4*>(&s.hi[row]), lo = *reinterpret_cast<const f32x4*>(&s.lo[row]);
+  const i32x4 ep = *reinterpret_cast<const i32x4*>(&s.episode[row]);
+  f32x4 f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float x = FROM ? (o.hi - hi[r]) + (o.lo - lo[r]) : (hi[r] - o.hi) + (lo[r] - o.lo);
+    f[r] = __builtin_amdgcn_exp2f(ep[r] == o.episode ? x : -1e9f);
+  }
+  return f;
 }
 
 // A workgroup of NW waves handles one env and value head; wave w owns the 16 value columns
@@ -225,12 +239,13 @@ __device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& s, const Gates& ga
       mma(qk, load_run(s.q + (16 * b + m) * LD, 32 * c, g), kj);
     }
     const float bj = gates.beta[j];
+    const f32x4 bi = *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);
+    const f32x4 f = decays<false>(gates, 16 * b + 4 * g, step_of(gates, j));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * b + 4 * g + r;
-      const float f = decay(gates, i, j);
-      s.n[i * AP + j] = j < i ? -(BACK ? gates.beta[i] : bj) * f * kk[r] : 0.0f;
-      float y = j <= i ? scale * f * qk[r] : 0.0f;
+      s.n[i * AP + j] = j < i ? -(BACK ? bi[r] : bj) * f[r] * kk[r] : 0.0f;
+      float y = j <= i ? scale * f[r] * qk[r] : 0.0f;
 #pragma unroll
       for (int o = 0; o < Parts<T, 2>::n; ++o) {
         const T z = (T)y;
@@ -576,45 +591,31 @@ struct Inside {
 };
 
 // Eight waves: 0..3 hold the 16 steps of tile w as they read the state (q', kr'), 4..7 those of tile
-// w - 4 as they write it (kw').
-template <class T, int DK, bool SHARED>
-__global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
+// w - 4 as they write it (kw').  The two run code of their own between the same barriers, so that
+// neither pays for the other's registers: two workgroups to a CU where LDS holds two and no sums over
+// shared heads take their registers (four waves a SIMD cover each other's loads), else one, which
+// loads a slice ahead.
+template <class T, int DK, bool SHARED> constexpr bool two_groups() { return !SHARED && 2 * sizeof(Inside<T, DK>) <= 160 * 1024; }
+
+template <class T, int DK, bool SHARED, bool READER>
+__device__ __forceinline__ void chunk_gradient(Inside<T, DK>& s, int ch, int hk, int e) {
   constexpr int LD = pitch<T>(DK), DT = DK / 16, GL = pitch<T>(SL), NT = 512;
-  constexpr int NS = DK * SL / 4 / NT;           // f32x4 of a state's slice to a thread
+  constexpr int NS = DK * SL / 4 / NT > 0 ? DK * SL / 4 / NT : 1;   // f32x4 of a state's slice to a thread
+  constexpr bool AHEAD = !two_groups<T, DK, SHARED>();
   static_assert(C * SL / 4 == NT, "one f32x4 of W and of M to a thread");
-  __shared__ __align__(16) Inside<T, DK> s;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), tile = w & 3;
-  const bool reader = w < 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), own = 16 * (w & 3) + m, tile = w & 3;
   const bsg_delta& a = arguments();
   const int chunks = (a.steps + C - 1) / C, group = a.heads_v / a.heads_k, DV = a.dim_v;
+  const int t0 = ch * C, rows = min(C, steps_of(a, e) - t0);
   const float scale = a.scale;
   const bool half = a.gate_dtype == BSG_BF16;
-  const int ch = blockIdx.x % chunks, ehk = blockIdx.x / chunks, hk = ehk % a.heads_k, e = ehk / a.heads_k;
-  const int n = steps_of(a, e), t0 = ch * C, rows = min(C, n - t0), all = min(C, a.steps - t0);
-  const int own = 16 * tile + m;
-  if (rows <= 0) {                 // padding
-    const Steps<T> dqs = steps_in<T>(a.dq, e, hk), dks = steps_in<T>(a.dk, e, hk);
-    for (int i = tid; i < all * DK; i += NT) dqs.at(t0 + i / DK)[i % DK] = dks.at(t0 + i / DK)[i % DK] = (T)0.0f;
-    for (int i = tid; i < all * group; i += NT) {
-      gate_out(a.dg, a.gate_dtype, e, t0 + i / group, hk * group + i % group, 0.0f);
-      gate_out(a.dbeta, a.gate_dtype, e, t0 + i / group, hk * group + i % group, 0.0f);
-    }
-    return;
-  }
-  {
-    Fetch<T, C, DK, NT> fk, fq;
-    fk.load(row<T>(a.k, e, t0, hk), a.k.step, rows, tid);
-    fq.load(row<T>(a.q, e, t0, hk), a.q.step, rows, tid);
-    fk.store(s.k, rows, tid);
-    fq.store(s.q, rows, tid);
-  }
 
-  // one slice on its way from memory: the next is loaded while this one is computed
+  // one slice on its way from memory to LDS
   constexpr int GV = Vec<T>::n, GROW = SL / GV;
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  u32x4 fgo;
-  f32x4 fw, fm, fs[NS > 0 ? NS : 1], fd[NS > 0 ? NS : 1];
+  u32x4 fgo = {0, 0, 0, 0};
+  f32x4 fw, fm, fs[NS], fd[NS];
   const auto fetch = [&](int h, int v0) {
     const bsg_delta& a = arguments();
     const int64_t ehc = ((int64_t)e * a.heads_v + h) * chunks + ch;
@@ -624,13 +625,13 @@ __global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
     fw = *reinterpret_cast<const f32x4*>(a.kept_w + at);
     fm = *reinterpret_cast<const f32x4*>(a.work_w + at);
 #pragma unroll
-    for (int i = 0; i < (NS > 0 ? NS : 1); ++i)
-      if (NS > 0 || tid < DK * SL / 4) {
+    for (int i = 0; i < NS; ++i)
+      if (DK * SL / 4 >= NT || tid < DK * SL / 4) {
         fs[i] = *reinterpret_cast<const f32x4*>(a.kept_states + as + i * 4 * NT);
         fd[i] = *reinterpret_cast<const f32x4*>(a.work_states + as + i * 4 * NT);
       }
   };
-  fetch(hk * group, 0);
+  if (AHEAD) fetch(hk * group, 0);
 
   f32x4 sum1[DT], sum2[DT];        // over the value heads: q', kr' (readers); kw' (writers)
 #pragma unroll
@@ -644,40 +645,43 @@ __global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
     for (int d = 0; d < DT; ++d) X1[d] = X2[d] = f32x4{0, 0, 0, 0};
     float dbeta = 0.0f, sd = 0.0f;
     RawGates raw = {0, 0, 0};
-    if (w == 0) raw = load_gates(GateSteps(arguments(), e, h), t0, rows, lane);
+    if (READER && w == 0) raw = load_gates(GateSteps(arguments(), e, h), t0, rows, lane);
     for (int v0 = 0; v0 < DV; v0 += SL) {
+      if (!AHEAD) fetch(h, v0);
       __syncthreads();             // the slice before is done with
-      if (v0 == 0 && w == 0) make_gates(s.gates, raw, half, lane);
+      if (READER && v0 == 0 && w == 0) make_gates(s.gates, raw, half, lane);
       if (tid < C * GROW)
         *reinterpret_cast<u32x4*>(&s.go[tid / GROW * GL + tid % GROW * GV]) = tid / GROW < rows ? fgo : u32x4{0, 0, 0, 0};
       s.w.put(tid / 64 % 4, tid / 256, lane, fw);
       s.mu.put(tid / 64 % 4, tid / 256, lane, fm);
 #pragma unroll
-      for (int i = 0; i < (NS > 0 ? NS : 1); ++i)
-        if (NS > 0 || tid < DK * SL / 4) {
+      for (int i = 0; i < NS; ++i)
+        if (DK * SL / 4 >= NT || tid < DK * SL / 4) {
           const int at = (tid + i * NT) / 64;
           s.st.put(at % DT, at / DT, lane, fs[i]);
           s.ds.put(at % DT, at / DT, lane, fd[i]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) sd = fmaf(fs[i][j], fd[i][j], sd);
         }
-      if (v0 + SL < DV) fetch(h, v0 + SL);
-      else if (SHARED && h < last) fetch(h + 1, 0);
+      if (AHEAD) {
+        if (v0 + SL < DV) fetch(h, v0 + SL);
+        else if (SHARED && h < last) fetch(h + 1, 0);
+      }
       __syncthreads();
       const WideOf<T, 2> wf = s.w.get(own, g);
-      if (reader) {
+      if (READER) {
         const Frag<T> go = load_run(s.go + own * GL, 0, g);
         const WideOf<T, 2> mf = s.mu.get(own, g);
         const f32x8 wx = whole(wf), mx = whole(mf);
 #pragma unroll
         for (int j = 0; j < 8; ++j) dbeta = fmaf(wx[j], mx[j], dbeta);
+        // (tiles behind the own one too: cheaper than a branch, and masked below)
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-          if (b <= tile) {
-            const WideOf<T, 2> x = s.w.get(16 * b + m, g);
-            mma<T>(ow[b], x, go);
-            mma<T>(mw[b], x, mf);
-          }
+        for (int b = 0; b < 4; ++b) {
+          const WideOf<T, 2> x = s.w.get(16 * b + m, g);
+          mma<T>(ow[b], x, go);
+          mma<T>(mw[b], x, mf);
+        }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const WideOf<T, 2> x = s.st.get(16 * d + m, g);
@@ -686,38 +690,39 @@ __global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
         }
       } else {
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-          if (b >= tile) {
-            mma<T>(ow[b], load_run(s.go + (16 * b + m) * GL, 0, g), wf);
-            mma<T>(mw[b], s.mu.get(16 * b + m, g), wf);
-          }
+        for (int b = 0; b < 4; ++b) {
+          mma<T>(ow[b], load_run(s.go + (16 * b + m) * GL, 0, g), wf);
+          mma<T>(mw[b], s.mu.get(16 * b + m, g), wf);
+        }
 #pragma unroll
         for (int d = 0; d < DT; ++d) mma<T>(X1[d], s.ds.get(16 * d + m, g), wf);
       }
     }
     // scale by the gates of the wave's own step (its lane) and add the chunk's own terms
     const Gates& G = s.gates;
+    const Step me = step_of(G, own);
     const float bi = G.beta[own], in = G.in[own], out = G.out[own], across = G.across;
     float y = 0.0f, dc = 0.0f;
-    if (reader) {
+    if (READER) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        X1[d] *= scale * in;
-        X2[d] *= -bi * in;
+        X1[d] *= in;
+        X2[d] *= in;
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c)
         if (2 * c <= tile) {       // rows j of tiles 2c, 2c + 1 against the own step i
           f32x4 f1[2], f2[2];
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < 2; ++u) {
+            const int row = 16 * (2 * c + u) + 4 * g;
+            const f32x4 f = decays<true>(G, row, me) * *reinterpret_cast<const f32x4*>(&G.beta[row]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int j = 16 * (2 * c + u) + 4 * g + r;
-              const float f = j <= own ? decay(G, own, j) * G.beta[j] : 0.0f;
-              f1[u][r] = scale * f * ow[2 * c + u][r];
-              f2[u][r] = j < own ? -bi * f * mw[2 * c + u][r] : 0.0f;
+              f1[u][r] = row + r <= own ? f[r] * ow[2 * c + u][r] : 0.0f;
+              f2[u][r] = row + r < own ? f[r] * mw[2 * c + u][r] : 0.0f;
             }
+          }
           WideOf<T, 2> w1, w2;
           split(w1, join(f1[0], f1[1]));
           split(w2, join(f2[0], f2[1]));
@@ -732,23 +737,25 @@ __global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const f32x4 k = widen(*reinterpret_cast<const Half<T>*>(&s.k[own * LD + 16 * d + 4 * g]));
-        X1[d] *= out * bi;
+        X1[d] *= out;
 #pragma unroll
         for (int r = 0; r < 4; ++r) y = fmaf(k[r], X1[d][r], y);
       }
+      y *= bi;
 #pragma unroll
       for (int c = 0; c < 2; ++c)
         if (2 * c + 1 >= tile) {   // rows i of tiles 2c, 2c + 1 against the own step j
           f32x4 f1[2], f2[2];
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < 2; ++u) {
+            const int row = 16 * (2 * c + u) + 4 * g;
+            const f32x4 f = decays<false>(G, row, me), bm = f * *reinterpret_cast<const f32x4*>(&G.beta[row]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int i = 16 * (2 * c + u) + 4 * g + r;
-              const float f = i >= own ? decay(G, i, own) * bi : 0.0f;
-              f1[u][r] = scale * f * ow[2 * c + u][r];
-              f2[u][r] = i > own ? -G.beta[i] * f * mw[2 * c + u][r] : 0.0f;
+              f1[u][r] = row + r >= own ? scale * f[r] * ow[2 * c + u][r] : 0.0f;
+              f2[u][r] = row + r > own ? -bm[r] * mw[2 * c + u][r] : 0.0f;
             }
+          }
           WideOf<T, 2> w1, w2;
           split(w1, join(f1[0], f1[1]));
           split(w2, join(f2[0], f2[1]));
@@ -762,35 +769,33 @@ __global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const f32x4 k = widen(*reinterpret_cast<const Half<T>*>(&s.k[own * LD + 16 * d + 4 * g]));
-      if (reader) {
+      X1[d] *= READER ? scale : bi;
+      if (READER) {
         const f32x4 q = widen(*reinterpret_cast<const Half<T>*>(&s.q[own * LD + 16 * d + 4 * g]));
+        X2[d] *= -bi;
 #pragma unroll
         for (int r = 0; r < 4; ++r) dc = fmaf(q[r], X1[d][r], fmaf(k[r], X2[d][r], dc));
+        sum2[d] = SHARED ? sum2[d] + X2[d] : X2[d];
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) dc = fmaf(-k[r], X1[d][r], dc);
       }
-      if (SHARED) {
-        sum1[d] += X1[d];
-        sum2[d] += X2[d];
-      } else {
-        sum1[d] = X1[d];
-        sum2[d] = X2[d];
-      }
+      sum1[d] = SHARED ? sum1[d] + X1[d] : X1[d];
     }
     dc = sum_groups(dc);
-    dbeta = sum_groups(dbeta);
     // the chunk's last step: across <S, D> + sum_j k_j.(out_j D u_j)
     y += across * sd;
 #pragma unroll
     for (int d = 32; d >= 1; d /= 2) y += __shfl_xor(y, d);
-    if (g == 0) s.dc[reader ? 0 : 1][own] = dc;
+    if (g == 0) s.dc[READER ? 0 : 1][own] = dc;
     if (lane == 0) s.part[w] = y;
     const bsg_delta& a = arguments();
-    if (reader && g == 0 && t0 + own < a.steps)
-      gate_out(a.dbeta, a.gate_dtype, e, t0 + own, h, own < rows ? dbeta : 0.0f);
+    if (READER) {
+      dbeta = sum_groups(dbeta);
+      if (g == 0 && t0 + own < a.steps) gate_out(a.dbeta, a.gate_dtype, e, t0 + own, h, own < rows ? dbeta : 0.0f);
+    }
     __syncthreads();
-    if (w == 0) {
+    if (READER && w == 0) {
       float x = s.dc[0][lane] + s.dc[1][lane];
       if (lane == 63)
 #pragma unroll
@@ -807,20 +812,48 @@ __global__ __launch_bounds__(512, 2) void backward_chunk_kernel(bsg_delta) {
         gate_out(a.dg, a.gate_dtype, e, t0 + lane, h, lane < rows && ep == before ? x : 0.0f);
     }
   }
-  if (!reader) {                   // the last slice is done with: every wave has passed the barrier above
+  if (!READER) {                   // the last slice is done with: every wave has passed the barrier above
 #pragma unroll
     for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&s.kw[own * (DK + 4) + 16 * d + 4 * g]) = sum1[d];
   }
   __syncthreads();
-  const bsg_delta& b = arguments();
-  if (!reader || t0 + own >= b.steps) return;
-  T *oq = row_out<T>(b.dq, e, t0 + own, hk), *ok = row_out<T>(b.dk, e, t0 + own, hk);
+  const bsg_delta& z = arguments();
+  if (!READER || t0 + own >= z.steps) return;
+  T *oq = row_out<T>(z.dq, e, t0 + own, hk), *ok = row_out<T>(z.dk, e, t0 + own, hk);
 #pragma unroll
   for (int d = 0; d < DT; ++d) {
     const f32x4 kw = *reinterpret_cast<const f32x4*>(&s.kw[own * (DK + 4) + 16 * d + 4 * g]);
     store4(oq + 16 * d + 4 * g, own < rows ? sum1[d] : f32x4{0, 0, 0, 0});
     store4(ok + 16 * d + 4 * g, own < rows ? sum2[d] + kw : f32x4{0, 0, 0, 0});
   }
+}
+
+template <class T, int DK, bool SHARED>
+__global__ __launch_bounds__(512, (two_groups<T, DK, SHARED>() ? 4 : 2)) void backward_chunk_kernel(bsg_delta) {
+  constexpr int NT = 512;
+  __shared__ __align__(16) Inside<T, DK> s;
+  const bsg_delta& a = arguments();
+  const int tid = threadIdx.x, chunks = (a.steps + C - 1) / C, group = a.heads_v / a.heads_k;
+  const int ch = blockIdx.x % chunks, ehk = blockIdx.x / chunks, hk = ehk % a.heads_k, e = ehk / a.heads_k;
+  const int t0 = ch * C, rows = min(C, steps_of(a, e) - t0), all = min(C, a.steps - t0);
+  if (rows <= 0) {                 // padding
+    const Steps<T> dqs = steps_in<T>(a.dq, e, hk), dks = steps_in<T>(a.dk, e, hk);
+    for (int i = tid; i < all * DK; i += NT) dqs.at(t0 + i / DK)[i % DK] = dks.at(t0 + i / DK)[i % DK] = (T)0.0f;
+    for (int i = tid; i < all * group; i += NT) {
+      gate_out(a.dg, a.gate_dtype, e, t0 + i / group, hk * group + i % group, 0.0f);
+      gate_out(a.dbeta, a.gate_dtype, e, t0 + i / group, hk * group + i % group, 0.0f);
+    }
+    return;
+  }
+  {
+    Fetch<T, C, DK, NT> fk, fq;
+    fk.load(row<T>(a.k, e, t0, hk), a.k.step, rows, tid);
+    fq.load(row<T>(a.q, e, t0, hk), a.q.step, rows, tid);
+    fk.store(s.k, rows, tid);
+    fq.store(s.q, rows, tid);
+  }
+  if (__builtin_amdgcn_readfirstlane(tid >> 6) < 4) chunk_gradient<T, DK, SHARED, true>(s, ch, hk, e);
+  else chunk_gradient<T, DK, SHARED, false>(s, ch, hk, e);
 }
 
 // ---- acting --------------------------------------------------------------------------------
