@@ -98,7 +98,7 @@ EXPORTED_SYMBOLS = (
     "bsg_comm_all_reduce", "bsg_set_params", "bsg_trajectory_bytes", "bsg_set_trajectory",
     "bsg_trajectory_info", "bsg_delta_forward", "bsg_delta_backward", "bsg_delta_step",
     "bsg_attention_forward", "bsg_attention_backward", "bsg_attention_step_bytes",
-    "bsg_attention_step", "bsg_attention_parts_bytes",
+    "bsg_attention_step", "bsg_attention_parts_bytes", "bsg_delta_work_bytes",
 )
 TRAJ_SYNC = 1                # include/bsg.h BSG_TRAJ_SYNC
 # include/bsg.h BSG_MP_*: MergeEnv-v0's module constants (merge_env.py:13-46), in this order,
@@ -143,7 +143,7 @@ class BsgDelta(C.Structure):
         [("scale", C.c_float), ("reserved", C.c_int32)] + \
         [(n, BsgRows) for n in ("q", "k", "v", "g", "beta", "out")] + \
         [("first", C.c_void_p), ("first_env", C.c_int64), ("first_step", C.c_int64)] + \
-        [(n, C.c_void_p) for n in ("lengths", "state", "final_state", "kept_states", "kept_w")] + \
+        [(n, C.c_void_p) for n in ("lengths", "state", "final_state", "kept_states", "kept_w", "work")] + \
         [(n, BsgRows) for n in ("dout", "dq", "dk", "dv", "dg", "dbeta")] + \
         [(n, C.c_void_p) for n in ("dfinal", "dstate", "work_states", "work_w")]
 
@@ -282,7 +282,7 @@ def load_library(path: str | None = None):
                "bsg_attention_backward", "bsg_attention_step"):
         getattr(lib, fn).restype = C.c_int32
         getattr(lib, fn).argtypes = [C.c_void_p, C.c_void_p]
-    for fn in ("bsg_attention_parts_bytes", "bsg_attention_step_bytes"):
+    for fn in ("bsg_attention_parts_bytes", "bsg_attention_step_bytes", "bsg_delta_work_bytes"):
         getattr(lib, fn).restype = C.c_int64
         getattr(lib, fn).argtypes = [C.c_void_p]
     if lib.bsg_abi_version() != ABI_VERSION:

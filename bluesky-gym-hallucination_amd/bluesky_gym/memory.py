@@ -191,6 +191,16 @@ def _delta_check(who, q, k, v, g, beta, state, first, lead):
         _shape(who, "first", first, lead, _FLAGS)
 
 
+def _with_work(fn, before, after, dev):
+    """The call with the fields around bsg_delta.work, and the scratch that it wants there."""
+    block = _pack_delta(*before, 0, *after)
+    need = nat.load_library().bsg_delta_work_bytes(block)
+    if need > 0:
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        block = _pack_delta(*before, work.data_ptr(), *after)
+    _call(fn, block, dev)
+
+
 class _DeltaRule(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, first, lengths, scale, dtype, keep):
@@ -205,9 +215,9 @@ class _DeltaRule(torch.autograd.Function):
             n = -(-T // nat.DELTA_CHUNK)
             states = torch.empty((E, H, n, Dk, Dv), dtype=torch.float32, device=dev)
             w = torch.empty((E, H, n * nat.DELTA_CHUNK, Dv), dtype=torch.float32, device=dev)
-        _call("bsg_delta_forward", _pack_delta(
+        _with_work("bsg_delta_forward", (
             *_delta_inputs(dtype, scale, q, k, v, g, beta, _rows(out), first, lengths), _ptr(state), final.data_ptr(),
-            _ptr(states), _ptr(w), *_NO_ROWS * 6, 0, 0, 0, 0), dev)
+            _ptr(states), _ptr(w)), (*_NO_ROWS * 6, 0, 0, 0, 0), dev)
         if keep:
             ctx.save_for_backward(q, k, v, g, beta, first, lengths, states, w)
             ctx.rest = scale, dtype
@@ -227,10 +237,10 @@ class _DeltaRule(torch.autograd.Function):
         if ctx.needs_input_grad[5]:
             dstate = torch.empty((v.shape[0], v.shape[2], q.shape[-1], v.shape[-1]), dtype=torch.float32, device=v.device)
         ws, ww = torch.empty_like(states), torch.empty_like(w)
-        _call("bsg_delta_backward", _pack_delta(
+        _with_work("bsg_delta_backward", (
             *_delta_inputs(dtype, scale, q, k, v, g, beta, _NO_ROWS, first, lengths), 0, 0, states.data_ptr(),
-            w.data_ptr(), *_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv), *_rows(dg), *_rows(db), _ptr(dfinal),
-            _ptr(dstate), ws.data_ptr(), ww.data_ptr()), v.device)
+            w.data_ptr()), (*_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv), *_rows(dg), *_rows(db), _ptr(dfinal),
+                            _ptr(dstate), ws.data_ptr(), ww.data_ptr()), v.device)
         return dq, dk, dv, dg, db, dstate, None, None, None, None, None
 
 

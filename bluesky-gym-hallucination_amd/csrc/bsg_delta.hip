@@ -82,8 +82,8 @@ template <class T> struct Steps {
   int64_t step;
   __device__ __forceinline__ T* at(int t) const { return p + t * step; }
 };
-template <class T> __device__ __forceinline__ Steps<T> steps_in(const bsg_rows& x, int e, int h) {
-  return {static_cast<T*>(x.p) + e * x.env + h * x.head, x.step};
+template <class T> __device__ __forceinline__ Steps<T> steps_in(const bsg_rows& x, int e, int h, int col = 0) {
+  return {static_cast<T*>(x.p) + e * x.env + h * x.head + col, x.step};
 }
 struct GateSteps {
   const char *g, *beta;
@@ -152,14 +152,10 @@ __device__ __forceinline__ f32x4 decays(const Gates& s, int row, const Step& o) 
   return f;
 }
 
-// A workgroup of NW waves handles one env and value head; wave w owns the 16 value columns
-// 16 w .. 16 w + 15 and keeps their part of the state in registers (as D tiles, whose rows are the
-// key dimension), so the waves only meet over the C x C matrices.
-template <class T, int DK, int NW>
-struct Chunk {
-  static constexpr int LD = pitch<T>(DK), VD = pitch<T>(16 * NW), PD = pitch<T>(C), parts = Parts<T, 2>::n;
-  T k[C * LD], q[C * LD];
-  T v[C * VD];                     // v (dout), then, column by column, out (v')
+// What the passes along a rollout need of a chunk besides its rows.
+template <class T>
+struct Solved {
+  static constexpr int PD = pitch<T>(C), parts = Parts<T, 2>::n;
   T p[parts][C * PD];              // P in parts of type T, zeros above its diagonal
   float n[C * AP];                 // minus the matrix of the system, below the diagonal
   float inv[4 * 16 * IP];          // inverses of the system's diagonal blocks
@@ -176,6 +172,19 @@ struct Chunk {
     for (int i = 0; i < parts; ++i) w.p[i] = load_col(p[i], PD, k0, m0, lane);
     return w;
   }
+};
+// ... of which all but the second gates pass through memory where the chunks are solved beforehand.
+template <class T> constexpr int solved_bytes() { return sizeof(Solved<T>) - sizeof(Gates); }
+
+// A workgroup of NW waves handles 16 NW value columns of one env and value head; wave w owns 16 of
+// them and keeps their part of the state in registers (as D tiles, whose rows are the key
+// dimension), so the waves only meet over the C x C matrices.
+template <class T, int DK, int NW>
+struct Chunk {
+  static constexpr int LD = pitch<T>(DK), VD = pitch<T>(16 * NW);
+  T k[C * LD], q[C * LD];
+  T v[C * VD];                     // v (dout), then, column by column, out (v')
+  Solved<T> s;
 };
 // Waves per SIMD that LDS leaves room for, two at most: what bounds the passes' registers.
 template <class T, int DK, int NW> constexpr int waves_per_simd() {
@@ -223,8 +232,9 @@ template <int J> __device__ __forceinline__ void eliminate(float (&x)[16], const
 // inverse's row lies in a lane, and its substitution takes the rows before from their lanes.
 // BACK: the system is (I + diag(beta) N)^T, else I + N diag(beta).
 template <class T, int DK, int NW, bool BACK>
-__device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& s, const Gates& gates, float scale, int lane, int w) {
+__device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& x, const Gates& gates, float scale, int lane, int w) {
   constexpr int LD = pitch<T>(DK);
+  Solved<T>& s = x.s;
   const int m = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t0 = 0; t0 < 10; t0 += NW) {
@@ -234,9 +244,9 @@ __device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& s, const Gates& ga
     f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < DK / 32; ++c) {
-      const Frag<T> kj = load_run(s.k + j * LD, 32 * c, g);
-      mma(kk, load_run(s.k + (16 * b + m) * LD, 32 * c, g), kj);
-      mma(qk, load_run(s.q + (16 * b + m) * LD, 32 * c, g), kj);
+      const Frag<T> kj = load_run(x.k + j * LD, 32 * c, g);
+      mma(kk, load_run(x.k + (16 * b + m) * LD, 32 * c, g), kj);
+      mma(qk, load_run(x.q + (16 * b + m) * LD, 32 * c, g), kj);
     }
     const float bj = gates.beta[j];
     const f32x4 bi = *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);
@@ -249,54 +259,103 @@ __device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& s, const Gates& ga
 #pragma unroll
       for (int o = 0; o < Parts<T, 2>::n; ++o) {
         const T z = (T)y;
-        s.p[o][i * Chunk<T, DK, NW>::PD + j] = z;
+        s.p[o][i * Solved<T>::PD + j] = z;
         y -= (float)z;
       }
     }
   }
   __syncthreads();
   if (w == NW - 1) {               // lane: block g, row m
-    float x[16], n[16];
+    float v[16], n[16];
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(&s.n[(16 * g + m) * AP + 16 * g + j]);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(&s.n[(16 * g + m) * AP + 16 * g + j]);
 #pragma unroll
-      for (int o = 0; o < 4; ++o) n[j + o] = v[o];
+      for (int o = 0; o < 4; ++o) n[j + o] = y[o];
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = j == m ? 1.0f : 0.0f;
-    eliminate<0>(x, n);
+    for (int j = 0; j < 16; ++j) v[j] = j == m ? 1.0f : 0.0f;
+    eliminate<0>(v, n);
 #pragma unroll
     for (int j = 0; j < 16; j += 4)
-      *reinterpret_cast<f32x4*>(&s.inv[(16 * g + m) * IP + j]) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
+      *reinterpret_cast<f32x4*>(&s.inv[(16 * g + m) * IP + j]) = f32x4{v[j], v[j + 1], v[j + 2], v[j + 3]};
   }
 }
 // P's tiles above the diagonal that share a product step with one on it
-template <class T, int DK, int NW>
-__device__ __forceinline__ void clear_above(Chunk<T, DK, NW>& s, int tid) {
-  for (int i = tid; i < 2 * 256; i += 64 * NW) {
+template <class T>
+__device__ __forceinline__ void clear_above(Solved<T>& s, int tid, int nt) {
+  for (int i = tid; i < 2 * 256; i += nt) {
     const int b = i / 256 * 32, r = i % 256 / 16, c = i % 16;
 #pragma unroll
-    for (int o = 0; o < Parts<T, 2>::n; ++o) s.p[o][(b + r) * Chunk<T, DK, NW>::PD + b + 16 + c] = (T)0.0f;
+    for (int o = 0; o < Solved<T>::parts; ++o) s.p[o][(b + r) * Solved<T>::PD + b + 16 + c] = (T)0.0f;
   }
 }
+
+// Few rows: the chunks are solved beforehand, all side by side, by workgroups of four waves.
+template <class T, int DK, bool BACK>
+__global__ __launch_bounds__(256) void solve_kernel(bsg_delta a) {
+  __shared__ __align__(16) Chunk<T, DK, 4> s;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int chunks = (a.steps + C - 1) / C, ch = blockIdx.x % chunks, eh = blockIdx.x / chunks;
+  const int h = eh % a.heads_v, e = eh / a.heads_v, hk = h / (a.heads_v / a.heads_k);
+  const int t0 = ch * C, rows = min(C, steps_of(a, e) - t0);
+  if (rows <= 0) return;
+  Fetch<T, C, DK, 256> fk, fq;
+  fk.load(row<T>(a.k, e, t0, hk), a.k.step, rows, tid);
+  fq.load(row<T>(a.q, e, t0, hk), a.q.step, rows, tid);
+  if (w == 0) {
+    const GateSteps gate(a, e, h);
+    make_gates(s.s.gates[0], load_gates(gate, t0, rows, lane), gate.half, lane);
+  }
+  clear_above(s.s, tid, 256);
+  fk.store(s.k, rows, tid);
+  fq.store(s.q, rows, tid);
+  __syncthreads();
+  solve_chunk<T, DK, 4, BACK>(s, s.s.gates[0], a.scale, lane, w);
+  __syncthreads();
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  constexpr int N = solved_bytes<T>() / 16;
+  u32x4* to = reinterpret_cast<u32x4*>(a.work) + ((int64_t)eh * chunks + ch) * N;
+  const u32x4* from = reinterpret_cast<const u32x4*>(&s.s);
+  for (int i = tid; i < N; i += 256) to[i] = from[i];
+}
+// ... and their results fetched a chunk ahead, as the rows are.
+template <class T, int NT>
+struct FetchSolved {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  static constexpr int N = solved_bytes<T>() / 16, n = (N + NT - 1) / NT;
+  u32x4 x[n];
+  __device__ __forceinline__ void load(const void* work, int64_t chunk, int tid) {
+    const u32x4* p = reinterpret_cast<const u32x4*>(work) + chunk * N;
+#pragma unroll
+    for (int i = 0; i < n; ++i) x[i] = p[min(tid + i * NT, N - 1)];
+  }
+  __device__ __forceinline__ void store(Solved<T>& s, int tid) const {
+    u32x4* p = reinterpret_cast<u32x4*>(&s);
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      if (tid + i * NT < N) p[tid + i * NT] = x[i];
+  }
+};
 
 // the first two parts: enough for what ends in an output of type T
 __device__ __forceinline__ const Wide<float, 1>& front(const Wide<float, 1>& w) { return w; }
 __device__ __forceinline__ Wide<bf16, 2> front(const Wide<bf16, 3>& w) { return Wide<bf16, 2>{{w.p[0], w.p[1]}}; }
 
 // States and W (M) that only these kernels read lie as their D tiles do: 16 bytes a lane, wave by wave.
-template <int NW> __device__ __forceinline__ float* tiles(float* p, int64_t chunk, int tiles_per_wave, int w, int lane) {
-  return p + ((chunk * NW + w) * tiles_per_wave * 64 + lane) * 4;
+__device__ __forceinline__ float* tiles(float* p, int64_t chunk, int waves, int tiles_per_wave, int w, int lane) {
+  return p + ((chunk * waves + w) * tiles_per_wave * 64 + lane) * 4;
 }
 
 // ---- forward -------------------------------------------------------------------------------
-template <class T, int DK, int NW>
-__global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void forward_kernel(bsg_delta a) {
+template <class T, int DK, int NW, bool SOLVED>
+__global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())) void forward_kernel(bsg_delta a) {
   constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW, VD = pitch<T>(DV);
   __shared__ __align__(16) Chunk<T, DK, NW> s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x % a.heads_v, e = blockIdx.x / a.heads_v, hk = h / (a.heads_v / a.heads_k);
+  // the workgroup's columns of all: all of them, but where the chunks are solved beforehand
+  const int all = SOLVED ? a.dim_v : DV, groups = all / DV, id = blockIdx.x / groups, c0 = blockIdx.x % groups * DV;
+  const int h = id % a.heads_v, e = id / a.heads_v, hk = h / (a.heads_v / a.heads_k);
   const int n = steps_of(a, e), col = 16 * w + m;
   const int chunks = (a.steps + C - 1) / C, live = (n + C - 1) / C;
   const int64_t eh = (int64_t)e * a.heads_v + h;
@@ -306,42 +365,48 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void forwar
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      S[d][r] = a.state ? a.state[(eh * DK + 16 * d + 4 * g + r) * DV + col] : 0.0f;
+      S[d][r] = a.state ? a.state[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] : 0.0f;
 
   Fetch<T, C, DK, NT> fk, fq;
   Fetch<T, C, DV, NT> fv;
+  FetchSolved<T, NT> fs;
   RawGates raw = {0, 0, 0};
-  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), v = steps_in<const T>(a.v, e, h);
-  const Steps<T> out = steps_in<T>(a.out, e, h);
+  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), v = steps_in<const T>(a.v, e, h, c0);
+  const Steps<T> out = steps_in<T>(a.out, e, h, c0);
   const GateSteps gate(a, e, h);
-  float *const ks = a.kept_states ? tiles<NW>(a.kept_states, eh * chunks, DT, w, lane) : nullptr;
-  float *const kw = a.kept_w ? tiles<NW>(a.kept_w, eh * chunks, 4, w, lane) : nullptr;
+  float *const ks = a.kept_states ? tiles(a.kept_states, eh * chunks, all / 16, DT, c0 / 16 + w, lane) : nullptr;
+  float *const kw = a.kept_w ? tiles(a.kept_w, eh * chunks, all / 16, 4, c0 / 16 + w, lane) : nullptr;
   if (live > 0) {
     fk.load(k.p, k.step, n, tid);
     fq.load(q.p, q.step, n, tid);
     fv.load(v.p, v.step, n, tid);
-    if (w == 0) make_gates(s.gates[0], load_gates(gate, 0, n, lane), gate.half, lane);
-    clear_above(s, tid);
+    if (SOLVED) fs.load(a.work, eh * chunks, tid);
+    else {
+      if (w == 0) make_gates(s.s.gates[0], load_gates(gate, 0, n, lane), gate.half, lane);
+      clear_above(s.s, tid, NT);
+    }
   }
   for (int ch = 0; ch < live; ++ch) {
     const int t0 = ch * C, rows = min(C, n - t0), t1 = t0 + C;
-    const Gates& gates = s.gates[ch & 1];
+    const Gates& gates = s.s.gates[SOLVED ? 0 : ch & 1];
     __syncthreads();               // the chunk before is done with LDS
     fk.store(s.k, rows, tid);
     fq.store(s.q, rows, tid);
     fv.store(s.v, rows, tid);
+    if (SOLVED) fs.store(s.s, tid);
     if (t1 < n) {
       fk.load(k.at(t1), k.step, n - t1, tid);
       fq.load(q.at(t1), q.step, n - t1, tid);
       fv.load(v.at(t1), v.step, n - t1, tid);
-      if (w == 0) raw = load_gates(gate, t1, n - t1, lane);
+      if (SOLVED) fs.load(a.work, eh * chunks + ch + 1, tid);
+      else if (w == 0) raw = load_gates(gate, t1, n - t1, lane);
     }
     __syncthreads();
-    solve_chunk<T, DK, NW, false>(s, gates, a.scale, lane, w);
+    if (!SOLVED) solve_chunk<T, DK, NW, false>(s, gates, a.scale, lane, w);
 
     if (ks) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(ks + (int64_t)ch * DK * DV + 256 * d) = S[d];
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(ks + (int64_t)ch * DK * all + 256 * d) = S[d];
     }
     // K S and Q S
     f32x4 x[4], o[4];
@@ -364,20 +429,22 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void forwar
       for (int r = 0; r < 4; ++r) x[b][r] = (float)s.v[(16 * b + 4 * g + r) * VD + col] - in[r] * x[b][r];
       o[b] *= in * a.scale;
     }
-    if (w == 0 && t1 < n) make_gates(s.gates[(ch + 1) & 1], raw, gate.half, lane);
-    __syncthreads();               // the inverses are there
+    if (!SOLVED) {
+      if (w == 0 && t1 < n) make_gates(s.s.gates[(ch + 1) & 1], raw, gate.half, lane);
+      __syncthreads();             // the inverses are there
+    }
     f32x4 W[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
 #pragma unroll
       for (int u = 0; u < b; ++u)
-        mma16(x[b], *reinterpret_cast<const f32x4*>(&s.n[(16 * b + m) * AP + 16 * u + 4 * g]), W[u]);
+        mma16(x[b], *reinterpret_cast<const f32x4*>(&s.s.n[(16 * b + m) * AP + 16 * u + 4 * g]), W[u]);
       W[b] = f32x4{0, 0, 0, 0};
-      mma16(W[b], *reinterpret_cast<const f32x4*>(&s.inv[(16 * b + m) * IP + 4 * g]), x[b]);
+      mma16(W[b], *reinterpret_cast<const f32x4*>(&s.s.inv[(16 * b + m) * IP + 4 * g]), x[b]);
     }
     if (kw) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) *reinterpret_cast<f32x4*>(kw + (int64_t)ch * C * DV + 256 * b) = W[b];
+      for (int b = 0; b < 4; ++b) *reinterpret_cast<f32x4*>(kw + (int64_t)ch * C * all + 256 * b) = W[b];
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) W[b] *= *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);   // U
@@ -386,7 +453,7 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void forwar
       WideOf<T, 2> uw;
       split(uw, join(W[2 * c], W[2 * c + 1]));
 #pragma unroll
-      for (int b = 2 * c; b < 4; ++b) mma<T>(o[b], s.p_row(16 * b + m, 32 * c, g), uw);
+      for (int b = 2 * c; b < 4; ++b) mma<T>(o[b], s.s.p_row(16 * b + m, 32 * c, g), uw);
     }
     put_columns<T, VD>(s.v, o, w, lane);
 #pragma unroll
@@ -408,19 +475,21 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void forwar
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) a.final_state[(eh * DK + 16 * d + 4 * g + r) * DV + col] = S[d][r];
+      for (int r = 0; r < 4; ++r) a.final_state[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] = S[d][r];
   }
 }
 
 // ---- backward along the rollout ------------------------------------------------------------
 // The gradient of the state, from the last chunk to the first, and with it M and v'.  Every
 // product's columns are value columns, so a wave works on its 16 alone, as in the forward pass.
-template <class T, int DK, int NW>
-__global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void backward_state_kernel(bsg_delta a) {
+template <class T, int DK, int NW, bool SOLVED>
+__global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())) void backward_state_kernel(bsg_delta a) {
   constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW, VD = pitch<T>(DV);
   __shared__ __align__(16) Chunk<T, DK, NW> s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x % a.heads_v, e = blockIdx.x / a.heads_v, hk = h / (a.heads_v / a.heads_k);
+  // the workgroup's columns of all: all of them, but where the chunks are solved beforehand
+  const int all = SOLVED ? a.dim_v : DV, groups = all / DV, id = blockIdx.x / groups, c0 = blockIdx.x % groups * DV;
+  const int h = id % a.heads_v, e = id / a.heads_v, hk = h / (a.heads_v / a.heads_k);
   const int n = steps_of(a, e), col = 16 * w + m;
   const int chunks = (a.steps + C - 1) / C, live = (n + C - 1) / C;
   const int64_t eh = (int64_t)e * a.heads_v + h;
@@ -430,41 +499,47 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void backwa
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      D[d][r] = a.dfinal ? a.dfinal[(eh * DK + 16 * d + 4 * g + r) * DV + col] : 0.0f;
+      D[d][r] = a.dfinal ? a.dfinal[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] : 0.0f;
 
   Fetch<T, C, DK, NT> fk, fq;
   Fetch<T, C, DV, NT> fv;
+  FetchSolved<T, NT> fs;
   RawGates raw = {0, 0, 0};
-  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), dout = steps_in<const T>(a.dout, e, h);
-  const Steps<T> dv = steps_in<T>(a.dv, e, h);
+  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), dout = steps_in<const T>(a.dout, e, h, c0);
+  const Steps<T> dv = steps_in<T>(a.dv, e, h, c0);
   const GateSteps gate(a, e, h);
-  float *const ws = tiles<NW>(a.work_states, eh * chunks, DT, w, lane), *const wm = tiles<NW>(a.work_w, eh * chunks, 4, w, lane);
+  float *const ws = tiles(a.work_states, eh * chunks, all / 16, DT, c0 / 16 + w, lane), *const wm = tiles(a.work_w, eh * chunks, all / 16, 4, c0 / 16 + w, lane);
   if (live > 0) {
     const int t0 = (live - 1) * C;
     fk.load(k.at(t0), k.step, n - t0, tid);
     fq.load(q.at(t0), q.step, n - t0, tid);
     fv.load(dout.at(t0), dout.step, n - t0, tid);
-    if (w == 0) make_gates(s.gates[(live - 1) & 1], load_gates(gate, t0, n - t0, lane), gate.half, lane);
-    clear_above(s, tid);
+    if (SOLVED) fs.load(a.work, eh * chunks + live - 1, tid);
+    else {
+      if (w == 0) make_gates(s.s.gates[(live - 1) & 1], load_gates(gate, t0, n - t0, lane), gate.half, lane);
+      clear_above(s.s, tid, NT);
+    }
   }
   for (int ch = live - 1; ch >= 0; --ch) {
     const int t0 = ch * C, rows = min(C, n - t0), t1 = t0 - C;
-    const Gates& gates = s.gates[ch & 1];
+    const Gates& gates = s.s.gates[SOLVED ? 0 : ch & 1];
     __syncthreads();               // the chunk after is done with LDS
     fk.store(s.k, rows, tid);
     fq.store(s.q, rows, tid);
     fv.store(s.v, rows, tid);
+    if (SOLVED) fs.store(s.s, tid);
     if (t1 >= 0) {
       fk.load(k.at(t1), k.step, C, tid);
       fq.load(q.at(t1), q.step, C, tid);
       fv.load(dout.at(t1), dout.step, C, tid);
-      if (w == 0) raw = load_gates(gate, t1, C, lane);
+      if (SOLVED) fs.load(a.work, eh * chunks + ch - 1, tid);
+      else if (w == 0) raw = load_gates(gate, t1, C, lane);
     }
     __syncthreads();
-    solve_chunk<T, DK, NW, true>(s, gates, a.scale, lane, w);
+    if (!SOLVED) solve_chunk<T, DK, NW, true>(s, gates, a.scale, lane, w);
 
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(ws + (int64_t)ch * DK * DV + 256 * d) = D[d];
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(ws + (int64_t)ch * DK * all + 256 * d) = D[d];
 
     f32x4 x[4], go[4];
 #pragma unroll
@@ -486,25 +561,27 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void backwa
     for (int c = 0; c < 2; ++c) {
       const Frag<T> gf = round_frag<T>(join(go[2 * c], go[2 * c + 1]));   // as it was read
 #pragma unroll
-      for (int b = 0; b < 2 * c + 2; ++b) mma<T>(x[b], s.p_col(16 * b, 32 * c, lane), gf);
+      for (int b = 0; b < 2 * c + 2; ++b) mma<T>(x[b], s.s.p_col(16 * b, 32 * c, lane), gf);
     }
-    if (w == 0 && t1 >= 0) make_gates(s.gates[(ch + 1) & 1], raw, gate.half, lane);
-    __syncthreads();               // the inverses are there
+    if (!SOLVED) {
+      if (w == 0 && t1 >= 0) make_gates(s.s.gates[(ch + 1) & 1], raw, gate.half, lane);
+      __syncthreads();             // the inverses are there
+    }
     f32x4 M[4];
 #pragma unroll
     for (int b = 3; b >= 0; --b) {
 #pragma unroll
       for (int u = b + 1; u < 4; ++u) {
-        const float* p = &s.n[(16 * u + 4 * g) * AP + 16 * b + m];
+        const float* p = &s.s.n[(16 * u + 4 * g) * AP + 16 * b + m];
         mma16(x[b], f32x4{p[0], p[AP], p[2 * AP], p[3 * AP]}, M[u]);
       }
-      const float* p = &s.inv[(16 * b + 4 * g) * IP + m];
+      const float* p = &s.s.inv[(16 * b + 4 * g) * IP + m];
       M[b] = f32x4{0, 0, 0, 0};
       mma16(M[b], f32x4{p[0], p[IP], p[2 * IP], p[3 * IP]}, x[b]);
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      *reinterpret_cast<f32x4*>(wm + (int64_t)ch * C * DV + 256 * b) = M[b];
+      *reinterpret_cast<f32x4*>(wm + (int64_t)ch * C * all + 256 * b) = M[b];
       M[b] *= *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);
     }
     put_columns<T, VD>(s.v, M, w, lane);
@@ -534,7 +611,7 @@ __global__ __launch_bounds__(64 * NW, (waves_per_simd<T, DK, NW>())) void backwa
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) a.dstate[(eh * DK + 16 * d + 4 * g + r) * DV + col] = D[d][r];
+      for (int r = 0; r < 4; ++r) a.dstate[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] = D[d][r];
   }
 }
 
@@ -919,16 +996,35 @@ hipError_t run(const bsg_delta_act& a, bool, hipStream_t st) {
   step_kernel<T, DK, DV><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st>>>(a, waves);
   return hipGetLastError();
 }
+// Where the rows (envs x value heads) leave CUs idle, the pass along a rollout is bound by the time
+// of one chunk, and the chunks are solved beforehand, side by side (SOLVED); where they do not, solving
+// in place saves the way of the matrices through memory.
+bool solved_first(const bsg_delta& a) {
+  return a.dim_v > 32 && a.steps > C && (int64_t)a.num_envs * a.heads_v < 256;
+}
 template <class T, int DK, int NW>
 hipError_t run(const bsg_delta& a, bool back, hipStream_t st) {
   const dim3 rows((unsigned)(a.num_envs * a.heads_v));
+  if (solved_first(a)) {
+    if constexpr (NW > 2) {
+      const dim3 all((unsigned)(a.num_envs * a.heads_v * ((a.steps + C - 1) / C))), groups(rows.x * (NW / 4));
+      if (back) {
+        solve_kernel<T, DK, true><<<all, dim3(256), 0, st>>>(a);
+        backward_state_kernel<T, DK, 4, true><<<groups, dim3(256), 0, st>>>(a);
+      } else {
+        solve_kernel<T, DK, false><<<all, dim3(256), 0, st>>>(a);
+        forward_kernel<T, DK, 4, true><<<groups, dim3(256), 0, st>>>(a);
+      }
+    }
+  } else if (back) {
+    backward_state_kernel<T, DK, NW, false><<<rows, dim3(64 * NW), 0, st>>>(a);
+  } else {
+    forward_kernel<T, DK, NW, false><<<rows, dim3(64 * NW), 0, st>>>(a);
+  }
   if (back) {
-    backward_state_kernel<T, DK, NW><<<rows, dim3(64 * NW), 0, st>>>(a);
     const dim3 chunks((unsigned)(a.num_envs * a.heads_k * ((a.steps + C - 1) / C)));
     if (a.heads_v > a.heads_k) backward_chunk_kernel<T, DK, true><<<chunks, dim3(512), 0, st>>>(a);
     else backward_chunk_kernel<T, DK, false><<<chunks, dim3(512), 0, st>>>(a);
-  } else {
-    forward_kernel<T, DK, NW><<<rows, dim3(64 * NW), 0, st>>>(a);
   }
   return hipGetLastError();
 }
@@ -951,6 +1047,11 @@ namespace bsg {
 // Shapes, strides and pointers are validated by the bsg_delta_* entry points (bsg_abi.cpp).
 hipError_t launch_delta_forward(const bsg_delta& a, hipStream_t st) { return run(a, false, st); }
 hipError_t launch_delta_backward(const bsg_delta& a, hipStream_t st) { return run(a, true, st); }
+int64_t delta_work_bytes(const bsg_delta& a) {
+  if (!solved_first(a)) return 0;
+  const int64_t chunks = (int64_t)a.num_envs * a.heads_v * ((a.steps + C - 1) / C);
+  return chunks * (a.dtype == BSG_BF16 ? solved_bytes<mma::bf16>() : solved_bytes<float>());
+}
 hipError_t launch_delta_step(const bsg_delta_act& a, hipStream_t st) { return run(a, false, st); }
 
 }  // namespace bsg
