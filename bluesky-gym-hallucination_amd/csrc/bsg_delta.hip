@@ -183,7 +183,7 @@ template <class T, int DK, int NW>
 struct Chunk {
   static constexpr int LD = pitch<T>(DK), VD = pitch<T>(16 * NW);
   T k[C * LD], q[C * LD];
-  T v[C * VD];                     // v (dout), then, column by column, out (v')
+  T v[sizeof(T) == 2 ? C * VD : 4];  // bf16: v (dout), then, column by column, out (v')
   Solved<T> s;
 };
 // Waves per SIMD that LDS leaves room for, two at most: what bounds the passes' registers.
@@ -191,28 +191,70 @@ template <class T, int DK, int NW> constexpr int waves_per_simd() {
   return NW == 2 ? 1 : NW == 8 || 2 * sizeof(Chunk<T, DK, NW>) <= 160 * 1024 ? 2 : 1;
 }
 
-// A wave's 16 columns of the C x 16 NW tile: from registers (D tiles) to LDS, and from there, in
-// 16-byte pieces, to the rows in memory.  Rows behind `rows` are padding: zeros, up to `all`.
-template <class T, int VD>
-__device__ __forceinline__ void put_columns(T* s, const f32x4* x, int w, int lane) {
-  const int m = lane & 15, g = lane >> 4;
+// A wave's 16 columns of the value rows, as D tiles.  bf16 passes through LDS, so that memory sees 16
+// bytes a lane, in and out; fp32, where 16 lanes make 64 bytes of a row, goes straight to and from
+// registers, and the LDS that saves lets two workgroups share a CU.
+template <class T, int NW>
+struct Columns {
+  static constexpr int NT = 64 * NW, VD = pitch<T>(16 * NW);
+  Fetch<T, C, 16 * NW, NT> f;
+  __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int tid, int) { f.load(p, stride, rows, tid); }
+  __device__ __forceinline__ void store(T* s, int rows, int tid) { f.store(s, rows, tid); }
+  __device__ __forceinline__ void get(f32x4 (&x)[4], const T* s, int, int w, int lane) const {
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
+    for (int b = 0; b < 4; ++b)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s[(16 * b + 4 * g + r) * VD + 16 * w + m] = (T)x[b][r];
-}
-template <class T, int VD>
-__device__ __forceinline__ void write_columns(const T* s, T* to, int64_t stride, int rows, int all, int w, int lane) {
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  constexpr int V = Vec<T>::n, P = 16 / V;       // pieces to a row
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const int r = (lane + 64 * i) / P, c = 16 * w + (lane + 64 * i) % P * V;
-    u32x4 x = *reinterpret_cast<const u32x4*>(s + r * VD + c);
-    if (r >= rows) x = u32x4{0, 0, 0, 0};
-    if (r < all) *reinterpret_cast<u32x4*>(to + r * stride + c) = x;
+      for (int r = 0; r < 4; ++r) x[b][r] = (float)s[(16 * b + 4 * (lane >> 4) + r) * VD + 16 * w + (lane & 15)];
   }
-}
+  // to LDS, and from there to memory; rows behind `rows` are padding: zeros, up to `all`
+  static __device__ __forceinline__ void put(T* s, const f32x4 (&x)[4], T*, int64_t, int, int, int w, int lane) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[(16 * b + 4 * (lane >> 4) + r) * VD + 16 * w + (lane & 15)] = (T)x[b][r];
+  }
+  static __device__ __forceinline__ void write(const T* s, T* to, int64_t stride, int rows, int all, int w, int lane) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    constexpr int V = Vec<T>::n, P = 16 / V;     // pieces to a row
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int r = (lane + 64 * i) / P, c = 16 * w + (lane + 64 * i) % P * V;
+      u32x4 x = *reinterpret_cast<const u32x4*>(s + r * VD + c);
+      if (r >= rows) x = u32x4{0, 0, 0, 0};
+      if (r < all) *reinterpret_cast<u32x4*>(to + r * stride + c) = x;
+    }
+  }
+};
+template <int NW>
+struct Columns<float, NW> {
+  f32x4 next[4], now[4];
+  __device__ __forceinline__ void load(const float* p, int64_t stride, int rows, int tid, int col) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) next[b][r] = p[min(16 * b + 4 * (tid % 64 >> 4) + r, rows - 1) * stride + col];
+  }
+  __device__ __forceinline__ void store(float*, int, int) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) now[b] = next[b];
+  }
+  __device__ __forceinline__ void get(f32x4 (&x)[4], const float*, int rows, int, int lane) const {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[b][r] = 16 * b + 4 * (lane >> 4) + r < rows ? now[b][r] : 0.0f;
+  }
+  static __device__ __forceinline__ void put(float*, const f32x4 (&x)[4], float* to, int64_t stride, int rows, int all, int w, int lane) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = 16 * b + 4 * (lane >> 4) + r;
+        if (t < all) to[t * stride + 16 * w + (lane & 15)] = t < rows ? x[b][r] : 0.0f;
+      }
+  }
+  static __device__ __forceinline__ void write(const float*, float*, int64_t, int, int, int, int) {}
+};
 
 // lane j of each row of 16 lanes, to all of them
 template <int J> __device__ __forceinline__ float from_lane(float x) {
@@ -238,8 +280,7 @@ __device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& x, const Gates& ga
   const int m = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t0 = 0; t0 < 10; t0 += NW) {
-    const int t = t0 + w;
-    if (t >= 10) break;
+    const int t = min(t0 + w, 9);  // waves without one of their own repeat the last: no branch
     const int b = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, u = t - b * (b + 1) / 2, j = 16 * u + m;
     f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
 #pragma unroll
@@ -350,7 +391,8 @@ __device__ __forceinline__ float* tiles(float* p, int64_t chunk, int waves, int 
 // ---- forward -------------------------------------------------------------------------------
 template <class T, int DK, int NW, bool SOLVED>
 __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())) void forward_kernel(bsg_delta a) {
-  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW, VD = pitch<T>(DV);
+  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW;
+  constexpr bool AHEAD = SOLVED || sizeof(T) == 2;   // fp32 rows a chunk ahead would cost spilled registers
   __shared__ __align__(16) Chunk<T, DK, NW> s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
   // the workgroup's columns of all: all of them, but where the chunks are solved beforehand
@@ -368,7 +410,7 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
       S[d][r] = a.state ? a.state[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] : 0.0f;
 
   Fetch<T, C, DK, NT> fk, fq;
-  Fetch<T, C, DV, NT> fv;
+  Columns<T, NW> fv;
   FetchSolved<T, NT> fs;
   RawGates raw = {0, 0, 0};
   const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), v = steps_in<const T>(a.v, e, h, c0);
@@ -377,9 +419,11 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
   float *const ks = a.kept_states ? tiles(a.kept_states, eh * chunks, all / 16, DT, c0 / 16 + w, lane) : nullptr;
   float *const kw = a.kept_w ? tiles(a.kept_w, eh * chunks, all / 16, 4, c0 / 16 + w, lane) : nullptr;
   if (live > 0) {
-    fk.load(k.p, k.step, n, tid);
-    fq.load(q.p, q.step, n, tid);
-    fv.load(v.p, v.step, n, tid);
+    if (AHEAD) {
+      fk.load(k.p, k.step, n, tid);
+      fq.load(q.p, q.step, n, tid);
+      fv.load(v.p, v.step, n, tid, col);
+    }
     if (SOLVED) fs.load(a.work, eh * chunks, tid);
     else {
       if (w == 0) make_gates(s.s.gates[0], load_gates(gate, 0, n, lane), gate.half, lane);
@@ -389,15 +433,22 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
   for (int ch = 0; ch < live; ++ch) {
     const int t0 = ch * C, rows = min(C, n - t0), t1 = t0 + C;
     const Gates& gates = s.s.gates[SOLVED ? 0 : ch & 1];
+    if (!AHEAD) {
+      fk.load(k.at(t0), k.step, rows, tid);
+      fq.load(q.at(t0), q.step, rows, tid);
+      fv.load(v.at(t0), v.step, rows, tid, col);
+    }
     __syncthreads();               // the chunk before is done with LDS
     fk.store(s.k, rows, tid);
     fq.store(s.q, rows, tid);
     fv.store(s.v, rows, tid);
     if (SOLVED) fs.store(s.s, tid);
     if (t1 < n) {
-      fk.load(k.at(t1), k.step, n - t1, tid);
-      fq.load(q.at(t1), q.step, n - t1, tid);
-      fv.load(v.at(t1), v.step, n - t1, tid);
+      if (AHEAD) {
+        fk.load(k.at(t1), k.step, n - t1, tid);
+        fq.load(q.at(t1), q.step, n - t1, tid);
+        fv.load(v.at(t1), v.step, n - t1, tid, col);
+      }
       if (SOLVED) fs.load(a.work, eh * chunks + ch + 1, tid);
       else if (w == 0) raw = load_gates(gate, t1, n - t1, lane);
     }
@@ -416,17 +467,21 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
     for (int c = 0; c < DK / 32; ++c) {
       WideOf<T, 3> sw;
       split(sw, join(S[2 * c], S[2 * c + 1]));
+      Frag<T> kf[4], qf[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        mma<T>(x[b], load_tile(s.k + (16 * b + m) * LD, 32 * c, g), sw);
-        mma<T>(o[b], load_tile(s.q + (16 * b + m) * LD, 32 * c, g), front(sw));
+        kf[b] = load_tile(s.k + (16 * b + m) * LD, 32 * c, g);
+        qf[b] = load_tile(s.q + (16 * b + m) * LD, 32 * c, g);
       }
+      mma_all<T>(x, kf, sw);
+      mma_all<T>(o, qf, front(sw));
     }
+    f32x4 vs[4];
+    fv.get(vs, s.v, rows, w, lane);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const f32x4 in = *reinterpret_cast<const f32x4*>(&gates.in[16 * b + 4 * g]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[b][r] = (float)s.v[(16 * b + 4 * g + r) * VD + col] - in[r] * x[b][r];
+      x[b] = vs[b] - in * x[b];
       o[b] *= in * a.scale;
     }
     if (!SOLVED) {
@@ -455,7 +510,7 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
 #pragma unroll
       for (int b = 2 * c; b < 4; ++b) mma<T>(o[b], s.s.p_row(16 * b + m, 32 * c, g), uw);
     }
-    put_columns<T, VD>(s.v, o, w, lane);
+    fv.put(s.v, o, out.at(t0), out.step, rows, min(C, a.steps - t0), w, lane);
 #pragma unroll
     for (int d = 0; d < DT; ++d) S[d] *= gates.across;
 #pragma unroll
@@ -465,10 +520,12 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
       for (int i = 0; i < 2; ++i) u[i] = W[2 * c + i] * *reinterpret_cast<const f32x4*>(&gates.out[16 * (2 * c + i) + 4 * g]);
       WideOf<T, 3> uw;
       split(uw, join(u[0], u[1]));
+      Frag<T> kf[DT];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) mma<T>(S[d], load_col(s.k, LD, 32 * c, 16 * d, lane), uw);
+      for (int d = 0; d < DT; ++d) kf[d] = load_col(s.k, LD, 32 * c, 16 * d, lane);
+      mma_all<T>(S, kf, uw);
     }
-    write_columns<T, VD>(s.v, out.at(t0), out.step, rows, min(C, a.steps - t0), w, lane);
+    fv.write(s.v, out.at(t0), out.step, rows, min(C, a.steps - t0), w, lane);
   }
   for (int t = live * C + tid / DV; t < a.steps; t += NT / DV) out.at(t)[tid % DV] = (T)0.0f;   // padding
   if (a.final_state) {
@@ -484,7 +541,8 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
 // product's columns are value columns, so a wave works on its 16 alone, as in the forward pass.
 template <class T, int DK, int NW, bool SOLVED>
 __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())) void backward_state_kernel(bsg_delta a) {
-  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW, VD = pitch<T>(DV);
+  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW;
+  constexpr bool AHEAD = SOLVED || sizeof(T) == 2;   // fp32 rows a chunk ahead would cost spilled registers
   __shared__ __align__(16) Chunk<T, DK, NW> s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
   // the workgroup's columns of all: all of them, but where the chunks are solved beforehand
@@ -494,6 +552,7 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
   const int chunks = (a.steps + C - 1) / C, live = (n + C - 1) / C;
   const int64_t eh = (int64_t)e * a.heads_v + h;
 
+  constexpr int SIDE = SOLVED ? DT : 2;          // tiles of D side by side: registers allow no more
   f32x4 D[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -502,7 +561,7 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
       D[d][r] = a.dfinal ? a.dfinal[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] : 0.0f;
 
   Fetch<T, C, DK, NT> fk, fq;
-  Fetch<T, C, DV, NT> fv;
+  Columns<T, NW> fv;
   FetchSolved<T, NT> fs;
   RawGates raw = {0, 0, 0};
   const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), dout = steps_in<const T>(a.dout, e, h, c0);
@@ -511,9 +570,11 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
   float *const ws = tiles(a.work_states, eh * chunks, all / 16, DT, c0 / 16 + w, lane), *const wm = tiles(a.work_w, eh * chunks, all / 16, 4, c0 / 16 + w, lane);
   if (live > 0) {
     const int t0 = (live - 1) * C;
-    fk.load(k.at(t0), k.step, n - t0, tid);
-    fq.load(q.at(t0), q.step, n - t0, tid);
-    fv.load(dout.at(t0), dout.step, n - t0, tid);
+    if (AHEAD) {
+      fk.load(k.at(t0), k.step, n - t0, tid);
+      fq.load(q.at(t0), q.step, n - t0, tid);
+      fv.load(dout.at(t0), dout.step, n - t0, tid, col);
+    }
     if (SOLVED) fs.load(a.work, eh * chunks + live - 1, tid);
     else {
       if (w == 0) make_gates(s.s.gates[(live - 1) & 1], load_gates(gate, t0, n - t0, lane), gate.half, lane);
@@ -523,15 +584,22 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
   for (int ch = live - 1; ch >= 0; --ch) {
     const int t0 = ch * C, rows = min(C, n - t0), t1 = t0 - C;
     const Gates& gates = s.s.gates[SOLVED ? 0 : ch & 1];
+    if (!AHEAD) {
+      fk.load(k.at(t0), k.step, rows, tid);
+      fq.load(q.at(t0), q.step, rows, tid);
+      fv.load(dout.at(t0), dout.step, rows, tid, col);
+    }
     __syncthreads();               // the chunk after is done with LDS
     fk.store(s.k, rows, tid);
     fq.store(s.q, rows, tid);
     fv.store(s.v, rows, tid);
     if (SOLVED) fs.store(s.s, tid);
     if (t1 >= 0) {
-      fk.load(k.at(t1), k.step, C, tid);
-      fq.load(q.at(t1), q.step, C, tid);
-      fv.load(dout.at(t1), dout.step, C, tid);
+      if (AHEAD) {
+        fk.load(k.at(t1), k.step, C, tid);
+        fq.load(q.at(t1), q.step, C, tid);
+        fv.load(dout.at(t1), dout.step, C, tid, col);
+      }
       if (SOLVED) fs.load(a.work, eh * chunks + ch - 1, tid);
       else if (w == 0) raw = load_gates(gate, t1, C, lane);
     }
@@ -543,17 +611,16 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
 
     f32x4 x[4], go[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      x[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) go[b][r] = (float)s.v[(16 * b + 4 * g + r) * VD + col];
-    }
+    for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
+    fv.get(go, s.v, rows, w, lane);
 #pragma unroll
     for (int c = 0; c < DK / 32; ++c) {
       WideOf<T, 3> dw;
       split(dw, join(D[2 * c], D[2 * c + 1]));
+      Frag<T> kf[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) mma<T>(x[b], load_tile(s.k + (16 * b + m) * LD, 32 * c, g), dw);
+      for (int b = 0; b < 4; ++b) kf[b] = load_tile(s.k + (16 * b + m) * LD, 32 * c, g);
+      mma_all<T>(x, kf, dw);
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) x[b] *= *reinterpret_cast<const f32x4*>(&gates.out[16 * b + 4 * g]);
@@ -584,7 +651,7 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
       *reinterpret_cast<f32x4*>(wm + (int64_t)ch * C * all + 256 * b) = M[b];
       M[b] *= *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);
     }
-    put_columns<T, VD>(s.v, M, w, lane);
+    fv.put(s.v, M, dv.at(t0), dv.step, rows, min(C, a.steps - t0), w, lane);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const f32x4 in = *reinterpret_cast<const f32x4*>(&gates.in[16 * b + 4 * g]);
@@ -599,12 +666,22 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
       split(lw, join(M[2 * c], M[2 * c + 1]));
       split(ow, join(go[2 * c], go[2 * c + 1]));
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        mma<T>(D[d], load_col(s.k, LD, 32 * c, 16 * d, lane), lw);
-        mma<T>(D[d], load_col(s.q, LD, 32 * c, 16 * d, lane), ow);
+      for (int d0 = 0; d0 < DT; d0 += SIDE) {
+        f32x4 part[SIDE];
+        Frag<T> kf[SIDE], qf[SIDE];
+#pragma unroll
+        for (int d = 0; d < SIDE; ++d) {
+          part[d] = D[d0 + d];
+          kf[d] = load_col(s.k, LD, 32 * c, 16 * (d0 + d), lane);
+          qf[d] = load_col(s.q, LD, 32 * c, 16 * (d0 + d), lane);
+        }
+        mma_all<T>(part, kf, lw);
+        mma_all<T>(part, qf, ow);
+#pragma unroll
+        for (int d = 0; d < SIDE; ++d) D[d0 + d] = part[d];
       }
     }
-    write_columns<T, VD>(s.v, dv.at(t0), dv.step, rows, min(C, a.steps - t0), w, lane);
+    fv.write(s.v, dv.at(t0), dv.step, rows, min(C, a.steps - t0), w, lane);
   }
   for (int t = live * C + tid / DV; t < a.steps; t += NT / DV) dv.at(t)[tid % DV] = (T)0.0f;   // padding
   if (a.dstate) {

@@ -68,6 +68,14 @@ __device__ __forceinline__ void mma(f32x4& d, const Wide<T, N>& a, const Wide<T,
 #pragma unroll
     for (int i = 0; i <= s; ++i) mma(d, a.p[i], b.p[s - i]);
 }
+// the same for several D that share B, a part at a time: products of one D do not wait for each other
+template <class T, int M, int N>
+__device__ __forceinline__ void mma_all(f32x4 (&d)[M], const Frag<T> (&a)[M], const Wide<T, N>& b) {
+#pragma unroll
+  for (int i = N - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = 0; j < M; ++j) mma(d[j], a[j], b.p[i]);
+}
 // D[16][16] += A[16][16] B[16][16] in fp32: a[r] = A[m][4g + r], b[r] = B[4g + r][m], which is
 // how a D tile lies in registers
 __device__ __forceinline__ void mma16(f32x4& d, const f32x4& a, const f32x4& b) {
