@@ -829,9 +829,10 @@ __device__ __forceinline__ void chunk_gradient(Inside<T, DK>& s, int ch, int hk,
         const f32x8 wx = whole(wf), mx = whole(mf);
 #pragma unroll
         for (int j = 0; j < 8; ++j) dbeta = fmaf(wx[j], mx[j], dbeta);
-        // (tiles behind the own one too: cheaper than a branch, and masked below)
+        // (bf16: tiles behind the own one too: cheaper than a branch, and masked below)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
+          if (sizeof(T) == 4 && b > tile) continue;
           const WideOf<T, 2> x = s.w.get(16 * b + m, g);
           mma<T>(ow[b], x, go);
           mma<T>(mw[b], x, mf);
@@ -845,6 +846,7 @@ __device__ __forceinline__ void chunk_gradient(Inside<T, DK>& s, int ch, int hk,
       } else {
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
+          if (sizeof(T) == 4 && b < tile) continue;
           mma<T>(ow[b], load_run(s.go + (16 * b + m) * GL, 0, g), wf);
           mma<T>(mw[b], s.mu.get(16 * b + m, g), wf);
         }
