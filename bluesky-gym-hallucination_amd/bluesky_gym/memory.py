@@ -79,12 +79,14 @@ def _heads(who, q, k, v, rank, **dims):
 
 def _aligned(x):
     """Whether the kernels can read or write x's rows in 16-byte vectors."""
-    if x.data_ptr() % 16:
+    s, m = x.stride(), 16 // x.element_size() - 1
+    if s[-1] != 1 or x.data_ptr() & 15:
         return False
-    if x.is_contiguous():
-        return True
-    b = x.element_size()
-    return x.stride(-1) == 1 and all(n == 1 or s * b % 16 == 0 for n, s in zip(x.shape[:-1], x.stride()[:-1]))
+    either = 0
+    for y in s[:-1]:
+        either |= y
+    # the strides of axes of one are not looked at
+    return not either & m or all(n == 1 or not y & m for n, y in zip(x.shape[:-1], s[:-1]))
 
 
 def _vectors(x):
@@ -92,23 +94,22 @@ def _vectors(x):
 
 
 def _empty_like(x):
-    """A dense tensor in x's order of axes, with rows the kernels can write."""
+    """A dense tensor in the order of axes of x, whose rows the kernels can read, with rows they
+    can write."""
     y = torch.empty_like(x)
-    return y if _aligned(y) else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return y if y.stride() == x.stride() or _aligned(y) else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _rows(x):
-    """A bsg_rows: a rollout's [E, T, H, D], a gate's [E, T, H].  The strides of axes of one are
-    not looked at."""
-    E, T, H = x.shape[:3]
-    s = x.stride()
-    return x.data_ptr(), s[0] if E > 1 else 0, s[1] if T > 1 else 0, s[2] if H > 1 else 0
+    """A bsg_rows: a rollout's [E, T, H, D], a gate's [E, T, H]."""
+    s, n = x.stride(), x.shape
+    return (x.data_ptr(), s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
 
 
 def _step_rows(x):
     """A bsg_rows of one step: [E, H, D] or a gate's [E, H]."""
-    s = x.stride()
-    return x.data_ptr(), s[0] if x.shape[0] > 1 else 0, 0, s[1] if x.shape[1] > 1 else 0
+    s, n = x.stride(), x.shape
+    return (x.data_ptr(), s[0] if n[0] > 1 else 0, 0, s[1] if n[1] > 1 else 0)
 
 
 _NO_ROWS = (0, 0, 0, 0)
@@ -146,22 +147,26 @@ def _no_grad(who, *xs):
 
 def _out(who, out, like):
     if out is None:
-        return _empty_like(like)
+        return _empty_like(_vectors(like))
     _shape(who, "out", out, like.shape, (like.dtype,))
     if not _aligned(out):
         raise ValueError(f"{who}: out must have contiguous, 16-byte aligned rows")
     return out
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(i).cuda_stream without the object
+
+
 def _call(fn, block, dev):
     """The launch goes to the tensors' device, on its current stream."""
-    call = getattr(nat.load_library(), fn)
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        nat.check(call(block, stream), fn)
+    call, i = getattr(nat.load_library(), fn), dev.index
+    if torch.cuda.current_device() == i:
+        rc = call(block, _raw_stream(i))
     else:
-        with torch.cuda.device(dev):
-            nat.check(call(block, stream), fn)
+        with torch.cuda.device(i):
+            rc = call(block, _raw_stream(i))
+    if rc:
+        nat.check(rc, fn)
 
 
 # ---- the gated delta rule -------------------------------------------------------------------
