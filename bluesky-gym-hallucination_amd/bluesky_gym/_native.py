@@ -285,6 +285,7 @@ def load_library(path: str | None = None):
     for fn in ("bsg_attention_parts_bytes", "bsg_attention_step_bytes", "bsg_delta_work_bytes"):
         getattr(lib, fn).restype = C.c_int64
         getattr(lib, fn).argtypes = [C.c_void_p]
+    lib.bsg_delta_work_bytes.argtypes = [C.c_void_p, C.c_int32]
     if lib.bsg_abi_version() != ABI_VERSION:
         raise BsgError(f"libbsg ABI {lib.bsg_abi_version()} != expected {ABI_VERSION}")
     if path is None:

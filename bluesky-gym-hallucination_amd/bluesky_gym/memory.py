@@ -199,7 +199,7 @@ def _delta_check(who, q, k, v, g, beta, state, first, lead):
 def _with_work(fn, before, after, dev):
     """The call with the fields around bsg_delta.work, and the scratch that it wants there."""
     block = _pack_delta(*before, 0, *after)
-    need = nat.load_library().bsg_delta_work_bytes(block)
+    need = nat.load_library().bsg_delta_work_bytes(block, fn == "bsg_delta_backward")
     if need > 0:
         work = torch.empty(need, dtype=torch.uint8, device=dev)
         block = _pack_delta(*before, work.data_ptr(), *after)

@@ -843,8 +843,8 @@ template <class A> bool delta_inputs(const A* a) {
   return vector_rows(a->q, a->dtype) && vector_rows(a->k, a->dtype) && vector_rows(a->v, a->dtype) && a->g.p && a->beta.p;
 }
 
-bool delta_work(const bsg_delta* a) {
-  return bsg::delta_work_bytes(*a) == 0 || (a->work && !(reinterpret_cast<uintptr_t>(a->work) & 15));
+bool delta_work(const bsg_delta* a, bool backward) {
+  return bsg::delta_work_bytes(*a, backward) == 0 || (a->work && !(reinterpret_cast<uintptr_t>(a->work) & 15));
 }
 
 int32_t check_heads(const char* who, int num_envs, int heads_q, int heads_k, int dim, int dtype, float softcap, int64_t per_head) {
@@ -881,10 +881,10 @@ bsg_attention with_begins(const bsg_attention* a) {
 
 extern "C" {
 
-int64_t bsg_delta_work_bytes(const bsg_delta* a) {
+int64_t bsg_delta_work_bytes(const bsg_delta* a, int32_t backward) {
   if (!a) return fail(BSG_E_INVALID_ARG, "bsg_delta_work_bytes: null arguments");
   if (int32_t r = check_delta(a, a->steps, "bsg_delta_work_bytes")) return r;
-  return bsg::delta_work_bytes(*a);
+  return bsg::delta_work_bytes(*a, backward != 0);
 }
 
 int32_t bsg_delta_forward(const bsg_delta* a, void* stream) {
@@ -895,7 +895,7 @@ int32_t bsg_delta_forward(const bsg_delta* a, void* stream) {
     return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: q, k, v, g, beta and out must be there, with 16-byte aligned rows of q, k, v and out");
   if (!a->kept_states != !a->kept_w || ((reinterpret_cast<uintptr_t>(a->kept_states) | reinterpret_cast<uintptr_t>(a->kept_w)) & 15))
     return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: kept_states and kept_w go together, 16-byte aligned");
-  if (!delta_work(a)) return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: work must be there, 16-byte aligned, where bsg_delta_work_bytes is not 0");
+  if (!delta_work(a, false)) return fail(BSG_E_INVALID_ARG, "bsg_delta_forward: work must be there, 16-byte aligned, where bsg_delta_work_bytes is not 0");
   hipError_t e = bsg::launch_delta_forward(*a, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_delta_forward launch");
 }
@@ -911,7 +911,7 @@ int32_t bsg_delta_backward(const bsg_delta* a, void* stream) {
   for (const void* p : scratch)
     if (!p || (reinterpret_cast<uintptr_t>(p) & 15))
       return fail(BSG_E_INVALID_ARG, "bsg_delta_backward: kept_* and work_* must be there, 16-byte aligned");
-  if (!delta_work(a)) return fail(BSG_E_INVALID_ARG, "bsg_delta_backward: work must be there, 16-byte aligned, where bsg_delta_work_bytes is not 0");
+  if (!delta_work(a, true)) return fail(BSG_E_INVALID_ARG, "bsg_delta_backward: work must be there, 16-byte aligned, where bsg_delta_work_bytes is not 0");
   hipError_t e = bsg::launch_delta_backward(*a, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? BSG_OK : hip_fail(e, "bsg_delta_backward launch");
 }

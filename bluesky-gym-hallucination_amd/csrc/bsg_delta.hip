@@ -260,18 +260,19 @@ struct Columns<float, NW> {
 template <int J> __device__ __forceinline__ float from_lane(float x) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + J, 0xf, 0xf, false));
 }
-// x[c] of lane i, c <= J: minus n_iJ times row J of the inverse, which is done
-template <int J> __device__ __forceinline__ void eliminate(float (&x)[16], const float (&n)[16]) {
+// some columns x[c] of lane i's row: less n_iJ times row J of the inverse, which is done (and 0 before
+// the column's own row)
+template <int J, int N> __device__ __forceinline__ void eliminate(float (&x)[N], const float (&n)[16]) {
   if constexpr (J < 15) {
 #pragma unroll
-    for (int c = 0; c <= J; ++c) x[c] = fmaf(from_lane<J>(x[c]), n[J], x[c]);
+    for (int c = 0; c < N; ++c) x[c] = fmaf(from_lane<J>(x[c]), n[J], x[c]);
     eliminate<J + 1>(x, n);
   }
 }
 
-// The ten lower tiles of N and P (one decay serves both), then, after a barrier, the inverses by
-// wave NW - 1, which has the fewest tiles; the others go on to what does not need them.  An
-// inverse's row lies in a lane, and its substitution takes the rows before from their lanes.
+// The ten lower tiles of N and P (one decay serves both), then, after a barrier, the inverses: 16 / NW
+// columns of each to a wave, a row to a lane; the substitution takes the rows before from their lanes
+// (by one wave alone it held the others up: 102 against 89 us, 512x50 fp32).  The inverses are there after the caller's next barrier.
 // BACK: the system is (I + diag(beta) N)^T, else I + N diag(beta).
 template <class T, int DK, int NW, bool BACK>
 __device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& x, const Gates& gates, float scale, int lane, int w) {
@@ -306,21 +307,20 @@ __device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& x, const Gates& ga
     }
   }
   __syncthreads();
-  if (w == NW - 1) {               // lane: block g, row m
-    float v[16], n[16];
+  constexpr int N = 16 / NW;
+  const int c0 = N * w;
+  float v[N], n[16];               // lane: block g, row m
 #pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(&s.n[(16 * g + m) * AP + 16 * g + j]);
+  for (int j = 0; j < 16; j += 4) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(&s.n[(16 * g + m) * AP + 16 * g + j]);
 #pragma unroll
-      for (int o = 0; o < 4; ++o) n[j + o] = y[o];
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = j == m ? 1.0f : 0.0f;
-    eliminate<0>(v, n);
-#pragma unroll
-    for (int j = 0; j < 16; j += 4)
-      *reinterpret_cast<f32x4*>(&s.inv[(16 * g + m) * IP + j]) = f32x4{v[j], v[j + 1], v[j + 2], v[j + 3]};
+    for (int o = 0; o < 4; ++o) n[j + o] = y[o];
   }
+#pragma unroll
+  for (int c = 0; c < N; ++c) v[c] = c0 + c == m ? 1.0f : 0.0f;
+  eliminate<0>(v, n);
+#pragma unroll
+  for (int c = 0; c < N; ++c) s.inv[(16 * g + m) * IP + c0 + c] = v[c];
 }
 // P's tiles above the diagonal that share a product step with one on it
 template <class T>
@@ -696,8 +696,10 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
 // q', k', beta', g' of one chunk, env and key head, all chunks side by side: a wave owns 16 steps.
 // The matrices o'.w and m.w are needed by rows (for q', kr') and by columns (for kw'); both are
 // computed, each in the layout in which it is the B operand of what follows, which costs less than
-// a turn through LDS, by different waves.  The value dimension is walked in slices of 32, the value heads that share
-// the key head one after the other, their q' and k' added up in registers.
+// a turn through LDS, by different waves.  The value dimension is walked in slices of 32.  Value heads
+// that share a key head take a launch each: all but the last leave their sums of q' and k' in fp32 to
+// the next (in one launch their sums cost the registers that let two workgroups share a CU: 420 us
+// against 2 x 164 us, two heads to a key head, 512 envs x 300 steps).
 constexpr int SL = 32;
 template <class T, int R>
 struct WideRows {                  // an R x SL tile of fp32 values as operand parts of type T
@@ -746,21 +748,20 @@ struct Inside {
 
 // Eight waves: 0..3 hold the 16 steps of tile w as they read the state (q', kr'), 4..7 those of tile
 // w - 4 as they write it (kw').  The two run code of their own between the same barriers, so that
-// neither pays for the other's registers: two workgroups to a CU where LDS holds two and no sums over
-// shared heads take their registers (four waves a SIMD cover each other's loads), else one, which
-// loads a slice ahead.
-template <class T, int DK, bool SHARED> constexpr bool two_groups() { return !SHARED && 2 * sizeof(Inside<T, DK>) <= 160 * 1024; }
+// neither pays for the other's registers: two workgroups to a CU where LDS holds two (four waves a
+// SIMD cover each other's loads), else one, which loads a slice ahead.
+template <class T, int DK> constexpr bool two_groups() { return 2 * sizeof(Inside<T, DK>) <= 160 * 1024; }
 
-template <class T, int DK, bool SHARED, bool READER>
-__device__ __forceinline__ void chunk_gradient(Inside<T, DK>& s, int ch, int hk, int e) {
+template <class T, int DK, bool READER>
+__device__ __forceinline__ void chunk_gradient(Inside<T, DK>& s, float* sums, int head, int ch, int hk, int e) {
   constexpr int LD = pitch<T>(DK), DT = DK / 16, GL = pitch<T>(SL), NT = 512;
   constexpr int NS = DK * SL / 4 / NT > 0 ? DK * SL / 4 / NT : 1;   // f32x4 of a state's slice to a thread
-  constexpr bool AHEAD = !two_groups<T, DK, SHARED>();
+  constexpr bool AHEAD = !two_groups<T, DK>();
   static_assert(C * SL / 4 == NT, "one f32x4 of W and of M to a thread");
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), own = 16 * (w & 3) + m, tile = w & 3;
   const bsg_delta& a = arguments();
-  const int chunks = (a.steps + C - 1) / C, group = a.heads_v / a.heads_k, DV = a.dim_v;
+  const int chunks = (a.steps + C - 1) / C, group = a.heads_v / a.heads_k, DV = a.dim_v, h = hk * group + head;
   const int t0 = ch * C, rows = min(C, steps_of(a, e) - t0);
   const float scale = a.scale;
   const bool half = a.gate_dtype == BSG_BF16;
@@ -770,7 +771,7 @@ __device__ __forceinline__ void chunk_gradient(Inside<T, DK>& s, int ch, int hk,
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   u32x4 fgo = {0, 0, 0, 0};
   f32x4 fw, fm, fs[NS], fd[NS];
-  const auto fetch = [&](int h, int v0) {
+  const auto fetch = [&](int v0) {
     const bsg_delta& a = arguments();
     const int64_t ehc = ((int64_t)e * a.heads_v + h) * chunks + ch;
     const int64_t at = ehc * C * DV + v0 * C + tid * 4, as = ehc * DK * DV + v0 * DK + tid * 4;
@@ -785,207 +786,216 @@ __device__ __forceinline__ void chunk_gradient(Inside<T, DK>& s, int ch, int hk,
         fd[i] = *reinterpret_cast<const f32x4*>(a.work_states + as + i * 4 * NT);
       }
   };
-  if (AHEAD) fetch(hk * group, 0);
+  if (AHEAD) fetch(0);
 
-  f32x4 sum1[DT], sum2[DT];        // over the value heads: q', kr' (readers); kw' (writers)
+  // readers: o'.w and m.w by rows j, q' and kr'; writers: by rows i, kw'
+  f32x4 ow[4], mw[4], X1[DT], X2[DT];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) sum1[d] = sum2[d] = f32x4{0, 0, 0, 0};
-  for (int h = hk * group, last = SHARED ? h + group - 1 : h; h <= last; ++h) {
-    // readers: o'.w and m.w by rows j, q' and kr'; writers: by rows i, kw'
-    f32x4 ow[4], mw[4], X1[DT], X2[DT];
+  for (int b = 0; b < 4; ++b) ow[b] = mw[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int b = 0; b < 4; ++b) ow[b] = mw[b] = f32x4{0, 0, 0, 0};
+  for (int d = 0; d < DT; ++d) X1[d] = X2[d] = f32x4{0, 0, 0, 0};
+  float dbeta = 0.0f, sd = 0.0f;
+  RawGates raw = {0, 0, 0};
+  if (READER && w == 0) raw = load_gates(GateSteps(arguments(), e, h), t0, rows, lane);
+  for (int v0 = 0; v0 < DV; v0 += SL) {
+    if (!AHEAD) fetch(v0);
+    __syncthreads();             // the slice before is done with
+    if (READER && v0 == 0 && w == 0) make_gates(s.gates, raw, half, lane);
+    if (tid < C * GROW)
+      *reinterpret_cast<u32x4*>(&s.go[tid / GROW * GL + tid % GROW * GV]) = tid / GROW < rows ? fgo : u32x4{0, 0, 0, 0};
+    s.w.put(tid / 64 % 4, tid / 256, lane, fw);
+    s.mu.put(tid / 64 % 4, tid / 256, lane, fm);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) X1[d] = X2[d] = f32x4{0, 0, 0, 0};
-    float dbeta = 0.0f, sd = 0.0f;
-    RawGates raw = {0, 0, 0};
-    if (READER && w == 0) raw = load_gates(GateSteps(arguments(), e, h), t0, rows, lane);
-    for (int v0 = 0; v0 < DV; v0 += SL) {
-      if (!AHEAD) fetch(h, v0);
-      __syncthreads();             // the slice before is done with
-      if (READER && v0 == 0 && w == 0) make_gates(s.gates, raw, half, lane);
-      if (tid < C * GROW)
-        *reinterpret_cast<u32x4*>(&s.go[tid / GROW * GL + tid % GROW * GV]) = tid / GROW < rows ? fgo : u32x4{0, 0, 0, 0};
-      s.w.put(tid / 64 % 4, tid / 256, lane, fw);
-      s.mu.put(tid / 64 % 4, tid / 256, lane, fm);
+    for (int i = 0; i < NS; ++i)
+      if (DK * SL / 4 >= NT || tid < DK * SL / 4) {
+        const int at = (tid + i * NT) / 64;
+        s.st.put(at % DT, at / DT, lane, fs[i]);
+        s.ds.put(at % DT, at / DT, lane, fd[i]);
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
-        if (DK * SL / 4 >= NT || tid < DK * SL / 4) {
-          const int at = (tid + i * NT) / 64;
-          s.st.put(at % DT, at / DT, lane, fs[i]);
-          s.ds.put(at % DT, at / DT, lane, fd[i]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sd = fmaf(fs[i][j], fd[i][j], sd);
-        }
-      if (AHEAD) {
-        if (v0 + SL < DV) fetch(h, v0 + SL);
-        else if (SHARED && h < last) fetch(h + 1, 0);
+        for (int j = 0; j < 4; ++j) sd = fmaf(fs[i][j], fd[i][j], sd);
       }
-      __syncthreads();
-      const WideOf<T, 2> wf = s.w.get(own, g);
-      if (READER) {
-        const Frag<T> go = load_run(s.go + own * GL, 0, g);
-        const WideOf<T, 2> mf = s.mu.get(own, g);
-        const f32x8 wx = whole(wf), mx = whole(mf);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dbeta = fmaf(wx[j], mx[j], dbeta);
-        // (bf16: tiles behind the own one too: cheaper than a branch, and masked below)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (sizeof(T) == 4 && b > tile) continue;
-          const WideOf<T, 2> x = s.w.get(16 * b + m, g);
-          mma<T>(ow[b], x, go);
-          mma<T>(mw[b], x, mf);
-        }
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const WideOf<T, 2> x = s.st.get(16 * d + m, g);
-          mma<T>(X1[d], x, go);
-          mma<T>(X2[d], x, mf);
-        }
-      } else {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (sizeof(T) == 4 && b < tile) continue;
-          mma<T>(ow[b], load_run(s.go + (16 * b + m) * GL, 0, g), wf);
-          mma<T>(mw[b], s.mu.get(16 * b + m, g), wf);
-        }
-#pragma unroll
-        for (int d = 0; d < DT; ++d) mma<T>(X1[d], s.ds.get(16 * d + m, g), wf);
-      }
+    if (AHEAD) {
+      if (v0 + SL < DV) fetch(v0 + SL);
     }
-    // scale by the gates of the wave's own step (its lane) and add the chunk's own terms
-    const Gates& G = s.gates;
-    const Step me = step_of(G, own);
-    const float bi = G.beta[own], in = G.in[own], out = G.out[own], across = G.across;
-    float y = 0.0f, dc = 0.0f;
+    __syncthreads();
+    const WideOf<T, 2> wf = s.w.get(own, g);
     if (READER) {
+      const Frag<T> go = load_run(s.go + own * GL, 0, g);
+      const WideOf<T, 2> mf = s.mu.get(own, g);
+      const f32x8 wx = whole(wf), mx = whole(mf);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dbeta = fmaf(wx[j], mx[j], dbeta);
+      // (bf16: tiles behind the own one too: cheaper than a branch, and masked below)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (sizeof(T) == 4 && b > tile) continue;
+        const WideOf<T, 2> x = s.w.get(16 * b + m, g);
+        mma<T>(ow[b], x, go);
+        mma<T>(mw[b], x, mf);
+      }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        X1[d] *= in;
-        X2[d] *= in;
+        const WideOf<T, 2> x = s.st.get(16 * d + m, g);
+        mma<T>(X1[d], x, go);
+        mma<T>(X2[d], x, mf);
       }
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (2 * c <= tile) {       // rows j of tiles 2c, 2c + 1 against the own step i
-          f32x4 f1[2], f2[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int row = 16 * (2 * c + u) + 4 * g;
-            const f32x4 f = decays<true>(G, row, me) * *reinterpret_cast<const f32x4*>(&G.beta[row]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              f1[u][r] = row + r <= own ? f[r] * ow[2 * c + u][r] : 0.0f;
-              f2[u][r] = row + r < own ? f[r] * mw[2 * c + u][r] : 0.0f;
-            }
-          }
-          WideOf<T, 2> w1, w2;
-          split(w1, join(f1[0], f1[1]));
-          split(w2, join(f2[0], f2[1]));
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const Frag<T> k = load_col(s.k, LD, 32 * c, 16 * d, lane);
-            mma<T>(X1[d], k, w1);
-            mma<T>(X2[d], k, w2);
-          }
-        }
     } else {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const f32x4 k = widen(*reinterpret_cast<const Half<T>*>(&s.k[own * LD + 16 * d + 4 * g]));
-        X1[d] *= out;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y = fmaf(k[r], X1[d][r], y);
+      for (int b = 0; b < 4; ++b) {
+        if (sizeof(T) == 4 && b < tile) continue;
+        mma<T>(ow[b], load_run(s.go + (16 * b + m) * GL, 0, g), wf);
+        mma<T>(mw[b], s.mu.get(16 * b + m, g), wf);
       }
-      y *= bi;
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (2 * c + 1 >= tile) {   // rows i of tiles 2c, 2c + 1 against the own step j
-          f32x4 f1[2], f2[2];
+      for (int d = 0; d < DT; ++d) mma<T>(X1[d], s.ds.get(16 * d + m, g), wf);
+    }
+  }
+  // scale by the gates of the wave's own step (its lane) and add the chunk's own terms
+  const Gates& G = s.gates;
+  const Step me = step_of(G, own);
+  const float bi = G.beta[own], in = G.in[own], out = G.out[own], across = G.across;
+  float y = 0.0f, dc = 0.0f;
+  if (READER) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int row = 16 * (2 * c + u) + 4 * g;
-            const f32x4 f = decays<false>(G, row, me), bm = f * *reinterpret_cast<const f32x4*>(&G.beta[row]);
+    for (int d = 0; d < DT; ++d) {
+      X1[d] *= in;
+      X2[d] *= in;
+    }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              f1[u][r] = row + r >= own ? scale * f[r] * ow[2 * c + u][r] : 0.0f;
-              f2[u][r] = row + r > own ? -bm[r] * mw[2 * c + u][r] : 0.0f;
-            }
-          }
-          WideOf<T, 2> w1, w2;
-          split(w1, join(f1[0], f1[1]));
-          split(w2, join(f2[0], f2[1]));
+    for (int c = 0; c < 2; ++c)
+      if (2 * c <= tile) {       // rows j of tiles 2c, 2c + 1 against the own step i
+        f32x4 f1[2], f2[2];
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            mma<T>(X1[d], load_col(s.q, LD, 32 * c, 16 * d, lane), w1);
-            mma<T>(X1[d], load_col(s.k, LD, 32 * c, 16 * d, lane), w2);
+        for (int u = 0; u < 2; ++u) {
+          const int row = 16 * (2 * c + u) + 4 * g;
+          const f32x4 f = decays<true>(G, row, me) * *reinterpret_cast<const f32x4*>(&G.beta[row]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            f1[u][r] = row + r <= own ? f[r] * ow[2 * c + u][r] : 0.0f;
+            f2[u][r] = row + r < own ? f[r] * mw[2 * c + u][r] : 0.0f;
           }
         }
-    }
+        WideOf<T, 2> w1, w2;
+        split(w1, join(f1[0], f1[1]));
+        split(w2, join(f2[0], f2[1]));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const Frag<T> k = load_col(s.k, LD, 32 * c, 16 * d, lane);
+          mma<T>(X1[d], k, w1);
+          mma<T>(X2[d], k, w2);
+        }
+      }
+  } else {
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const f32x4 k = widen(*reinterpret_cast<const Half<T>*>(&s.k[own * LD + 16 * d + 4 * g]));
-      X1[d] *= READER ? scale : bi;
-      if (READER) {
-        const f32x4 q = widen(*reinterpret_cast<const Half<T>*>(&s.q[own * LD + 16 * d + 4 * g]));
-        X2[d] *= -bi;
+      X1[d] *= out;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) dc = fmaf(q[r], X1[d][r], fmaf(k[r], X2[d][r], dc));
-        sum2[d] = SHARED ? sum2[d] + X2[d] : X2[d];
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) dc = fmaf(-k[r], X1[d][r], dc);
-      }
-      sum1[d] = SHARED ? sum1[d] + X1[d] : X1[d];
+      for (int r = 0; r < 4; ++r) y = fmaf(k[r], X1[d][r], y);
     }
-    dc = sum_groups(dc);
-    // the chunk's last step: across <S, D> + sum_j k_j.(out_j D u_j)
-    y += across * sd;
+    y *= bi;
 #pragma unroll
-    for (int d = 32; d >= 1; d /= 2) y += __shfl_xor(y, d);
-    if (g == 0) s.dc[READER ? 0 : 1][own] = dc;
-    if (lane == 0) s.part[w] = y;
-    const bsg_delta& a = arguments();
+    for (int c = 0; c < 2; ++c)
+      if (2 * c + 1 >= tile) {   // rows i of tiles 2c, 2c + 1 against the own step j
+        f32x4 f1[2], f2[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = 16 * (2 * c + u) + 4 * g;
+          const f32x4 f = decays<false>(G, row, me), bm = f * *reinterpret_cast<const f32x4*>(&G.beta[row]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            f1[u][r] = row + r >= own ? scale * f[r] * ow[2 * c + u][r] : 0.0f;
+            f2[u][r] = row + r > own ? -bm[r] * mw[2 * c + u][r] : 0.0f;
+          }
+        }
+        WideOf<T, 2> w1, w2;
+        split(w1, join(f1[0], f1[1]));
+        split(w2, join(f2[0], f2[1]));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          mma<T>(X1[d], load_col(s.q, LD, 32 * c, 16 * d, lane), w1);
+          mma<T>(X1[d], load_col(s.k, LD, 32 * c, 16 * d, lane), w2);
+        }
+      }
+  }
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    const f32x4 k = widen(*reinterpret_cast<const Half<T>*>(&s.k[own * LD + 16 * d + 4 * g]));
+    X1[d] *= READER ? scale : bi;
     if (READER) {
-      dbeta = sum_groups(dbeta);
-      if (g == 0 && t0 + own < a.steps) gate_out(a.dbeta, a.gate_dtype, e, t0 + own, h, own < rows ? dbeta : 0.0f);
-    }
-    __syncthreads();
-    if (READER && w == 0) {
-      float x = s.dc[0][lane] + s.dc[1][lane];
-      if (lane == 63)
+      const f32x4 q = widen(*reinterpret_cast<const Half<T>*>(&s.q[own * LD + 16 * d + 4 * g]));
+      X2[d] *= -bi;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x += s.part[i];
-      const int ep = G.episode[lane], before = lane ? G.episode[lane - 1] : 0;
+      for (int r = 0; r < 4; ++r) dc = fmaf(q[r], X1[d][r], fmaf(k[r], X2[d][r], dc));
+    } else {
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const float o = __shfl_down(x, d);
-        const int oe = __shfl_down(ep, d);
-        if (lane + d < 64 && oe == ep) x += o;
-      }
-      // a first step's decay meets no state
-      if (t0 + lane < a.steps)
-        gate_out(a.dg, a.gate_dtype, e, t0 + lane, h, lane < rows && ep == before ? x : 0.0f);
+      for (int r = 0; r < 4; ++r) dc = fmaf(-k[r], X1[d][r], dc);
     }
+  }
+  dc = sum_groups(dc);
+  // the chunk's last step: across <S, D> + sum_j k_j.(out_j D u_j)
+  y += across * sd;
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) y += __shfl_xor(y, d);
+  if (g == 0) s.dc[READER ? 0 : 1][own] = dc;
+  if (lane == 0) s.part[w] = y;
+  const bsg_delta& z = arguments();
+  if (READER) {
+    dbeta = sum_groups(dbeta);
+    if (g == 0 && t0 + own < z.steps) gate_out(z.dbeta, z.gate_dtype, e, t0 + own, h, own < rows ? dbeta : 0.0f);
+  }
+  __syncthreads();
+  if (READER && w == 0) {
+    float x = s.dc[0][lane] + s.dc[1][lane];
+    if (lane == 63)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x += s.part[i];
+    const int ep = G.episode[lane], before = lane ? G.episode[lane - 1] : 0;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const float o = __shfl_down(x, d);
+      const int oe = __shfl_down(ep, d);
+      if (lane + d < 64 && oe == ep) x += o;
+    }
+    // a first step's decay meets no state
+    if (t0 + lane < z.steps)
+      gate_out(z.dg, z.gate_dtype, e, t0 + lane, h, lane < rows && ep == before ? x : 0.0f);
   }
   if (!READER) {                   // the last slice is done with: every wave has passed the barrier above
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&s.kw[own * (DK + 4) + 16 * d + 4 * g]) = sum1[d];
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&s.kw[own * (DK + 4) + 16 * d + 4 * g]) = X1[d];
   }
   __syncthreads();
-  const bsg_delta& z = arguments();
-  if (!READER || t0 + own >= z.steps) return;
+  if (!READER) return;
+  // 16 bytes a lane of the sums over the heads before, as the D tiles lie
+  float* sum = sums ? sums + ((((int64_t)e * z.heads_k + hk) * chunks + ch) * 4 + tile) * 2 * DT * 256 + lane * 4 : nullptr;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    X2[d] += *reinterpret_cast<const f32x4*>(&s.kw[own * (DK + 4) + 16 * d + 4 * g]);
+    if (sum && head > 0) {
+      X1[d] += *reinterpret_cast<const f32x4*>(sum + 512 * d);
+      X2[d] += *reinterpret_cast<const f32x4*>(sum + 512 * d + 256);
+    }
+  }
+  if (head + 1 < group) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      *reinterpret_cast<f32x4*>(sum + 512 * d) = X1[d];
+      *reinterpret_cast<f32x4*>(sum + 512 * d + 256) = X2[d];
+    }
+    return;
+  }
+  if (t0 + own >= z.steps) return;
   T *oq = row_out<T>(z.dq, e, t0 + own, hk), *ok = row_out<T>(z.dk, e, t0 + own, hk);
 #pragma unroll
   for (int d = 0; d < DT; ++d) {
-    const f32x4 kw = *reinterpret_cast<const f32x4*>(&s.kw[own * (DK + 4) + 16 * d + 4 * g]);
-    store4(oq + 16 * d + 4 * g, own < rows ? sum1[d] : f32x4{0, 0, 0, 0});
-    store4(ok + 16 * d + 4 * g, own < rows ? sum2[d] + kw : f32x4{0, 0, 0, 0});
+    store4(oq + 16 * d + 4 * g, own < rows ? X1[d] : f32x4{0, 0, 0, 0});
+    store4(ok + 16 * d + 4 * g, own < rows ? X2[d] : f32x4{0, 0, 0, 0});
   }
 }
 
-template <class T, int DK, bool SHARED>
-__global__ __launch_bounds__(512, (two_groups<T, DK, SHARED>() ? 4 : 2)) void backward_chunk_kernel(bsg_delta) {
+template <class T, int DK>
+__global__ __launch_bounds__(512, (two_groups<T, DK>() ? 4 : 2)) void backward_chunk_kernel(bsg_delta, float* sums, int head) {
   constexpr int NT = 512;
   __shared__ __align__(16) Inside<T, DK> s;
   const bsg_delta& a = arguments();
@@ -993,6 +1003,7 @@ __global__ __launch_bounds__(512, (two_groups<T, DK, SHARED>() ? 4 : 2)) void ba
   const int ch = blockIdx.x % chunks, ehk = blockIdx.x / chunks, hk = ehk % a.heads_k, e = ehk / a.heads_k;
   const int t0 = ch * C, rows = min(C, steps_of(a, e) - t0), all = min(C, a.steps - t0);
   if (rows <= 0) {                 // padding
+    if (head > 0) return;
     const Steps<T> dqs = steps_in<T>(a.dq, e, hk), dks = steps_in<T>(a.dk, e, hk);
     for (int i = tid; i < all * DK; i += NT) dqs.at(t0 + i / DK)[i % DK] = dks.at(t0 + i / DK)[i % DK] = (T)0.0f;
     for (int i = tid; i < all * group; i += NT) {
@@ -1008,8 +1019,8 @@ __global__ __launch_bounds__(512, (two_groups<T, DK, SHARED>() ? 4 : 2)) void ba
     fk.store(s.k, rows, tid);
     fq.store(s.q, rows, tid);
   }
-  if (__builtin_amdgcn_readfirstlane(tid >> 6) < 4) chunk_gradient<T, DK, SHARED, true>(s, ch, hk, e);
-  else chunk_gradient<T, DK, SHARED, false>(s, ch, hk, e);
+  if (__builtin_amdgcn_readfirstlane(tid >> 6) < 4) chunk_gradient<T, DK, true>(s, sums, head, ch, hk, e);
+  else chunk_gradient<T, DK, false>(s, sums, head, ch, hk, e);
 }
 
 // ---- acting --------------------------------------------------------------------------------
@@ -1081,6 +1092,11 @@ hipError_t run(const bsg_delta_act& a, bool, hipStream_t st) {
 bool solved_first(const bsg_delta& a) {
   return a.dim_v > 32 && a.steps > C && (int64_t)a.num_envs * a.heads_v < 256;
 }
+int64_t solved_work(const bsg_delta& a) {
+  if (!solved_first(a)) return 0;
+  const int64_t chunks = (int64_t)a.num_envs * a.heads_v * ((a.steps + C - 1) / C);
+  return chunks * (a.dtype == BSG_BF16 ? solved_bytes<bf16>() : solved_bytes<float>());
+}
 template <class T, int DK, int NW>
 hipError_t run(const bsg_delta& a, bool back, hipStream_t st) {
   const dim3 rows((unsigned)(a.num_envs * a.heads_v));
@@ -1102,8 +1118,9 @@ hipError_t run(const bsg_delta& a, bool back, hipStream_t st) {
   }
   if (back) {
     const dim3 chunks((unsigned)(a.num_envs * a.heads_k * ((a.steps + C - 1) / C)));
-    if (a.heads_v > a.heads_k) backward_chunk_kernel<T, DK, true><<<chunks, dim3(512), 0, st>>>(a);
-    else backward_chunk_kernel<T, DK, false><<<chunks, dim3(512), 0, st>>>(a);
+    const int group = a.heads_v / a.heads_k;
+    float* sums = group > 1 ? reinterpret_cast<float*>(static_cast<char*>(a.work) + solved_work(a)) : nullptr;
+    for (int head = 0; head < group; ++head) backward_chunk_kernel<T, DK><<<chunks, dim3(512), 0, st>>>(a, sums, head);
   }
   return hipGetLastError();
 }
@@ -1126,10 +1143,9 @@ namespace bsg {
 // Shapes, strides and pointers are validated by the bsg_delta_* entry points (bsg_abi.cpp).
 hipError_t launch_delta_forward(const bsg_delta& a, hipStream_t st) { return run(a, false, st); }
 hipError_t launch_delta_backward(const bsg_delta& a, hipStream_t st) { return run(a, true, st); }
-int64_t delta_work_bytes(const bsg_delta& a) {
-  if (!solved_first(a)) return 0;
-  const int64_t chunks = (int64_t)a.num_envs * a.heads_v * ((a.steps + C - 1) / C);
-  return chunks * (a.dtype == BSG_BF16 ? solved_bytes<mma::bf16>() : solved_bytes<float>());
+int64_t delta_work_bytes(const bsg_delta& a, bool back) {
+  const int64_t chunks = (int64_t)a.num_envs * a.heads_k * ((a.steps + C - 1) / C);
+  return solved_work(a) + (back && a.heads_v > a.heads_k ? chunks * C * a.dim_k * 2 * 4 : 0);
 }
 hipError_t launch_delta_step(const bsg_delta_act& a, hipStream_t st) { return run(a, false, st); }
 

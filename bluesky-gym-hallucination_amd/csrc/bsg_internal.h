@@ -165,7 +165,7 @@ hipError_t launch_sac_actor(const bsg_sac_actor& w, const float* obs, int E, int
 // the memory operators (bsg_delta.hip, bsg_attention.hip)
 hipError_t launch_delta_forward(const bsg_delta& a, hipStream_t stream);
 hipError_t launch_delta_backward(const bsg_delta& a, hipStream_t stream);
-int64_t delta_work_bytes(const bsg_delta& a);
+int64_t delta_work_bytes(const bsg_delta& a, bool backward);
 hipError_t launch_delta_step(const bsg_delta_act& a, hipStream_t stream);
 hipError_t launch_attention(const bsg_attention& a, bool backward, hipStream_t stream);
 bool attention_wants_parts(const bsg_attention& a);

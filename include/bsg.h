@@ -390,7 +390,7 @@ typedef struct bsg_delta {
    * chunks = ceil(steps / BSG_DELTA_CHUNK); the order of their values is the library's */
   float* kept_states;        /* [num_envs][heads_v][chunks] x dim_k x dim_v */
   float* kept_w;             /* [num_envs][heads_v][chunks] x BSG_DELTA_CHUNK x dim_v */
-  void* work;                /* scratch of bsg_delta_work_bytes() bytes, NULL if that is 0; each pass's own */
+  void* work;                /* scratch of bsg_delta_work_bytes() bytes for the pass, NULL if that is 0 */
   /* backward only */
   bsg_rows dout, dq, dk, dv, dg, dbeta;
   const float* dfinal;       /* gradient of final_state; NULL = 0 */
@@ -398,7 +398,7 @@ typedef struct bsg_delta {
   float* work_states;        /* scratch, as kept_states */
   float* work_w;             /* scratch, as kept_w */
 } bsg_delta;
-int64_t bsg_delta_work_bytes(const bsg_delta* a);
+int64_t bsg_delta_work_bytes(const bsg_delta* a, int32_t backward);
 int32_t bsg_delta_forward(const bsg_delta* a, void* stream);
 int32_t bsg_delta_backward(const bsg_delta* a, void* stream);
 /* One step of every env, with the state updated in place; a first step forgets it, whatever it

@@ -146,9 +146,12 @@ def test_packed_blocks_are_the_structures():
 def test_delta_work_is_wanted_where_rows_are_few():
     """Scratch for chunks solved beforehand: few envs x heads, more than one chunk."""
     lib = nat.load_library()
-    need = lambda **kw: lib.bsg_delta_work_bytes(C.byref(delta_args(**kw)))  # noqa: E731
+    need = lambda back=0, **kw: lib.bsg_delta_work_bytes(C.byref(delta_args(**kw)), back)  # noqa: E731
     assert need() == 0 and need(steps=64) == 0 and need(steps=65, dim_v=32) == 0 and need(steps=65, num_envs=4096) == 0
     assert need(steps=65) == 2 * 2 * (need(steps=65, num_envs=1) // 2) > 0 and need(steps=-1) == INVALID
+    # and for the sums over value heads that share a key head, backward
+    assert need(1, steps=64, heads_v=3) == 2 * 64 * 64 * 2 * 4 and need(0, steps=64, heads_v=3) == 0 and need(1, steps=64) == 0
+    assert lib.bsg_delta_backward(C.byref(delta_args(steps=64, heads_v=3)), None) == INVALID
     for fn in ("bsg_delta_forward", "bsg_delta_backward"):
         assert getattr(lib, fn)(C.byref(delta_args(steps=65)), None) == INVALID
         assert getattr(lib, fn)(C.byref(delta_args(steps=65, work=P + 4)), None) == INVALID
