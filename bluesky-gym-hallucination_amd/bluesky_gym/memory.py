@@ -28,7 +28,7 @@ HIP graph.  ``first`` and ``lengths`` are read again by the backward pass.  No C
 """
 from __future__ import annotations
 
-import ctypes as C
+from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -196,14 +196,16 @@ def _delta_check(who, q, k, v, g, beta, state, first, lead):
         _shape(who, "first", first, lead, _FLAGS)
 
 
-def _with_work(fn, before, after, dev):
-    """The call with the fields around bsg_delta.work, and the scratch that it wants there."""
-    block = _pack_delta(*before, 0, *after)
-    need = nat.load_library().bsg_delta_work_bytes(block, fn == "bsg_delta_backward")
-    if need > 0:
-        work = torch.empty(need, dtype=torch.uint8, device=dev)
-        block = _pack_delta(*before, work.data_ptr(), *after)
-    _call(fn, block, dev)
+@lru_cache(maxsize=256)
+def _delta_sizes(E, T, Hk, H, Dk, Dv, dtype):
+    """From the sizes alone: floats of kept_states and of kept_w, bytes of work forward and backward."""
+    block = _pack_delta(E, T, Hk, H, Dk, Dv, dtype, dtype, 1.0, 0, *_NO_ROWS * 6, 0, 0, 0, 0, 0, 0, 0, 0, 0, *_NO_ROWS * 6, 0, 0, 0, 0)
+    work = [nat.load_library().bsg_delta_work_bytes(block, back) for back in (0, 1)]
+    for n in work:
+        if n < 0:
+            nat.check(n, "bsg_delta_work_bytes")
+    rows = E * H * -(-T // nat.DELTA_CHUNK) * Dv
+    return rows * Dk, rows * nat.DELTA_CHUNK, *work
 
 
 class _DeltaRule(torch.autograd.Function):
@@ -212,19 +214,20 @@ class _DeltaRule(torch.autograd.Function):
         q, k, v = _vectors(q), _vectors(k), _vectors(v)
         state = None if state is None else state.contiguous()
         E, T, H, Dv = v.shape
-        Dk, dev = q.shape[-1], v.device
+        Hk, Dk, dev = q.shape[2], q.shape[3], v.device
+        ns, nw, work, _ = _delta_sizes(E, T, Hk, H, Dk, Dv, dtype)
         out = _empty_like(v)
         final = torch.empty((E, H, Dk, Dv), dtype=torch.float32, device=dev)
-        states = w = None
-        if keep:
-            n = -(-T // nat.DELTA_CHUNK)
-            states = torch.empty((E, H, n, Dk, Dv), dtype=torch.float32, device=dev)
-            w = torch.empty((E, H, n * nat.DELTA_CHUNK, Dv), dtype=torch.float32, device=dev)
-        _with_work("bsg_delta_forward", (
+        scratch = torch.empty(work, dtype=torch.uint8, device=dev) if work else None
+        kept, at = None, (0, 0)
+        if keep:                               # the states, then w
+            kept = torch.empty(ns + nw, dtype=torch.float32, device=dev)
+            at = kept.data_ptr(), kept.data_ptr() + 4 * ns
+        _call("bsg_delta_forward", _pack_delta(
             *_delta_inputs(dtype, scale, q, k, v, g, beta, _rows(out), first, lengths), _ptr(state), final.data_ptr(),
-            _ptr(states), _ptr(w)), (*_NO_ROWS * 6, 0, 0, 0, 0), dev)
+            *at, _ptr(scratch), *_NO_ROWS * 6, 0, 0, 0, 0), dev)
         if keep:
-            ctx.save_for_backward(q, k, v, g, beta, first, lengths, states, w)
+            ctx.save_for_backward(q, k, v, g, beta, first, lengths, kept)
             ctx.rest = scale, dtype
             ctx.set_materialize_grads(False)
         return out, final
@@ -232,20 +235,23 @@ class _DeltaRule(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dfinal):
-        q, k, v, g, beta, first, lengths, states, w = ctx.saved_tensors
+        q, k, v, g, beta, first, lengths, kept = ctx.saved_tensors
         scale, dtype = ctx.rest
+        E, T, H, Dv = v.shape
+        Hk, Dk, dev = q.shape[2], q.shape[3], v.device
+        ns, nw, _, work = _delta_sizes(E, T, Hk, H, Dk, Dv, dtype)
         dout = torch.zeros_like(v, memory_format=torch.contiguous_format) if dout is None else _vectors(dout)
         dfinal = None if dfinal is None else dfinal.contiguous()
         dq, dk, dv = _empty_like(q), _empty_like(k), _empty_like(v)
-        dg, db = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (g, beta))
-        dstate = None
-        if ctx.needs_input_grad[5]:
-            dstate = torch.empty((v.shape[0], v.shape[2], q.shape[-1], v.shape[-1]), dtype=torch.float32, device=v.device)
-        ws, ww = torch.empty_like(states), torch.empty_like(w)
-        _with_work("bsg_delta_backward", (
-            *_delta_inputs(dtype, scale, q, k, v, g, beta, _NO_ROWS, first, lengths), 0, 0, states.data_ptr(),
-            w.data_ptr()), (*_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv), *_rows(dg), *_rows(db), _ptr(dfinal),
-                            _ptr(dstate), ws.data_ptr(), ww.data_ptr()), v.device)
+        dg = torch.empty(g.shape, dtype=g.dtype, device=dev)
+        db = torch.empty(beta.shape, dtype=beta.dtype, device=dev)
+        dstate = torch.empty((E, H, Dk, Dv), dtype=torch.float32, device=dev) if ctx.needs_input_grad[5] else None
+        scratch = torch.empty(4 * (ns + nw) + work, dtype=torch.uint8, device=dev)
+        p, s = kept.data_ptr(), scratch.data_ptr()
+        _call("bsg_delta_backward", _pack_delta(
+            *_delta_inputs(dtype, scale, q, k, v, g, beta, _NO_ROWS, first, lengths), 0, 0, p, p + 4 * ns,
+            s + 4 * (ns + nw), *_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv), *_rows(dg), *_rows(db), _ptr(dfinal),
+            _ptr(dstate), s, s + 4 * ns), dev)
         return dq, dk, dv, dg, db, dstate, None, None, None, None, None
 
 
@@ -319,6 +325,26 @@ def _attention_block(dtype, numbers, q, k, v, slopes, first, lengths, begins, ls
                            _ptr(rest), *grads, delta, parts)
 
 
+@lru_cache(maxsize=256)
+def _attention_parts(E, T, H, Hk, D, dtype):
+    """Bytes of bsg_attention.parts, from the sizes alone."""
+    r = (16, 0, 0, 0)                          # an address that is checked and never followed
+    n = nat.load_library().bsg_attention_parts_bytes(
+        _pack_attention(E, T, H, Hk, D, dtype, 0, 1.0, 0.0, 0, *r * 4, *[0] * 8, *_NO_ROWS * 4, 0, 0))
+    if n < 0:
+        nat.check(n, "bsg_attention_parts_bytes")
+    return n
+
+
+@lru_cache(maxsize=256)
+def _attention_step_work(E, S, H, Hk, D, dtype):
+    n = nat.load_library().bsg_attention_step_bytes(
+        _pack_attention_act(E, S, H, Hk, D, dtype, 1.0, 0.0, *_NO_ROWS * 4, *[0] * 8))
+    if n < 0:
+        nat.check(n, "bsg_attention_step_bytes")
+    return n
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, first, lengths, slopes, numbers, dtype, keep):
@@ -348,13 +374,11 @@ class _Attention(torch.autograd.Function):
         numbers, dtype = ctx.rest
         dout = _vectors(dout)
         dq, dk, dv, delta = _empty_like(q), _empty_like(k), _empty_like(v), torch.empty_like(lse)
-        grads = (*_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv))
-        block, parts = _attention_block(dtype, numbers, *saved, out, grads, delta.data_ptr()), None
-        need = nat.load_library().bsg_attention_parts_bytes(block)
-        if need > 0:
-            parts = torch.empty(need // 4, dtype=torch.float32, device=q.device)
-            block = _attention_block(dtype, numbers, *saved, out, grads, delta.data_ptr(), parts.data_ptr())
-        _call("bsg_attention_backward", block, q.device)
+        need = _attention_parts(*q.shape[:3], k.shape[2], q.shape[3], dtype)
+        parts = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _call("bsg_attention_backward", _attention_block(
+            dtype, numbers, *saved, out, (*_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv)), delta.data_ptr(), _ptr(parts)),
+            q.device)
         return dq, dk, dv, None, None, None, None, None, None
 
 
@@ -429,13 +453,10 @@ def episode_attention_step(q, k, v, k_cache, v_cache, steps, first=None, *, scal
     if E == 0:
         return out
     q, k, v = _vectors(q), _vectors(k), _vectors(v)
-    fields = (E, S, H, Hk, D, dtype, scale, softcap, *_step_rows(q), *_step_rows(k), *_step_rows(v), *_step_rows(out),
-              _ptr(slopes), _ptr(first), 0 if first is None else first.stride(0), steps.data_ptr(), k_cache.data_ptr(),
-              v_cache.data_ptr())
-    block, work = _pack_attention_act(*fields, 0, 0), None
-    need = nat.load_library().bsg_attention_step_bytes(block)
-    if need > 0:
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        block = _pack_attention_act(*fields, work.data_ptr(), need)
-    _call("bsg_attention_step", block, q.device)
+    need = _attention_step_work(E, S, H, Hk, D, dtype)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _call("bsg_attention_step", _pack_attention_act(
+        E, S, H, Hk, D, dtype, scale, softcap, *_step_rows(q), *_step_rows(k), *_step_rows(v), *_step_rows(out),
+        _ptr(slopes), _ptr(first), 0 if first is None else first.stride(0), steps.data_ptr(), k_cache.data_ptr(),
+        v_cache.data_ptr(), _ptr(work), need), q.device)
     return out
