@@ -835,8 +835,9 @@ template <class A> int32_t check_delta(const A* a, int steps, const char* who) {
   if ((a->dtype != BSG_F32 && a->dtype != BSG_BF16) || (a->gate_dtype != BSG_F32 && a->gate_dtype != a->dtype))
     return fail(BSG_E_INVALID_ARG, "%s: dtype must be BSG_F32 or BSG_BF16, gate_dtype that or BSG_F32", who);
   const int64_t chunks = ((int64_t)steps + BSG_DELTA_CHUNK - 1) / BSG_DELTA_CHUNK;
-  if ((int64_t)a->num_envs * a->heads_v * (chunks > 4 ? chunks : 4) > 0x7fffffffll)
-    return fail(BSG_E_INVALID_ARG, "%s: num_envs x heads_v x chunks exceeds 2^31 - 1", who);
+  // a launch holds fewer than 2^32 threads, 512 to a workgroup
+  if ((int64_t)a->num_envs * a->heads_v * (chunks > 1 ? chunks : 1) >= 1ll << 23)
+    return fail(BSG_E_INVALID_ARG, "%s: num_envs x heads_v x chunks must be below 2^23", who);
   return BSG_OK;
 }
 template <class A> bool delta_inputs(const A* a) {
@@ -854,8 +855,9 @@ int32_t check_heads(const char* who, int num_envs, int heads_q, int heads_k, int
   if (!head_dim(dim)) return fail(BSG_E_INVALID_ARG, "%s: dim must be 32, 64 or 128 (got %d)", who, dim);
   if (dtype != BSG_F32 && dtype != BSG_BF16) return fail(BSG_E_INVALID_ARG, "%s: dtype must be BSG_F32 or BSG_BF16", who);
   if (!(softcap >= 0.0f)) return fail(BSG_E_INVALID_ARG, "%s: softcap must be >= 0", who);
-  if ((int64_t)num_envs * heads_q * per_head > 0x7fffffffll)
-    return fail(BSG_E_INVALID_ARG, "%s: num_envs x heads_q x tiles exceeds 2^31 - 1", who);
+  // a launch holds fewer than 2^32 threads, 256 to a workgroup
+  if ((int64_t)num_envs * heads_q * (per_head > 1 ? per_head : 1) >= 1ll << 24)
+    return fail(BSG_E_INVALID_ARG, "%s: num_envs x heads_q x tiles of 64 steps must be below 2^24", who);
   return BSG_OK;
 }
 int32_t check_attention(const bsg_attention* a, const char* who) {

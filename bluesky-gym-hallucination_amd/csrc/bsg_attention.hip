@@ -555,14 +555,18 @@ __global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) dk[i][d] = dv[i][d] = f32x4{0, 0, 0, 0};
   }
-  // the queries that see one of the keys end where the next episode (window) begins
+  // the queries that see one of the keys end with the tile where the next episode (window) has begun:
+  // begins never falls, so halving finds it
   int qend = n;
-  if (begins)
-    for (int q = k0 + TILE; q < n; q += TILE)
-      if (begins[q] > k0 + TILE * QW - 1) {
-        qend = q;
-        break;
-      }
+  if (begins && k0 < n) {
+    int some = 0, none = (n - k0 + TILE - 1) / TILE;             // tiles from k0 that see, that do not
+    while (none - some > 1) {
+      const int t = (some + none) / 2;
+      if (begins[k0 + t * TILE] > k0 + TILE * QW - 1) none = t;
+      else some = t;
+    }
+    qend = min(n, k0 + none * TILE);
+  }
 
   Fetch<T, TILE, D, 256> fq, fd;
   float flse = 0.0f, fdelta = 0.0f;

@@ -41,6 +41,7 @@ constexpr int C = BSG_DELTA_CHUNK;
 constexpr int AP = C + 4;          // row pitch of the C x C matrices in LDS
 constexpr int IP = 20;             // ... of the 16 x 16 inverses
 constexpr float LOWEST = -1e5f;    // the least log decay: its exponential is 0
+__device__ __forceinline__ float at_least_lowest(float g) { return g < LOWEST ? LOWEST : g; }   // NaN stays
 
 template <class T> __device__ __forceinline__ const T* row(const bsg_rows& x, int e, int t, int h) {
   return static_cast<const T*>(x.p) + e * x.env + t * x.step + h * x.head;
@@ -117,7 +118,7 @@ __device__ __forceinline__ RawGates load_gates(const GateSteps& s, int t0, int r
   return r;
 }
 __device__ __forceinline__ void make_gates(Gates& s, const RawGates& raw, bool half, int lane) {
-  double c = (double)fmaxf(__uint_as_float(half ? raw.g << 16 : raw.g), LOWEST) * 1.4426950408889634074;
+  double c = (double)at_least_lowest(__uint_as_float(half ? raw.g << 16 : raw.g)) * 1.4426950408889634074;
   const unsigned long long begun = __ballot(raw.first != 0);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -1044,7 +1045,7 @@ __global__ __launch_bounds__(256) void step_kernel(bsg_delta_act a, int64_t wave
     S[i] = first ? f32x4{0, 0, 0, 0} : *reinterpret_cast<const f32x4*>(st + (i * RG + rg) * DV);
   const T *kr = row<T>(a.k, e, 0, hk), *qr = row<T>(a.q, e, 0, hk);
   const f32x4 v = widen(*reinterpret_cast<const Half<T>*>(row<T>(a.v, e, 0, h) + c0));
-  const float alpha = expf(fmaxf(gate(a.g, a.gate_dtype, e, 0, h), LOWEST)), beta = gate(a.beta, a.gate_dtype, e, 0, h);
+  const float alpha = expf(at_least_lowest(gate(a.g, a.gate_dtype, e, 0, h))), beta = gate(a.beta, a.gate_dtype, e, 0, h);
   float k[N], kq = 0.0f;
   f32x4 sk = {0, 0, 0, 0}, sq = {0, 0, 0, 0};
 #pragma unroll

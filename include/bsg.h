@@ -360,7 +360,8 @@ int32_t bsg_policy_sac(const bsg_sac_actor* actor, const float* obs, int32_t num
  * read, and their outputs and gradients are written as zeros.  The values of the steps before
  * it have to be finite where the output is to be: a non-finite value may reach every output of
  * its env, but no other env's.
- * All calls are asynchronous on `stream`, capturable, and use no memory but the caller's. */
+ * All calls are asynchronous on `stream`, capturable, use no memory but the caller's and add nothing
+ * in an order that varies.  Outputs may not overlap inputs. */
 enum { BSG_F32 = 0, BSG_BF16 = 1 };
 typedef struct bsg_rows {
   void* p;
@@ -372,7 +373,8 @@ typedef struct bsg_rows {
  * Query/key head h serves the value heads h r .. h r + r - 1, r = heads_v / heads_k.
  * g <= 0 is the log of the decay (values below -1e5 act as -1e5: nothing is left).  The solve
  * inside a chunk of steps is well conditioned for unit keys and beta in [0, 2].
- * dims: 32, 64 or 128.  gates (g, beta, their gradients): dtype or fp32. */
+ * dims: 32, 64 or 128; num_envs x heads_v x chunks below 2^23.  gates (g, beta, their gradients):
+ * dtype or fp32. */
 #define BSG_DELTA_CHUNK 64
 typedef struct bsg_delta {
   int32_t num_envs, steps;
@@ -419,7 +421,8 @@ int32_t bsg_delta_step(const bsg_delta_act* a, void* stream);
  *   s_ij = scale q_i.k_j, capped to softcap tanh(s_ij / softcap) if softcap > 0, less
  *   slopes[h] (i - j);  out_i = sum_j softmax_j(s_ij) v_j
  * over j <= i of the same episode, and i - j < window if window > 0.  Key/value head h serves
- * the query heads h r .. h r + r - 1, r = heads_q / heads_k.  dim: 32, 64 or 128. */
+ * the query heads h r .. h r + r - 1, r = heads_q / heads_k.  dim: 32, 64 or 128; num_envs x heads_q x
+ * tiles of 64 steps below 2^24. */
 typedef struct bsg_attention {
   int32_t num_envs, steps;
   int32_t heads_q, heads_k, dim;

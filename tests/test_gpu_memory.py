@@ -121,6 +121,14 @@ DELTA = [  # E, T, Hk, H, Dk, Dv, dtype, first, lengths, order, state, gates
     (2, 200, 1, 1, 128, 128, "fp32", None, None, "te", True, None),
     (1, 321, 1, 1, 64, 128, "bf16", "0.004", None, "odd", True, None),
     (5, 70, 4, 4, 32, 32, "bf16", None, "ragged", "et", True, None),
+    # rows enough for every CU: chunks are solved in place
+    (64, 70, 2, 4, 32, 64, "bf16", "0.03", "ragged", "te", True, None),
+    (64, 66, 4, 4, 64, 64, "fp32", "0.05", None, "te", True, None),
+    (86, 66, 1, 3, 32, 128, "bf16", None, None, "et", False, "fp32"),
+    (65, 129, 4, 4, 32, 128, "fp32", "0.01", "ragged", "te", True, None),
+    (129, 65, 1, 2, 128, 32, "bf16", "edges", None, "te", True, None),
+    (260, 65, 1, 1, 128, 64, "bf16", None, "ragged", "te", True, None),
+    (256, 65, 1, 1, 128, 128, "fp32", "0.1", None, "te", True, None),
 ]
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
 
@@ -270,6 +278,12 @@ ATTEND = [  # E, T, H, Hk, D, dtype, first, lengths, order, softcap, bias, windo
     (1, 321, 4, 1, 128, "bf16", None, None, "odd", 0.0, True, 0, 3.0),
     (1, 300, 2, 2, 64, "fp32", "0.004", None, "te", 30.0, True, 200, 4.0),
     (5, 70, 5, 5, 32, "bf16", None, "ragged", "et", 0.0, False, 0, 8.0),
+    # two tiles of queries to a wave; one key head of many envs, without partial sums
+    (1, 600, 2, 1, 64, "bf16", "0.005", None, "te", 15.0, True, 0, 2.0),
+    (2, 577, 2, 2, 128, "bf16", None, "ragged", "te", 0.0, False, 0, 2.0),
+    (2, 530, 3, 1, 32, "bf16", "0.02", "ragged", "gap", 0.0, True, 100, 1.0),
+    (350, 130, 2, 1, 32, "bf16", "0.05", "ragged", "te", 0.0, True, 0, 1.0),
+    (350, 130, 2, 1, 32, "fp32", None, None, "te", 4.0, False, 0, 1.0),
 ]
 
 
@@ -589,6 +603,68 @@ def test_graph_capture_and_replay():
         for a, w in zip(captured, want):
             assert torch.equal(a, w)
         assert torch.equal(steps, n0 + 1)
+
+
+def test_backward_twice_and_again_is_the_same():
+    """A kept graph's second backward pass, and a second forward and backward, repeat bit for bit."""
+    x, dout, g = attention_data(3, 200, 4, 2, 64, torch.bfloat16, 61)
+    d, do2, state, _ = delta_data(3, 200, 2, 4, 64, 64, torch.bfloat16, 62)
+    first = flags(3, 200, "0.02", g).to(DEV)
+    a = {n: v.to(DEV).requires_grad_(True) for n, v in x.items()}
+    b = {n: v.to(DEV).requires_grad_(True) for n, v in d.items()}
+    runs = []
+    for _ in range(2):
+        o1 = memory.episode_attention(**a, first=first)
+        o2, f = memory.gated_delta_rule(**b, state=state.to(DEV), first=first)
+        for keep in (True, False):
+            runs.append([o1.detach(), o2.detach(), f.detach(), *torch.autograd.grad(
+                [o1, o2], list(a.values()) + list(b.values()), [dout.to(DEV), do2.to(DEV)], retain_graph=keep)])
+    for r in runs[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(r, runs[0]))
+
+
+def test_only_some_inputs_and_the_state_alone_need_gradients():
+    d, dout, state, _ = delta_data(2, 70, 1, 2, 32, 32, torch.float32, 63)
+    dev = {n: v.to(DEV) for n, v in d.items()}
+    st = state.to(DEV).requires_grad_(True)
+    out, fin = memory.gated_delta_rule(**dev, state=st)
+    got, = torch.autograd.grad(fin.sum(), st)          # out takes no part: its gradient is None
+    ref = {n: d64(v) for n, v in d.items()}
+    sr = d64(state).requires_grad_(True)
+    want, = torch.autograd.grad(delta_ref(**ref, state=sr)[1].sum(), sr)
+    close(got, want, delta_tol(want, torch.float32, (0, 1), True, state=True), "dstate")
+    x, do, _ = attention_data(2, 70, 2, 1, 32, torch.float32, 64)
+    q, k, v = (x[n].to(DEV) for n in "qkv")
+    v.requires_grad_(True)
+    got, = torch.autograd.grad(memory.episode_attention(q, k, v), v, do.to(DEV))
+    (_, _), grads = attention_tols(x, d64(do), torch.float32)
+    close(got, *grads[2], "dv")
+
+
+def test_nan_gate_is_not_hidden():
+    d, _, state, _ = delta_data(2, 70, 1, 1, 32, 32, torch.float32, 65)
+    d["g"][0, 40] = float("nan")
+    dev = {n: v.to(DEV) for n, v in d.items()}
+    out, fin = memory.gated_delta_rule(**dev, state=state.to(DEV))
+    assert out[0, 40:].isnan().all() and fin[0].isnan().all()
+    assert out[1].isfinite().all() and fin[1].isfinite().all()      # no other env's
+    st = state.to(DEV)
+    memory.gated_delta_step(*(dev[n][:, 40] for n in ("q", "k", "v", "g", "beta")), state=st)
+    assert st[0].isnan().all() and st[1].isfinite().all()
+
+
+def test_ring_whose_offsets_pass_32_bits():
+    """More than 2^31 values to a ring: the last slots are found, the step goes where it belongs."""
+    S, D = 34_000_000, 64
+    kc = torch.zeros(1, 1, S, D, dtype=torch.bfloat16, device=DEV)
+    vc = torch.zeros(1, 1, S, D, dtype=torch.bfloat16, device=DEV)
+    q = torch.ones(1, 1, D, dtype=torch.bfloat16, device=DEV)
+    kc[0, 0, S - 2] = 40 * D ** 0.5 / D                # score 40: e^40 against S e^0
+    vc[0, 0, S - 2] = 3.0
+    steps = torch.tensor([S - 1], dtype=torch.int32, device=DEV)
+    out = memory.episode_attention_step(q, torch.zeros_like(q), torch.full_like(q, 5.0), kc, vc, steps)
+    assert (out.float() - 3.0).abs().max().item() <= 3 * 2.0 ** -8 and steps.item() == S
+    assert (vc[0, 0, S - 1] == 5).all() and (vc[0, 0, S - 2] == 3).all() and not vc[0, 0, :4].any()
 
 
 def test_side_stream_and_two_calls_in_flight():

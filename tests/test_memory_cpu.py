@@ -77,7 +77,7 @@ def act_args(**kw):
 
 INVALID = -1
 BAD_DELTA = [dict(num_envs=-1), dict(steps=-1), dict(heads_k=0), dict(heads_k=2, heads_v=3), dict(dim_k=48), dict(dim_v=256),
-             dict(dtype=2), dict(gate_dtype=1), dict(dtype=1, gate_dtype=2), dict(num_envs=1 << 30), dict(q=rows(0)),
+             dict(dtype=2), dict(gate_dtype=1), dict(dtype=1, gate_dtype=2), dict(num_envs=1 << 23), dict(q=rows(0)),
              dict(k=rows(P + 4)), dict(v=rows(env=3)), dict(g=rows(0)), dict(beta=rows(0))]
 
 
@@ -105,7 +105,7 @@ def test_delta_calls_refuse(fn, kw):
 
 @pytest.mark.parametrize("kw", [
     dict(num_envs=-1), dict(steps=-1), dict(window=-1), dict(heads_q=0), dict(heads_q=3, heads_k=2), dict(dim=16), dict(dtype=7),
-    dict(softcap=-1.0), dict(softcap=float("nan")), dict(num_envs=1 << 30), dict(q=rows(0)), dict(k=rows(P + 2)), dict(out=rows(head=2)),
+    dict(softcap=-1.0), dict(softcap=float("nan")), dict(num_envs=1 << 23), dict(num_envs=1 << 20, steps=1000), dict(q=rows(0)), dict(k=rows(P + 2)), dict(out=rows(head=2)),
     dict(window=4), dict(first=P)], ids=str)
 def test_attention_entry_points_refuse(kw):
     lib = nat.load_library()
@@ -122,7 +122,7 @@ def test_attention_backward_refuses(kw):
 
 @pytest.mark.parametrize("kw", [
     dict(num_envs=-1), dict(slots=0), dict(slots=-5), dict(slots=(1 << 30) + 1), dict(heads_q=3, heads_k=2), dict(dim=65), dict(dtype=-1),
-    dict(softcap=-1.0), dict(q=rows(0)), dict(out=rows(P + 8)), dict(steps=None), dict(k_cache=None), dict(v_cache=P + 2), dict(work=None),
+    dict(softcap=-1.0), dict(num_envs=1 << 23), dict(q=rows(0)), dict(out=rows(P + 8)), dict(steps=None), dict(k_cache=None), dict(v_cache=P + 2), dict(work=None),
     dict(work_bytes=16)], ids=str)
 def test_attention_step_refuses(kw):
     assert nat.load_library().bsg_attention_step(C.byref(act_args(**kw)), None) == INVALID
