@@ -14,8 +14,6 @@
 #include <math.h>
 #include <stdint.h>
 
-#include <type_traits>
-
 #include "bsg_internal.h"
 #include "bsg_mma.h"
 
@@ -145,15 +143,15 @@ __global__ __launch_bounds__(256) void forward_kernel(bsg_attention a) {
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) o[i][d] = f32x4{0, 0, 0, 0};
   }
-  const auto tile = [&](int k0, auto masked) {
-    constexpr bool MASK = decltype(masked)::value;
+  const auto tile = [&](int k0, bool masked) {
     f32x4 s[QW][KT];
     float top[QW];
 #pragma unroll
     for (int i = 0; i < QW; ++i) top[i] = mx[i];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      if (MASK && k0 + 16 * t > qw + 16 * QW - 1) {              // behind the wave's last query
+      // behind the wave's last query (fp32: worth a branch)
+      if (sizeof(T) == 4 && k0 + 16 * t > qw + 16 * QW - 1) {
 #pragma unroll
         for (int i = 0; i < QW; ++i) s[i][t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         continue;
@@ -173,19 +171,22 @@ __global__ __launch_bounds__(256) void forward_kernel(bsg_attention a) {
         for (int r = 0; r < 4; ++r) {
           float y;
           s[i][t][r] = score<T, CAP, BIAS>(sc, s[i][t][r], ago - (float)(16 * t + r), y);
-          if (MASK) {
+        }
+        if (masked)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
             const int j = k0 + 16 * t + 4 * g + r;
             s[i][t][r] = j <= qi[i] && j >= begin[i] ? s[i][t][r] : -INFINITY;
           }
-          top[i] = fmaxf(top[i], s[i][t][r]);
-        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top[i] = fmaxf(top[i], s[i][t][r]);
       }
     }
 #pragma unroll
     for (int i = 0; i < QW; ++i) {
       top[i] = max_groups(top[i]);
       // a query whose keys all lie in other tiles has nothing yet: exp2(-inf - 0) = 0
-      const float base = MASK && top[i] == -INFINITY ? 0.0f : top[i];
+      const float base = top[i] == -INFINITY ? 0.0f : top[i];
       const float old = __builtin_amdgcn_exp2f(mx[i] - base);
       mx[i] = top[i];
       sum[i] *= old;
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(256) void forward_kernel(bsg_attention a) {
     }
 #pragma unroll
     for (int c = 0; c < KT / 2; ++c) {
-      if (MASK && k0 + 32 * c > qw + 16 * QW - 1) continue;
+      if (sizeof(T) == 4 && k0 + 32 * c > qw + 16 * QW - 1) continue;
       Frag<T> pf[QW];
 #pragma unroll
       for (int i = 0; i < QW; ++i) pf[i] = round_frag<T>(join(s[i][2 * c], s[i][2 * c + 1]));
@@ -228,8 +229,7 @@ __global__ __launch_bounds__(256) void forward_kernel(bsg_attention a) {
     }
     __syncthreads();
     if (qw >= n || k0 > qw + 16 * QW - 1 || k0 + TILE <= see_any) continue;
-    if (k0 + TILE - 1 <= qw && k0 >= see_all) tile(k0, std::false_type());
-    else tile(k0, std::true_type());
+    tile(k0, k0 + TILE - 1 > qw || k0 < see_all);
   }
 #pragma unroll
   for (int i = 0; i < QW; ++i) {
@@ -254,18 +254,26 @@ __global__ __launch_bounds__(256) void forward_kernel(bsg_attention a) {
 }
 
 // ---- backward ------------------------------------------------------------------------------
-// p and ds of 16 keys (rows 4g + r, from key j0) and a lane's query, or of 16 queries and a lane's
-// key (SWAP: i0 and `at` change places).
-template <class T, bool CAP, bool BIAS>
-__device__ __forceinline__ void p_and_ds(const Score& sc, float ago, const f32x4& step, const f32x4& lse,
-                                         const f32x4& delta, const f32x4& s, const f32x4& dp, f32x4& p, f32x4& ds) {
+// p and ds of 16 keys (rows 4g + r) and a lane's query, or of 16 queries and a lane's key, `ago` +
+// `step` apart; where an edge crosses the tile, on(r) says which are seen.
+template <class T, bool CAP, bool BIAS, class On>
+__device__ __forceinline__ void p_and_ds(const Score& sc, float ago, const f32x4& step, const f32x4& lse, const f32x4& delta,
+                                         const f32x4& s, const f32x4& dp, bool masked, On on, f32x4& p, f32x4& ds) {
+  f32x4 x, y = {0, 0, 0, 0};
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    float y = 0.0f;
-    const float x = score<T, CAP, BIAS>(sc, s[r], ago + step[r], y);
-    p[r] = __builtin_amdgcn_exp2f(x - lse[r]);
+    float t = 0.0f;
+    x[r] = score<T, CAP, BIAS>(sc, s[r], ago + step[r], t) - lse[r];
+    y[r] = t;
+  }
+  if (masked)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = on(r) ? x[r] : -INFINITY;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    p[r] = __builtin_amdgcn_exp2f(x[r]);
     ds[r] = p[r] * (dp[r] - delta[r]);
-    if (CAP) ds[r] *= fmaf(-y, y, 1.0f);
+    if (CAP) ds[r] *= fmaf(-y[r], y[r], 1.0f);
   }
 }
 
@@ -443,11 +451,10 @@ __global__ __launch_bounds__(256) void backward_q_kernel(bsg_attention a) {
   for (int i = 0; i < QW; ++i)
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) dq[i][d] = f32x4{0, 0, 0, 0};
-  const auto tile = [&](int k0, auto masked) {
-    constexpr bool MASK = decltype(masked)::value;
+  const auto tile = [&](int k0, bool masked) {
 #pragma unroll
     for (int c = 0; c < KT / 2; ++c) {
-      if (MASK && k0 + 32 * c > qw + 16 * QW - 1) continue;
+      if (sizeof(T) == 4 && k0 + 32 * c > qw + 16 * QW - 1) continue;
       f32x4 ds[QW][2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -468,13 +475,11 @@ __global__ __launch_bounds__(256) void backward_q_kernel(bsg_attention a) {
         for (int i = 0; i < QW; ++i) {
           f32x4 p;
           const f32x4 l = {lse[i], lse[i], lse[i], lse[i]}, dl = {delta[i], delta[i], delta[i], delta[i]};
-          p_and_ds<T, CAP, BIAS>(sc, (float)(qi[i] - k0 - 4 * g) - (float)(16 * t), f32x4{0, -1, -2, -3}, l, dl, s[i], dp[i], p, ds[i][u]);
-          if (MASK)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int j = k0 + 16 * t + 4 * g + r;
-              ds[i][u][r] = j <= qi[i] && j >= begin[i] ? ds[i][u][r] : 0.0f;
-            }
+          const auto on = [&](int r) {
+            const int j = k0 + 16 * t + 4 * g + r;
+            return j <= qi[i] && j >= begin[i];
+          };
+          p_and_ds<T, CAP, BIAS>(sc, (float)(qi[i] - k0 - 4 * g) - (float)(16 * t), f32x4{0, -1, -2, -3}, l, dl, s[i], dp[i], masked, on, p, ds[i][u]);
         }
       }
       Frag<T> f[QW];
@@ -503,8 +508,7 @@ __global__ __launch_bounds__(256) void backward_q_kernel(bsg_attention a) {
     }
     __syncthreads();
     if (qw >= n || k0 > qw + 16 * QW - 1 || k0 + TILE <= see_any) continue;
-    if (k0 + TILE - 1 <= qw && k0 >= see_all) tile(k0, std::false_type());
-    else tile(k0, std::true_type());
+    tile(k0, k0 + TILE - 1 > qw || k0 < see_all);
   }
 #pragma unroll
   for (int i = 0; i < QW; ++i) {
@@ -583,11 +587,10 @@ __global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
   if (k0 < qend) fetch(h0, k0);
   for (int h = h0; h < h1; ++h) {
     const Score sc = score_of(a.scale, a.softcap, a.slopes, h);
-    const auto tile = [&](int q0, auto masked) {
-      constexpr bool MASK = decltype(masked)::value;
+    const auto tile = [&](int q0, bool masked) {
 #pragma unroll
       for (int c = 0; c < QT / 2; ++c) {
-        if (MASK && q0 + 32 * c + 31 < kw) continue;             // before the wave's first key
+        if (sizeof(T) == 4 && q0 + 32 * c + 31 < kw) continue;   // before the wave's first key
         f32x4 ps[QW][2], ds[QW][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -608,15 +611,11 @@ __global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
           const f32x4 delta = *reinterpret_cast<const f32x4*>(&sDelta[16 * t + 4 * g]);
 #pragma unroll
           for (int i = 0; i < QW; ++i) {
-            p_and_ds<T, CAP, BIAS>(sc, (float)(q0 + 4 * g - kj[i]) + (float)(16 * t), f32x4{0, 1, 2, 3}, lse, delta, s[i], dp[i], ps[i][u], ds[i][u]);
-            if (MASK)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int l = 16 * t + 4 * g + r;
-                const bool on = kj[i] <= q0 + l && kj[i] >= sBegin[l];
-                ps[i][u][r] = on ? ps[i][u][r] : 0.0f;
-                ds[i][u][r] = on ? ds[i][u][r] : 0.0f;
-              }
+            const auto on = [&](int r) {
+              const int l = 16 * t + 4 * g + r;
+              return kj[i] <= q0 + l && kj[i] >= sBegin[l];
+            };
+            p_and_ds<T, CAP, BIAS>(sc, (float)(q0 + 4 * g - kj[i]) + (float)(16 * t), f32x4{0, 1, 2, 3}, lse, delta, s[i], dp[i], masked, on, ps[i][u], ds[i][u]);
           }
         }
         Frag<T> pf[QW], f[QW];
@@ -650,9 +649,8 @@ __global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
       else if (h + 1 < h1) fetch(h + 1, k0);
       __syncthreads();
       if (kw >= n || q0 + TILE - 1 < kw || sBegin[0] > kw + 16 * QW - 1) continue;
-      // every query of the tile sees every key of the wave
-      if (kw + 16 * QW - 1 <= q0 && sBegin[TILE - 1] <= kw) tile(q0, std::false_type());
-      else tile(q0, std::true_type());
+      // unless every query of the tile sees every key of the wave
+      tile(q0, kw + 16 * QW - 1 > q0 || sBegin[TILE - 1] > kw);
     }
   }
 #pragma unroll
