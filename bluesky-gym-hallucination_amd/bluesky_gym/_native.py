@@ -128,7 +128,7 @@ class BsgSacActor(C.Structure):
 
 F32, BF16 = 0, 1             # include/bsg.h BSG_F32, BSG_BF16
 DELTA_CHUNK = 64             # BSG_DELTA_CHUNK
-ATTENTION_TILE = 64          # steps up to which bsg_attention.out_rest is not wanted
+ATTENTION_TILE = 64          # BSG_ATTENTION_TILE: up to it bsg_attention.out_rest is not wanted
 
 
 class BsgRows(C.Structure):

@@ -863,7 +863,7 @@ int32_t check_heads(const char* who, int num_envs, int heads_q, int heads_k, int
 int32_t check_attention(const bsg_attention* a, const char* who) {
   if (!a) return fail(BSG_E_INVALID_ARG, "%s: null arguments", who);
   if (a->steps < 0 || a->window < 0) return fail(BSG_E_INVALID_ARG, "%s: steps or window < 0", who);
-  if (int32_t r = check_heads(who, a->num_envs, a->heads_q, a->heads_k, a->dim, a->dtype, a->softcap, ((int64_t)a->steps + 63) / 64)) return r;
+  if (int32_t r = check_heads(who, a->num_envs, a->heads_q, a->heads_k, a->dim, a->dtype, a->softcap, ((int64_t)a->steps + BSG_ATTENTION_TILE - 1) / BSG_ATTENTION_TILE)) return r;
   if (a->num_envs == 0 || a->steps == 0) return BSG_OK;
   if (!vector_rows(a->q, a->dtype) || !vector_rows(a->k, a->dtype) || !vector_rows(a->v, a->dtype) || !vector_rows(a->out, a->dtype))
     return fail(BSG_E_INVALID_ARG, "%s: q, k, v and out must be there, with 16-byte aligned rows", who);
@@ -949,7 +949,7 @@ int32_t bsg_attention_backward(const bsg_attention* a, void* stream) {
   if (!vector_rows(a->dout, a->dtype) || !vector_rows(a->dq, a->dtype) || !vector_rows(a->dk, a->dtype) || !vector_rows(a->dv, a->dtype))
     return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: dout, dq, dk and dv must be there, with 16-byte aligned rows");
   if (!a->lse || !a->delta) return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: null lse or delta");
-  if (a->dtype == BSG_BF16 && a->steps > 64 && !a->out_rest)
+  if (a->dtype == BSG_BF16 && a->steps > BSG_ATTENTION_TILE && !a->out_rest)
     return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: null out_rest");
   if (bsg::attention_wants_parts(*a) != (a->parts != nullptr) || (reinterpret_cast<uintptr_t>(a->parts) & 15))
     return fail(BSG_E_INVALID_ARG, "bsg_attention_backward: parts must be there, 16-byte aligned, where bsg_attention_parts_bytes is not 0");

@@ -21,7 +21,7 @@ namespace {
 
 using namespace bsg::mma;
 
-constexpr int TILE = 64;           // queries (keys) per workgroup, keys (queries) per pass of its loop
+constexpr int TILE = BSG_ATTENTION_TILE;   // queries (keys) to a workgroup, keys (queries) to a turn of its loop
 constexpr float LOG2E = 1.44269504088896340736f;
 
 template <class T> __device__ __forceinline__ const T* row(const bsg_rows& x, int e, int t, int h) {
@@ -94,124 +94,96 @@ __global__ __launch_bounds__(256) void begins_kernel(const uint8_t* first, int64
 }
 
 // ---- forward -------------------------------------------------------------------------------
-// A workgroup of four waves takes 64 QW queries of one head, a wave 16 QW of them, and walks the
+// A workgroup of four waves takes 64 queries of one head, a wave 16 of them, and walks the
 // keys in tiles of 64, fetched one tile ahead through registers and shared in LDS.  Scores are
 // computed transposed (keys x queries), so a lane holds one query: its running maximum and sum are
 // in-lane but for two lane swaps, and the probabilities lie in registers as the B operand of
-// out^T[dim][query] += V^T[dim][key] P^T[key][query].  QW = 2 halves the LDS reads per product;
-// fp32 operands, which the matrix cores take at a sixteenth of the rate, have no use for it.
+// out^T[dim][query] += V^T[dim][key] P^T[key][query].  (32 queries to a wave read LDS half as often
+// but leave a SIMD half the waves to cover its loads: 605 against 581 us forward and backward at 2 envs x
+// 4095 steps, dim 128; 459 against 370 us at dim 64.)
 // Masks are only applied in tiles that an edge crosses.
-template <class T, int D, int QW, bool CAP, bool BIAS>
+template <class T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) void forward_kernel(bsg_attention a) {
   constexpr int LD = pitch<T>(D), KT = TILE / 16;
   __shared__ __align__(16) T sK[TILE * LD];
   __shared__ __align__(16) T sV[TILE * LD];
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW), id = swizzled(blockIdx.x, gridDim.x);
-  const int q0 = (nt - 1 - id % nt) * TILE * QW;                 // the longest ranges first
+  const int nt = (a.steps + TILE - 1) / TILE, id = swizzled(blockIdx.x, gridDim.x);
+  const int q0 = (nt - 1 - id % nt) * TILE;                 // the longest ranges first
   const int eh = id / nt, h = eh % a.heads_q, e = eh / a.heads_q;
   const int hk = h / (a.heads_q / a.heads_k);
   const int n = a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
-  const int qw = q0 + 16 * QW * w;                               // the wave's first query
+  const int qw = q0 + 16 * w;                               // the wave's first query
   const Score sc = score_of(a.scale, a.softcap, a.slopes, h);
   const int32_t* begins = a.begins ? a.begins + (int64_t)e * a.steps : nullptr;
 
-  Frag<T> qf[QW][D / 32];
-  int qi[QW], begin[QW];
+  Frag<T> qf[D / 32];
+  const int qi = qw + m;
+  // a query behind the last step reads the last one's row and is not written
+  const int at = max(min(qi, n - 1), 0);
+  const T* qr = row<T>(a.q, e, at, h);
 #pragma unroll
-  for (int i = 0; i < QW; ++i) {
-    qi[i] = qw + 16 * i + m;
-    // a query behind the last step reads the last one's row and is not written
-    const int at = max(min(qi[i], n - 1), 0);
-    const T* qr = row<T>(a.q, e, at, h);
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) qf[i][s] = load_run(qr, 32 * s, g);
-    begin[i] = begins ? begins[at] : 0;
-  }
-  const int kend = min(q0 + TILE * QW, n), kbeg = begins && q0 < n ? begins[q0] / TILE * TILE : 0;
+  for (int s = 0; s < D / 32; ++s) qf[s] = load_run(qr, 32 * s, g);
+  const int begin = begins ? begins[at] : 0;
+  const int kend = min(q0 + TILE, n), kbeg = begins && q0 < n ? begins[q0] / TILE * TILE : 0;
   // what the wave's queries see: from the first one's begin; all of them from the last one's
   const int see_any = begins && qw < n ? begins[qw] : 0;
-  const int see_all = begins && qw < n ? begins[min(qw + 16 * QW, n) - 1] : 0;
+  const int see_all = begins && qw < n ? begins[min(qw + 16, n) - 1] : 0;
 
-  f32x4 o[QW][D / 16];
-  float mx[QW], sum[QW];
+  f32x4 o[D / 16];
+  float mx = -INFINITY, sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < QW; ++i) {
-    mx[i] = -INFINITY;
-    sum[i] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) o[i][d] = f32x4{0, 0, 0, 0};
-  }
+  for (int d = 0; d < D / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
   const auto tile = [&](int k0, bool masked) {
-    f32x4 s[QW][KT];
-    float top[QW];
-#pragma unroll
-    for (int i = 0; i < QW; ++i) top[i] = mx[i];
+    f32x4 s[KT];
+    float top = mx;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       // behind the wave's last query (fp32: worth a branch)
-      if (sizeof(T) == 4 && k0 + 16 * t > qw + 16 * QW - 1) {
-#pragma unroll
-        for (int i = 0; i < QW; ++i) s[i][t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (sizeof(T) == 4 && k0 + 16 * t > qw + 15) {
+        s[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         continue;
       }
+      s[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < QW; ++i) s[i][t] = f32x4{0, 0, 0, 0};
+      for (int c = 0; c < D / 32; ++c) mma(s[t], load_run(sK + (16 * t + m) * LD, 32 * c, g), qf[c]);
+      const float ago = (float)(qi - k0 - 4 * g);
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        const Frag<T> kf = load_run(sK + (16 * t + m) * LD, 32 * c, g);
-#pragma unroll
-        for (int i = 0; i < QW; ++i) mma(s[i][t], kf, qf[i][c]);
+      for (int r = 0; r < 4; ++r) {
+        float y;
+        s[t][r] = score<T, CAP, BIAS>(sc, s[t][r], ago - (float)(16 * t + r), y);
       }
-#pragma unroll
-      for (int i = 0; i < QW; ++i) {
-        const float ago = (float)(qi[i] - k0 - 4 * g);
+      if (masked)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float y;
-          s[i][t][r] = score<T, CAP, BIAS>(sc, s[i][t][r], ago - (float)(16 * t + r), y);
+          const int j = k0 + 16 * t + 4 * g + r;
+          s[t][r] = j <= qi && j >= begin ? s[t][r] : -INFINITY;
         }
-        if (masked)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = k0 + 16 * t + 4 * g + r;
-            s[i][t][r] = j <= qi[i] && j >= begin[i] ? s[i][t][r] : -INFINITY;
-          }
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][r]);
+    }
+    top = max_groups(top);
+    // a query whose keys all lie in other tiles has nothing yet: exp2(-inf - 0) = 0
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float old = __builtin_amdgcn_exp2f(mx - base);
+    mx = top;
+    sum *= old;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) top[i] = fmaxf(top[i], s[i][t][r]);
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - base);
+        sum += s[t][r];
       }
-    }
 #pragma unroll
-    for (int i = 0; i < QW; ++i) {
-      top[i] = max_groups(top[i]);
-      // a query whose keys all lie in other tiles has nothing yet: exp2(-inf - 0) = 0
-      const float base = top[i] == -INFINITY ? 0.0f : top[i];
-      const float old = __builtin_amdgcn_exp2f(mx[i] - base);
-      mx[i] = top[i];
-      sum[i] *= old;
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[i][t][r] = __builtin_amdgcn_exp2f(s[i][t][r] - base);
-          sum[i] += s[i][t][r];
-        }
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) o[i][d] *= old;
-    }
+    for (int d = 0; d < D / 16; ++d) o[d] *= old;
 #pragma unroll
     for (int c = 0; c < KT / 2; ++c) {
-      if (sizeof(T) == 4 && k0 + 32 * c > qw + 16 * QW - 1) continue;
-      Frag<T> pf[QW];
+      if (sizeof(T) == 4 && k0 + 32 * c > qw + 15) continue;
+      const Frag<T> pf = round_frag<T>(join(s[2 * c], s[2 * c + 1]));
 #pragma unroll
-      for (int i = 0; i < QW; ++i) pf[i] = round_frag<T>(join(s[i][2 * c], s[i][2 * c + 1]));
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        const Frag<T> vf = load_col(sV, LD, 32 * c, 16 * d, lane);
-#pragma unroll
-        for (int i = 0; i < QW; ++i) mma(o[i][d], vf, pf[i]);
-      }
+      for (int d = 0; d < D / 16; ++d) mma(o[d], load_col(sV, LD, 32 * c, 16 * d, lane), pf);
     }
   };
   Fetch<T, TILE, D, 256> fk, fv;
@@ -228,29 +200,26 @@ __global__ __launch_bounds__(256) void forward_kernel(bsg_attention a) {
       fv.load(row<T>(a.v, e, k0 + TILE, hk), a.v.step, kend - k0 - TILE, tid);
     }
     __syncthreads();
-    if (qw >= n || k0 > qw + 16 * QW - 1 || k0 + TILE <= see_any) continue;
+    if (qw >= n || k0 > qw + 15 || k0 + TILE <= see_any) continue;
     tile(k0, k0 + TILE - 1 > qw || k0 < see_all);
   }
+  if (qi >= a.steps) return;
+  const bool live = qi < n;
+  const float all = sum_groups(sum), inv = live ? 1.0f / all : 0.0f;
+  const int64_t to = ((int64_t)e * a.heads_q + h) * a.steps + qi;
+  T* out = row_out<T>(a.out, e, qi, h);
 #pragma unroll
-  for (int i = 0; i < QW; ++i) {
-    if (qi[i] >= a.steps) continue;
-    const bool live = qi[i] < n;
-    const float all = sum_groups(sum[i]), inv = live ? 1.0f / all : 0.0f;
-    const int64_t at = ((int64_t)e * a.heads_q + h) * a.steps + qi[i];
-    T* out = row_out<T>(a.out, e, qi[i], h);
+  for (int d = 0; d < D / 16; ++d) {
+    const f32x4 x = live ? o[d] * inv : f32x4{0, 0, 0, 0};
+    store4(out + 16 * d + 4 * g, x);
+    if (sizeof(T) == 2 && a.out_rest) {                        // what the rounding left
+      f32x4 rest;
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) {
-      const f32x4 x = live ? o[i][d] * inv : f32x4{0, 0, 0, 0};
-      store4(out + 16 * d + 4 * g, x);
-      if (sizeof(T) == 2 && a.out_rest) {                        // what the rounding left
-        f32x4 rest;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) rest[r] = x[r] - (float)(T)x[r];
-        store4(static_cast<T*>(a.out_rest) + at * D + 16 * d + 4 * g, rest);
-      }
+      for (int r = 0; r < 4; ++r) rest[r] = x[r] - (float)(T)x[r];
+      store4(static_cast<T*>(a.out_rest) + to * D + 16 * d + 4 * g, rest);
     }
-    if (a.lse && g == 0 && live) a.lse[at] = mx[i] + log2f(all);
   }
+  if (a.lse && g == 0 && live) a.lse[to] = mx + log2f(all);
 }
 
 // ---- backward ------------------------------------------------------------------------------
@@ -400,97 +369,73 @@ __global__ __launch_bounds__(256) void backward_short_kernel(bsg_attention a) {
 // Longer rollouts.  dq: as the forward pass, with dp^T = V dout^T next to the scores and
 // dq^T += K^T ds^T.  It also writes delta_i = dout_i.out_i for the pass over keys; out is taken
 // with what its rounding left, else delta would carry that rounding into every ds of the row.
-template <class T, int D, int QW, bool CAP, bool BIAS>
+template <class T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) void backward_q_kernel(bsg_attention a) {
   constexpr int LD = pitch<T>(D), KT = TILE / 16;
   __shared__ __align__(16) T sK[TILE * LD];
   __shared__ __align__(16) T sV[TILE * LD];
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW), id = swizzled(blockIdx.x, gridDim.x);
-  const int q0 = (nt - 1 - id % nt) * TILE * QW;
+  const int nt = (a.steps + TILE - 1) / TILE, id = swizzled(blockIdx.x, gridDim.x);
+  const int q0 = (nt - 1 - id % nt) * TILE;
   const int eh = id / nt, h = eh % a.heads_q, e = eh / a.heads_q;
   const int hk = h / (a.heads_q / a.heads_k);
   const int n = a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
-  const int qw = q0 + 16 * QW * w;
+  const int qw = q0 + 16 * w;
   const Score sc = score_of(a.scale, a.softcap, a.slopes, h);
   const int64_t base = ((int64_t)e * a.heads_q + h) * a.steps;
   const int32_t* begins = a.begins ? a.begins + (int64_t)e * a.steps : nullptr;
 
-  Frag<T> qf[QW][D / 32], df[QW][D / 32];
-  float delta[QW], lse[QW];
-  int qi[QW], begin[QW];
+  Frag<T> qf[D / 32], df[D / 32];
+  const int qi = qw + m, at = max(min(qi, n - 1), 0);            // a query behind the last step: the last one's row
+  const T *qr = row<T>(a.q, e, at, h), *dr = row<T>(a.dout, e, at, h), *orow = row<T>(a.out, e, at, h);
+  const T* rest = static_cast<const T*>(a.out_rest) + (base + at) * D;
+  float x = 0.0f;
 #pragma unroll
-  for (int i = 0; i < QW; ++i) {
-    qi[i] = qw + 16 * i + m;
-    const int at = max(min(qi[i], n - 1), 0);      // a query behind the last step: the last one's row
-    const T *qr = row<T>(a.q, e, at, h), *dr = row<T>(a.dout, e, at, h), *orow = row<T>(a.out, e, at, h);
-    const T* rest = static_cast<const T*>(a.out_rest) + (base + at) * D;
-    float x = 0.0f;
+  for (int s = 0; s < D / 32; ++s) {
+    qf[s] = load_run(qr, 32 * s, g);
+    df[s] = load_run(dr, 32 * s, g);
+    const f32x8 u = widen(df[s]);
+    f32x8 v = widen(load_run(orow, 32 * s, g));
+    if (sizeof(T) == 2) v += widen(load_run(rest, 32 * s, g));
 #pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      qf[i][s] = load_run(qr, 32 * s, g);
-      df[i][s] = load_run(dr, 32 * s, g);
-      const f32x8 u = widen(df[i][s]);
-      f32x8 v = widen(load_run(orow, 32 * s, g));
-      if (sizeof(T) == 2) v += widen(load_run(rest, 32 * s, g));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x = fmaf(u[j], v[j], x);
-    }
-    delta[i] = sum_groups(x);
-    if (g == 0 && qi[i] < n) a.delta[base + qi[i]] = delta[i];
-    lse[i] = n > 0 ? a.lse[base + at] : 0.0f;
-    begin[i] = begins ? begins[at] : 0;
+    for (int j = 0; j < 8; ++j) x = fmaf(u[j], v[j], x);
   }
-  const int kend = min(q0 + TILE * QW, n), kbeg = begins && q0 < n ? begins[q0] / TILE * TILE : 0;
+  const float delta = sum_groups(x), lse = n > 0 ? a.lse[base + at] : 0.0f;
+  if (g == 0 && qi < n) a.delta[base + qi] = delta;
+  const int begin = begins ? begins[at] : 0;
+  const int kend = min(q0 + TILE, n), kbeg = begins && q0 < n ? begins[q0] / TILE * TILE : 0;
   const int see_any = begins && qw < n ? begins[qw] : 0;
-  const int see_all = begins && qw < n ? begins[min(qw + 16 * QW, n) - 1] : 0;
+  const int see_all = begins && qw < n ? begins[min(qw + 16, n) - 1] : 0;
 
-  f32x4 dq[QW][D / 16];
+  f32x4 dq[D / 16];
 #pragma unroll
-  for (int i = 0; i < QW; ++i)
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) dq[i][d] = f32x4{0, 0, 0, 0};
+  for (int d = 0; d < D / 16; ++d) dq[d] = f32x4{0, 0, 0, 0};
   const auto tile = [&](int k0, bool masked) {
 #pragma unroll
     for (int c = 0; c < KT / 2; ++c) {
-      if (sizeof(T) == 4 && k0 + 32 * c > qw + 16 * QW - 1) continue;
-      f32x4 ds[QW][2];
+      if (sizeof(T) == 4 && k0 + 32 * c > qw + 15) continue;
+      f32x4 ds[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int t = 2 * c + u;
-        f32x4 s[QW], dp[QW];
-#pragma unroll
-        for (int i = 0; i < QW; ++i) s[i] = dp[i] = f32x4{0, 0, 0, 0};
+        f32x4 s = {0, 0, 0, 0}, dp = {0, 0, 0, 0};
 #pragma unroll
         for (int x = 0; x < D / 32; ++x) {
-          const Frag<T> kf = load_run(sK + (16 * t + m) * LD, 32 * x, g), vf = load_run(sV + (16 * t + m) * LD, 32 * x, g);
-#pragma unroll
-          for (int i = 0; i < QW; ++i) {
-            mma(s[i], kf, qf[i][x]);
-            mma(dp[i], vf, df[i][x]);
-          }
+          mma(s, load_run(sK + (16 * t + m) * LD, 32 * x, g), qf[x]);
+          mma(dp, load_run(sV + (16 * t + m) * LD, 32 * x, g), df[x]);
         }
-#pragma unroll
-        for (int i = 0; i < QW; ++i) {
-          f32x4 p;
-          const f32x4 l = {lse[i], lse[i], lse[i], lse[i]}, dl = {delta[i], delta[i], delta[i], delta[i]};
-          const auto on = [&](int r) {
-            const int j = k0 + 16 * t + 4 * g + r;
-            return j <= qi[i] && j >= begin[i];
-          };
-          p_and_ds<T, CAP, BIAS>(sc, (float)(qi[i] - k0 - 4 * g) - (float)(16 * t), f32x4{0, -1, -2, -3}, l, dl, s[i], dp[i], masked, on, p, ds[i][u]);
-        }
+        f32x4 p;
+        const f32x4 l = {lse, lse, lse, lse}, dl = {delta, delta, delta, delta};
+        const auto on = [&](int r) {
+          const int j = k0 + 16 * t + 4 * g + r;
+          return j <= qi && j >= begin;
+        };
+        p_and_ds<T, CAP, BIAS>(sc, (float)(qi - k0 - 4 * g) - (float)(16 * t), f32x4{0, -1, -2, -3}, l, dl, s, dp, masked, on, p, ds[u]);
       }
-      Frag<T> f[QW];
+      const Frag<T> f = round_frag<T>(join(ds[0], ds[1]));
 #pragma unroll
-      for (int i = 0; i < QW; ++i) f[i] = round_frag<T>(join(ds[i][0], ds[i][1]));
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        const Frag<T> kf = load_col(sK, LD, 32 * c, 16 * d, lane);
-#pragma unroll
-        for (int i = 0; i < QW; ++i) mma(dq[i][d], kf, f[i]);
-      }
+      for (int d = 0; d < D / 16; ++d) mma(dq[d], load_col(sK, LD, 32 * c, 16 * d, lane), f);
     }
   };
   Fetch<T, TILE, D, 256> fk, fv;
@@ -507,24 +452,21 @@ __global__ __launch_bounds__(256) void backward_q_kernel(bsg_attention a) {
       fv.load(row<T>(a.v, e, k0 + TILE, hk), a.v.step, kend - k0 - TILE, tid);
     }
     __syncthreads();
-    if (qw >= n || k0 > qw + 16 * QW - 1 || k0 + TILE <= see_any) continue;
+    if (qw >= n || k0 > qw + 15 || k0 + TILE <= see_any) continue;
     tile(k0, k0 + TILE - 1 > qw || k0 < see_all);
   }
+  if (qi >= a.steps) return;
+  const bool live = qi < n;
+  T* out = row_out<T>(a.dq, e, qi, h);
 #pragma unroll
-  for (int i = 0; i < QW; ++i) {
-    if (qi[i] >= a.steps) continue;
-    const bool live = qi[i] < n;
-    T* out = row_out<T>(a.dq, e, qi[i], h);
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) store4(out + 16 * d + 4 * g, live ? dq[i][d] * a.scale : f32x4{0, 0, 0, 0});
-  }
+  for (int d = 0; d < D / 16; ++d) store4(out + 16 * d + 4 * g, live ? dq[d] * a.scale : f32x4{0, 0, 0, 0});
 }
 
-// dk, dv: a wave holds 16 QW keys and walks the queries that see them, in tiles of 64 fetched one
+// dk, dv: a wave holds 16 keys and walks the queries that see them, in tiles of 64 fetched one
 // ahead.  A workgroup does so for every query head that shares the key's head, so that nothing is
 // added across workgroups; or, where that leaves CUs idle (`parts`), for one of them, into fp32
 // partial sums that add_parts_kernel adds.
-template <class T, int D, int QW, bool CAP, bool BIAS>
+template <class T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
   constexpr int LD = pitch<T>(D), QT = TILE / 16;
   __shared__ __align__(16) T sQ[TILE * LD];
@@ -533,32 +475,27 @@ __global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
   __shared__ __align__(16) int sBegin[TILE];
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW), id = swizzled(blockIdx.x, gridDim.x);
-  const int k0 = id % nt * TILE * QW;                            // the longest ranges first
+  const int nt = (a.steps + TILE - 1) / TILE, id = swizzled(blockIdx.x, gridDim.x);
+  const int k0 = id % nt * TILE;                            // the longest ranges first
   const int group = a.heads_q / a.heads_k, eh = id / nt;
   const bool split = a.parts != nullptr;
   const int h0 = split ? eh % a.heads_q : eh % a.heads_k * group, h1 = split ? h0 + 1 : h0 + group;
   const int hk = h0 / group, e = split ? eh / a.heads_q : eh / a.heads_k;
   const int n = a.lengths ? min(max(a.lengths[e], 0), a.steps) : a.steps;
-  const int kw = k0 + 16 * QW * w;                               // the wave's first key
+  const int kw = k0 + 16 * w;                               // the wave's first key
   const int32_t* begins = a.begins ? a.begins + (int64_t)e * a.steps : nullptr;
 
-  Frag<T> kf[QW][D / 32], vf[QW][D / 32];
-  f32x4 dk[QW][D / 16], dv[QW][D / 16];
-  int kj[QW];
+  Frag<T> kf[D / 32], vf[D / 32];
+  f32x4 dk[D / 16], dv[D / 16];
+  const int kj = kw + m, at = max(min(kj, n - 1), 0);
+  const T *kr = row<T>(a.k, e, at, hk), *vr = row<T>(a.v, e, at, hk);
 #pragma unroll
-  for (int i = 0; i < QW; ++i) {
-    kj[i] = kw + 16 * i + m;
-    const int at = max(min(kj[i], n - 1), 0);
-    const T *kr = row<T>(a.k, e, at, hk), *vr = row<T>(a.v, e, at, hk);
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      kf[i][s] = load_run(kr, 32 * s, g);
-      vf[i][s] = load_run(vr, 32 * s, g);
-    }
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) dk[i][d] = dv[i][d] = f32x4{0, 0, 0, 0};
+  for (int s = 0; s < D / 32; ++s) {
+    kf[s] = load_run(kr, 32 * s, g);
+    vf[s] = load_run(vr, 32 * s, g);
   }
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) dk[d] = dv[d] = f32x4{0, 0, 0, 0};
   // the queries that see one of the keys end with the tile where the next episode (window) has begun:
   // begins never falls, so halving finds it
   int qend = n;
@@ -566,7 +503,7 @@ __global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
     int some = 0, none = (n - k0 + TILE - 1) / TILE;             // tiles from k0 that see, that do not
     while (none - some > 1) {
       const int t = (some + none) / 2;
-      if (begins[k0 + t * TILE] > k0 + TILE * QW - 1) none = t;
+      if (begins[k0 + t * TILE] > k0 + TILE - 1) none = t;
       else some = t;
     }
     qend = min(n, k0 + none * TILE);
@@ -591,47 +528,29 @@ __global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
 #pragma unroll
       for (int c = 0; c < QT / 2; ++c) {
         if (sizeof(T) == 4 && q0 + 32 * c + 31 < kw) continue;   // before the wave's first key
-        f32x4 ps[QW][2], ds[QW][2];
+        f32x4 ps[2], ds[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int t = 2 * c + u;
-          f32x4 s[QW], dp[QW];
-#pragma unroll
-          for (int i = 0; i < QW; ++i) s[i] = dp[i] = f32x4{0, 0, 0, 0};
+          f32x4 s = {0, 0, 0, 0}, dp = {0, 0, 0, 0};
 #pragma unroll
           for (int x = 0; x < D / 32; ++x) {
-            const Frag<T> qf = load_run(sQ + (16 * t + m) * LD, 32 * x, g), df = load_run(sD + (16 * t + m) * LD, 32 * x, g);
-#pragma unroll
-            for (int i = 0; i < QW; ++i) {
-              mma(s[i], qf, kf[i][x]);
-              mma(dp[i], df, vf[i][x]);
-            }
+            mma(s, load_run(sQ + (16 * t + m) * LD, 32 * x, g), kf[x]);
+            mma(dp, load_run(sD + (16 * t + m) * LD, 32 * x, g), vf[x]);
           }
           const f32x4 lse = *reinterpret_cast<const f32x4*>(&sLse[16 * t + 4 * g]);
           const f32x4 delta = *reinterpret_cast<const f32x4*>(&sDelta[16 * t + 4 * g]);
-#pragma unroll
-          for (int i = 0; i < QW; ++i) {
-            const auto on = [&](int r) {
-              const int l = 16 * t + 4 * g + r;
-              return kj[i] <= q0 + l && kj[i] >= sBegin[l];
-            };
-            p_and_ds<T, CAP, BIAS>(sc, (float)(q0 + 4 * g - kj[i]) + (float)(16 * t), f32x4{0, 1, 2, 3}, lse, delta, s[i], dp[i], masked, on, ps[i][u], ds[i][u]);
-          }
+          const auto on = [&](int r) {
+            const int l = 16 * t + 4 * g + r;
+            return kj <= q0 + l && kj >= sBegin[l];
+          };
+          p_and_ds<T, CAP, BIAS>(sc, (float)(q0 + 4 * g - kj) + (float)(16 * t), f32x4{0, 1, 2, 3}, lse, delta, s, dp, masked, on, ps[u], ds[u]);
         }
-        Frag<T> pf[QW], f[QW];
-#pragma unroll
-        for (int i = 0; i < QW; ++i) {
-          pf[i] = round_frag<T>(join(ps[i][0], ps[i][1]));
-          f[i] = round_frag<T>(join(ds[i][0], ds[i][1]));
-        }
+        const Frag<T> pf = round_frag<T>(join(ps[0], ps[1])), f = round_frag<T>(join(ds[0], ds[1]));
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-          const Frag<T> dc = load_col(sD, LD, 32 * c, 16 * d, lane), qc = load_col(sQ, LD, 32 * c, 16 * d, lane);
-#pragma unroll
-          for (int i = 0; i < QW; ++i) {
-            mma(dv[i][d], dc, pf[i]);
-            mma(dk[i][d], qc, f[i]);
-          }
+          mma(dv[d], load_col(sD, LD, 32 * c, 16 * d, lane), pf);
+          mma(dk[d], load_col(sQ, LD, 32 * c, 16 * d, lane), f);
         }
       }
     };
@@ -648,29 +567,26 @@ __global__ __launch_bounds__(256) void backward_kv_kernel(bsg_attention a) {
       if (q0 + TILE < qend) fetch(h, q0 + TILE);
       else if (h + 1 < h1) fetch(h + 1, k0);
       __syncthreads();
-      if (kw >= n || q0 + TILE - 1 < kw || sBegin[0] > kw + 16 * QW - 1) continue;
+      if (kw >= n || q0 + TILE - 1 < kw || sBegin[0] > kw + 15) continue;
       // unless every query of the tile sees every key of the wave
-      tile(q0, kw + 16 * QW - 1 > q0 || sBegin[TILE - 1] > kw);
+      tile(q0, kw + 15 > q0 || sBegin[TILE - 1] > kw);
     }
   }
+  if (kj >= a.steps) return;
+  const bool live = kj < n;
+  if (split) {
+    float* to = a.parts + (((int64_t)e * a.heads_q + h0) * a.steps + kj) * 2 * D;
 #pragma unroll
-  for (int i = 0; i < QW; ++i) {
-    if (kj[i] >= a.steps) continue;
-    const bool live = kj[i] < n;
-    if (split) {
-      float* to = a.parts + (((int64_t)e * a.heads_q + h0) * a.steps + kj[i]) * 2 * D;
+    for (int d = 0; d < D / 16; ++d) {
+      store4(to + 16 * d + 4 * g, live ? dk[d] * a.scale : f32x4{0, 0, 0, 0});
+      store4(to + D + 16 * d + 4 * g, live ? dv[d] : f32x4{0, 0, 0, 0});
+    }
+  } else {
+    T *ok = row_out<T>(a.dk, e, kj, hk), *ov = row_out<T>(a.dv, e, kj, hk);
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        store4(to + 16 * d + 4 * g, live ? dk[i][d] * a.scale : f32x4{0, 0, 0, 0});
-        store4(to + D + 16 * d + 4 * g, live ? dv[i][d] : f32x4{0, 0, 0, 0});
-      }
-    } else {
-      T *ok = row_out<T>(a.dk, e, kj[i], hk), *ov = row_out<T>(a.dv, e, kj[i], hk);
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        store4(ok + 16 * d + 4 * g, live ? dk[i][d] * a.scale : f32x4{0, 0, 0, 0});
-        store4(ov + 16 * d + 4 * g, live ? dv[i][d] : f32x4{0, 0, 0, 0});
-      }
+    for (int d = 0; d < D / 16; ++d) {
+      store4(ok + 16 * d + 4 * g, live ? dk[d] * a.scale : f32x4{0, 0, 0, 0});
+      store4(ov + 16 * d + 4 * g, live ? dv[d] : f32x4{0, 0, 0, 0});
     }
   }
 }
@@ -1038,28 +954,24 @@ hipError_t act(const bsg_attention_act& a, hipStream_t st) {
   return cap ? act<T, D, 1, true>(a, p, st) : act<T, D, 1, false>(a, p, st);
 }
 
-// Queries (keys) per wave: 32 for bf16 rollouts of more than one tile, else 16.
-template <class T> bool two_tiles(const bsg_attention& a) { return sizeof(T) == 2 && a.steps > 512; }
-
-template <class T, int D, int QW, bool CAP, bool BIAS>
+template <class T, int D, bool CAP, bool BIAS>
 hipError_t forward(const bsg_attention& a, hipStream_t st) {
-  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW);
+  const int nt = (a.steps + TILE - 1) / TILE;
   if (a.begins)
     begins_kernel<<<dim3(a.num_envs), dim3(256), 0, st>>>(a.first, a.first_env, a.first_step, a.steps, a.window, a.begins);
-  forward_kernel<T, D, QW, CAP, BIAS><<<dim3(a.num_envs * a.heads_q * nt), dim3(256), 0, st>>>(a);
+  forward_kernel<T, D, CAP, BIAS><<<dim3(a.num_envs * a.heads_q * nt), dim3(256), 0, st>>>(a);
   return hipGetLastError();
 }
-template <class T, int D, int QW, bool CAP, bool BIAS>
+template <class T, int D, bool CAP, bool BIAS>
 hipError_t backward(const bsg_attention& a, hipStream_t st) {
   if (a.steps <= TILE) {
     backward_short_kernel<T, D, CAP, BIAS><<<dim3(a.num_envs * a.heads_k), dim3(256), 0, st>>>(a);
     return hipGetLastError();
   }
-  const int nt = (a.steps + TILE * QW - 1) / (TILE * QW);
-  backward_q_kernel<T, D, QW, CAP, BIAS><<<dim3(a.num_envs * a.heads_q * nt), dim3(256), 0, st>>>(a);
-  constexpr int KW = D == 128 ? 1 : QW;
-  const int heads = a.parts ? a.heads_q : a.heads_k, kt = (a.steps + TILE * KW - 1) / (TILE * KW);
-  backward_kv_kernel<T, D, KW, CAP, BIAS><<<dim3(a.num_envs * heads * kt), dim3(256), 0, st>>>(a);
+  const int nt = (a.steps + TILE - 1) / TILE;
+  backward_q_kernel<T, D, CAP, BIAS><<<dim3(a.num_envs * a.heads_q * nt), dim3(256), 0, st>>>(a);
+  const int heads = a.parts ? a.heads_q : a.heads_k;
+  backward_kv_kernel<T, D, CAP, BIAS><<<dim3(a.num_envs * heads * nt), dim3(256), 0, st>>>(a);
   if (a.parts) {
     const int64_t all = (int64_t)a.num_envs * a.heads_k * a.steps * (D / 2);
     add_parts_kernel<T, D><<<dim3((unsigned)((all + 255) / 256)), dim3(256), 0, st>>>(a, all);
@@ -1068,9 +980,7 @@ hipError_t backward(const bsg_attention& a, hipStream_t st) {
 }
 template <class T, int D, bool CAP, bool BIAS>
 hipError_t learn(const bsg_attention& a, bool back, hipStream_t st) {
-  if constexpr (sizeof(T) == 2)
-    if (two_tiles<T>(a)) return back ? backward<T, D, 2, CAP, BIAS>(a, st) : forward<T, D, 2, CAP, BIAS>(a, st);
-  return back ? backward<T, D, 1, CAP, BIAS>(a, st) : forward<T, D, 1, CAP, BIAS>(a, st);
+  return back ? backward<T, D, CAP, BIAS>(a, st) : forward<T, D, CAP, BIAS>(a, st);
 }
 template <class T, int D>
 hipError_t learn(const bsg_attention& a, bool back, hipStream_t st) {
@@ -1100,8 +1010,7 @@ hipError_t launch_attention_step(const bsg_attention_act& a, hipStream_t st) {
 // Parts by query head are wanted where key tiles alone give fewer than four workgroups to a CU.
 bool attention_wants_parts(const bsg_attention& a) {
   if (a.heads_q == a.heads_k || a.steps <= TILE) return false;
-  const int rows = a.dtype == BSG_BF16 && two_tiles<mma::bf16>(a) ? 2 * TILE : TILE;
-  return (int64_t)a.num_envs * a.heads_k * ((a.steps + rows - 1) / rows) < 1024;
+  return (int64_t)a.num_envs * a.heads_k * ((a.steps + TILE - 1) / TILE) < 1024;
 }
 int64_t attention_step_bytes(const bsg_attention_act& a) {
   const Plan p = plan_of(a);

@@ -423,6 +423,7 @@ int32_t bsg_delta_step(const bsg_delta_act* a, void* stream);
  * over j <= i of the same episode, and i - j < window if window > 0.  Key/value head h serves
  * the query heads h r .. h r + r - 1, r = heads_q / heads_k.  dim: 32, 64 or 128; num_envs x heads_q x
  * tiles of 64 steps below 2^24. */
+#define BSG_ATTENTION_TILE 64
 typedef struct bsg_attention {
   int32_t num_envs, steps;
   int32_t heads_q, heads_k, dim;
@@ -441,7 +442,7 @@ typedef struct bsg_attention {
   /* kept by the forward pass for the backward pass (NULL: not kept) */
   float* lse;                /* [num_envs][heads_q][steps] */
   void* out_rest;            /* [num_envs][heads_q][steps][dim] dtype: what rounding left of out; read
-                                and wanted for BSG_BF16 and more than 64 steps only */
+                                and wanted for BSG_BF16 and more than BSG_ATTENTION_TILE steps only */
   /* backward only (out as the forward pass wrote it) */
   bsg_rows dout, dq, dk, dv;
   float* delta;              /* [num_envs][heads_q][steps] scratch */

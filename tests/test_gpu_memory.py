@@ -278,7 +278,7 @@ ATTEND = [  # E, T, H, Hk, D, dtype, first, lengths, order, softcap, bias, windo
     (1, 321, 4, 1, 128, "bf16", None, None, "odd", 0.0, True, 0, 3.0),
     (1, 300, 2, 2, 64, "fp32", "0.004", None, "te", 30.0, True, 200, 4.0),
     (5, 70, 5, 5, 32, "bf16", None, "ragged", "et", 0.0, False, 0, 8.0),
-    # two tiles of queries to a wave; one key head of many envs, without partial sums
+    # long rollouts; one key head of many envs, without partial sums
     (1, 600, 2, 1, 64, "bf16", "0.005", None, "te", 15.0, True, 0, 2.0),
     (2, 577, 2, 2, 128, "bf16", None, "ragged", "te", 0.0, False, 0, 2.0),
     (2, 530, 3, 1, 32, "bf16", "0.02", "ragged", "gap", 0.0, True, 100, 1.0),
