@@ -38,8 +38,7 @@ namespace {
 using namespace bsg::mma;
 
 constexpr int C = BSG_DELTA_CHUNK;
-constexpr int AP = C + 4;          // row pitch of the C x C matrices in LDS
-constexpr int IP = 20;             // ... of the 16 x 16 inverses
+constexpr int IP = 20;             // row pitch of a 16 x 16 tile of fp32 in LDS
 constexpr float LOWEST = -1e5f;    // the least log decay: its exponential is 0
 __device__ __forceinline__ float at_least_lowest(float g) { return g < LOWEST ? LOWEST : g; }   // NaN stays
 
@@ -153,14 +152,21 @@ __device__ __forceinline__ f32x4 decays(const Gates& s, int row, const Step& o) 
   return f;
 }
 
-// What the passes along a rollout need of a chunk besides its rows.
-template <class T>
+// The passes along a rollout.  ALONE solves each chunk where it needs it.  Where the chunks are solved
+// beforehand, CARRY takes each segment of the rollout to its transition and JOINED runs all segments side
+// by side, each from the state that the joined transitions give it.
+enum Pass { ALONE, JOINED, CARRY };
+
+// What the passes along a rollout need of a chunk besides its rows (ALL: with P; HERE: solved in place).
+template <class T, bool ALL, bool HERE>
 struct Solved {
   static constexpr int PD = pitch<T>(C), parts = Parts<T, 2>::n;
-  T p[parts][C * PD];              // P in parts of type T, zeros above its diagonal
-  float n[C * AP];                 // minus the matrix of the system, below the diagonal
-  float inv[4 * 16 * IP];          // inverses of the system's diagonal blocks
-  Gates gates[2];                  // of this chunk and the one that comes next
+  T p[ALL ? parts : 1][ALL ? C * PD : Vec<T>::n];   // P in parts of type T, zeros above its diagonal
+  float n[6 * 16 * IP];            // minus the matrix of the system: the tiles below the diagonal,
+  float inv[4 * 16 * IP];          // ... the inverses of those on it,
+  Gates gates[HERE ? 2 : 1];       // (of this chunk and the one that comes next)
+  float diagonal[HERE ? 4 * 16 * IP : 4];   // ... and those themselves
+  static constexpr int tile(int b, int u) { return (b * (b - 1) / 2 + u) * 16 * IP; }
   __device__ __forceinline__ WideOf<T, 2> p_row(int r, int k0, int g) const {
     WideOf<T, 2> w;
 #pragma unroll
@@ -174,18 +180,19 @@ struct Solved {
     return w;
   }
 };
-// ... of which all but the second gates pass through memory where the chunks are solved beforehand.
-template <class T> constexpr int solved_bytes() { return sizeof(Solved<T>) - sizeof(Gates); }
+// ... which passes through memory up to the first gates where the chunks are solved beforehand.
+template <class T> constexpr int solved_bytes() { return sizeof(Solved<T, true, false>) - 16; }
+template <class T> constexpr int p_bytes() { return sizeof(Solved<T, true, false>::p); }
 
 // A workgroup of NW waves handles 16 NW value columns of one env and value head; wave w owns 16 of
 // them and keeps their part of the state in registers (as D tiles, whose rows are the key
 // dimension), so the waves only meet over the C x C matrices.
-template <class T, int DK, int NW>
+template <class T, int DK, int NW, bool HERE = true, bool Q = true, bool V = sizeof(T) == 2>
 struct Chunk {
   static constexpr int LD = pitch<T>(DK), VD = pitch<T>(16 * NW);
-  T k[C * LD], q[C * LD];
-  T v[sizeof(T) == 2 ? C * VD : 4];  // bf16: v (dout), then, column by column, out (v')
-  Solved<T> s;
+  T k[C * LD], q[Q ? C * LD : Vec<T>::n];
+  T v[V ? C * VD : Vec<T>::n];       // v (dout), then, column by column, out (v')
+  Solved<T, Q, HERE> s;
 };
 // Waves per SIMD that LDS leaves room for, two at most: what bounds the passes' registers.
 template <class T, int DK, int NW> constexpr int waves_per_simd() {
@@ -195,7 +202,7 @@ template <class T, int DK, int NW> constexpr int waves_per_simd() {
 // A wave's 16 columns of the value rows, as D tiles.  bf16 passes through LDS, so that memory sees 16
 // bytes a lane, in and out; fp32, where 16 lanes make 64 bytes of a row, goes straight to and from
 // registers, and the LDS that saves lets two workgroups share a CU.
-template <class T, int NW>
+template <class T, int NW, bool LDS>
 struct Columns {
   static constexpr int NT = 64 * NW, VD = pitch<T>(16 * NW);
   Fetch<T, C, 16 * NW, NT> f;
@@ -226,35 +233,35 @@ struct Columns {
     }
   }
 };
-template <int NW>
-struct Columns<float, NW> {
+template <class T, int NW>
+struct Columns<T, NW, false> {
   f32x4 next[4], now[4];
-  __device__ __forceinline__ void load(const float* p, int64_t stride, int rows, int tid, int col) {
+  __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int tid, int col) {
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) next[b][r] = p[min(16 * b + 4 * (tid % 64 >> 4) + r, rows - 1) * stride + col];
+      for (int r = 0; r < 4; ++r) next[b][r] = (float)p[min(16 * b + 4 * (tid % 64 >> 4) + r, rows - 1) * stride + col];
   }
-  __device__ __forceinline__ void store(float*, int, int) {
+  __device__ __forceinline__ void store(T*, int, int) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) now[b] = next[b];
   }
-  __device__ __forceinline__ void get(f32x4 (&x)[4], const float*, int rows, int, int lane) const {
+  __device__ __forceinline__ void get(f32x4 (&x)[4], const T*, int rows, int, int lane) const {
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[b][r] = 16 * b + 4 * (lane >> 4) + r < rows ? now[b][r] : 0.0f;
   }
-  static __device__ __forceinline__ void put(float*, const f32x4 (&x)[4], float* to, int64_t stride, int rows, int all, int w, int lane) {
+  static __device__ __forceinline__ void put(T*, const f32x4 (&x)[4], T* to, int64_t stride, int rows, int all, int w, int lane) {
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int t = 16 * b + 4 * (lane >> 4) + r;
-        if (t < all) to[t * stride + 16 * w + (lane & 15)] = t < rows ? x[b][r] : 0.0f;
+        if (t < all) to[t * stride + 16 * w + (lane & 15)] = (T)(t < rows ? x[b][r] : 0.0f);
       }
   }
-  static __device__ __forceinline__ void write(const float*, float*, int64_t, int, int, int, int) {}
+  static __device__ __forceinline__ void write(const T*, T*, int64_t, int, int, int, int) {}
 };
 
 // lane j of each row of 16 lanes, to all of them
@@ -275,10 +282,10 @@ template <int J, int N> __device__ __forceinline__ void eliminate(float (&x)[N],
 // columns of each to a wave, a row to a lane; the substitution takes the rows before from their lanes
 // (by one wave alone it held the others up: 102 against 89 us, 512x50 fp32).  The inverses are there after the caller's next barrier.
 // BACK: the system is (I + diag(beta) N)^T, else I + N diag(beta).
-template <class T, int DK, int NW, bool BACK>
-__device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& x, const Gates& gates, float scale, int lane, int w) {
-  constexpr int LD = pitch<T>(DK);
-  Solved<T>& s = x.s;
+template <class T, int DK, int NW, bool BACK, class X>
+__device__ __forceinline__ void solve_chunk(X& x, const Gates& gates, float scale, int lane, int w) {
+  constexpr int LD = pitch<T>(DK), PD = pitch<T>(C);
+  auto& s = x.s;
   const int m = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t0 = 0; t0 < 10; t0 += NW) {
@@ -294,15 +301,16 @@ __device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& x, const Gates& ga
     const float bj = gates.beta[j];
     const f32x4 bi = *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);
     const f32x4 f = decays<false>(gates, 16 * b + 4 * g, step_of(gates, j));
+    float* n = (b == u ? s.diagonal + 16 * IP * b : s.n + s.tile(b, u)) + 4 * g * IP + m;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * b + 4 * g + r;
-      s.n[i * AP + j] = j < i ? -(BACK ? bi[r] : bj) * f[r] * kk[r] : 0.0f;
+      n[r * IP] = j < i ? -(BACK ? bi[r] : bj) * f[r] * kk[r] : 0.0f;
       float y = j <= i ? scale * f[r] * qk[r] : 0.0f;
 #pragma unroll
       for (int o = 0; o < Parts<T, 2>::n; ++o) {
         const T z = (T)y;
-        s.p[o][i * Solved<T>::PD + j] = z;
+        s.p[o][i * PD + j] = z;
         y -= (float)z;
       }
     }
@@ -313,7 +321,7 @@ __device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& x, const Gates& ga
   float v[N], n[16];               // lane: block g, row m
 #pragma unroll
   for (int j = 0; j < 16; j += 4) {
-    const f32x4 y = *reinterpret_cast<const f32x4*>(&s.n[(16 * g + m) * AP + 16 * g + j]);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(&s.diagonal[(16 * g + m) * IP + j]);
 #pragma unroll
     for (int o = 0; o < 4; ++o) n[j + o] = y[o];
   }
@@ -325,18 +333,18 @@ __device__ __forceinline__ void solve_chunk(Chunk<T, DK, NW>& x, const Gates& ga
 }
 // P's tiles above the diagonal that share a product step with one on it
 template <class T>
-__device__ __forceinline__ void clear_above(Solved<T>& s, int tid, int nt) {
+__device__ __forceinline__ void clear_above(Solved<T, true, true>& s, int tid, int nt) {
   for (int i = tid; i < 2 * 256; i += nt) {
     const int b = i / 256 * 32, r = i % 256 / 16, c = i % 16;
 #pragma unroll
-    for (int o = 0; o < Solved<T>::parts; ++o) s.p[o][(b + r) * Solved<T>::PD + b + 16 + c] = (T)0.0f;
+    for (int o = 0; o < s.parts; ++o) s.p[o][(b + r) * s.PD + b + 16 + c] = (T)0.0f;
   }
 }
 
 // Few rows: the chunks are solved beforehand, all side by side, by workgroups of four waves.
 template <class T, int DK, bool BACK>
 __global__ __launch_bounds__(256) void solve_kernel(bsg_delta a) {
-  __shared__ __align__(16) Chunk<T, DK, 4> s;
+  __shared__ __align__(16) Chunk<T, DK, 4, true, true, false> s;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int chunks = (a.steps + C - 1) / C, ch = blockIdx.x % chunks, eh = blockIdx.x / chunks;
   const int h = eh % a.heads_v, e = eh / a.heads_v, hk = h / (a.heads_v / a.heads_k);
@@ -362,18 +370,18 @@ __global__ __launch_bounds__(256) void solve_kernel(bsg_delta a) {
   for (int i = tid; i < N; i += 256) to[i] = from[i];
 }
 // ... and their results fetched a chunk ahead, as the rows are.
-template <class T, int NT>
+template <class T, int NT, bool ALL>
 struct FetchSolved {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  static constexpr int N = solved_bytes<T>() / 16, n = (N + NT - 1) / NT;
+  static constexpr int skip = ALL ? 0 : p_bytes<T>() / 16, N = solved_bytes<T>() / 16 - skip, n = (N + NT - 1) / NT;
   u32x4 x[n];
   __device__ __forceinline__ void load(const void* work, int64_t chunk, int tid) {
-    const u32x4* p = reinterpret_cast<const u32x4*>(work) + chunk * N;
+    const u32x4* p = reinterpret_cast<const u32x4*>(work) + chunk * (N + skip) + skip;
 #pragma unroll
     for (int i = 0; i < n; ++i) x[i] = p[min(tid + i * NT, N - 1)];
   }
-  __device__ __forceinline__ void store(Solved<T>& s, int tid) const {
-    u32x4* p = reinterpret_cast<u32x4*>(&s);
+  __device__ __forceinline__ void store(Solved<T, ALL, false>& s, int tid) const {
+    u32x4* p = reinterpret_cast<u32x4*>(ALL ? (void*)&s : (void*)s.n);
 #pragma unroll
     for (int i = 0; i < n; ++i)
       if (tid + i * NT < N) p[tid + i * NT] = x[i];
@@ -389,51 +397,138 @@ __device__ __forceinline__ float* tiles(float* p, int64_t chunk, int waves, int 
   return p + ((chunk * waves + w) * tiles_per_wave * 64 + lane) * 4;
 }
 
-// ---- forward -------------------------------------------------------------------------------
-template <class T, int DK, int NW, bool SOLVED>
-__global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())) void forward_kernel(bsg_delta a) {
-  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW;
-  constexpr bool AHEAD = SOLVED || sizeof(T) == 2;   // fp32 rows a chunk ahead would cost spilled registers
-  __shared__ __align__(16) Chunk<T, DK, NW> s;
+// A rollout in segments of whole chunks.  What a segment does to the state before it is affine: with
+// the products of its chunks' transitions A[dim_k][dim_k] (the pass run on the unit matrix, without
+// values) and what it makes of no state, B[dim_k][dim_v], S' = A S + B.  `carry` holds, per row (env and
+// value head) and boundary of segments, B by D tiles and A by rows; join_kernel puts the state at the
+// boundary in B's place.
+struct Segments {
+  float* carry;
+  int count, chunks;               // segments to a rollout, chunks to a segment
+};
+__device__ __forceinline__ float* boundary(const Segments& seg, int64_t row, int at, int dk, int dv) {
+  return seg.carry + (row * (seg.count - 1) + at) * dk * (dk + dv);
+}
+
+template <int DT>
+__device__ __forceinline__ void put_carry(float* to, const f32x4 (&x)[DT], bool unit, int all, int c0, int w, int lane) {
+  const int col = c0 + 16 * w + (lane & 15);
+  if (!unit) {
+    float* p = tiles(to, 0, 1, DT, c0 / 16 + w, lane);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p + 256 * d) = x[d];
+  } else if (col < 16 * DT) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) to[16 * DT * all + (16 * d + 4 * (lane >> 4) + r) * 16 * DT + col] = x[d][r];
+  }
+}
+// S' = A S + B from boundary to boundary (BACK: from the last one to the first).  A workgroup holds 16
+// columns; a wave computes 16 rows of each product, and the waves meet in LDS after it.
+template <int DK, bool BACK>
+__global__ __launch_bounds__(4 * DK) void join_kernel(bsg_delta a, Segments seg) {
+  constexpr int DT = DK / 16;
+  __shared__ f32x4 sS[2][DT][64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
-  // the workgroup's columns of all: all of them, but where the chunks are solved beforehand
-  const int all = SOLVED ? a.dim_v : DV, groups = all / DV, id = blockIdx.x / groups, c0 = blockIdx.x % groups * DV;
-  const int h = id % a.heads_v, e = id / a.heads_v, hk = h / (a.heads_v / a.heads_k);
-  const int n = steps_of(a, e), col = 16 * w + m;
-  const int chunks = (a.steps + C - 1) / C, live = (n + C - 1) / C;
-  const int64_t eh = (int64_t)e * a.heads_v + h;
+  const int all = a.dim_v, c0 = blockIdx.x % (all / 16) * 16, eh = blockIdx.x / (all / 16);
+  const int live = (steps_of(a, eh / a.heads_v) + C - 1) / C;
+  const int boundaries = (live + seg.chunks - 1) / seg.chunks - 1;
+  if (boundaries <= 0) return;
+  const float* start = BACK ? a.dfinal : a.state;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    sS[0][w][lane][r] = start ? start[((int64_t)eh * DK + 16 * w + 4 * g + r) * all + c0 + m] : 0.0f;
+  struct Step {
+    f32x4 a[DT], x;
+  } even, odd;                     // of a boundary, loaded while the one before it is computed
+  const auto at = [&](int i) { return boundary(seg, eh, BACK ? boundaries - 1 - i : i, DK, all); };
+  const auto load = [&](Step& o, int i) {
+    float* p = at(i);
+    o.x = *reinterpret_cast<const f32x4*>(tiles(p, 0, 1, DT, c0 / 16, lane) + 256 * w);
+#pragma unroll
+    for (int u = 0; u < DT; ++u) o.a[u] = *reinterpret_cast<const f32x4*>(p + DK * all + (16 * w + m) * DK + 16 * u + 4 * g);
+  };
+  const auto step = [&](Step& o, Step& next, int i) {
+    if (i + 1 < boundaries) load(next, i + 1);
+    f32x4 y = {0, 0, 0, 0};        // two sums, so that products do not wait for each other
+#pragma unroll
+    for (int u = 0; u < DT; u += 2) {
+      mma16(o.x, o.a[u], sS[i & 1][u][lane]);
+      mma16(y, o.a[u + 1], sS[i & 1][u + 1][lane]);
+    }
+    o.x += y;
+    *reinterpret_cast<f32x4*>(tiles(at(i), 0, 1, DT, c0 / 16, lane) + 256 * w) = o.x;
+    sS[~i & 1][w][lane] = o.x;
+    __syncthreads();
+  };
+  load(even, 0);
+  __syncthreads();
+  for (int i = 0; i < boundaries; i += 2) {
+    step(even, odd, i);
+    if (i + 1 < boundaries) step(odd, even, i + 1);
+  }
+}
+
+// ---- forward -------------------------------------------------------------------------------
+template <class T, int DK, int NW, Pass PASS>
+__global__ __launch_bounds__(64 * NW, (PASS == ALONE ? waves_per_simd<T, DK, NW>() : PASS == CARRY && sizeof(T) == 2 ? 2 : 1)) void forward_kernel(bsg_delta a, Segments seg) {
+  constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW;
+  constexpr bool AHEAD = PASS != ALONE || sizeof(T) == 2;   // fp32 rows a chunk ahead would cost spilled registers
+  constexpr bool OUT = PASS != CARRY, LDS = sizeof(T) == 2;
+  __shared__ __align__(16) Chunk<T, DK, NW, PASS == ALONE, OUT, LDS> s;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
+  // the workgroup's columns of all (CARRY: and of the unit matrix's, behind them) and its segment
+  const int all = PASS == ALONE ? DV : a.dim_v, groups = all / DV + (OUT ? 0 : (DK + DV - 1) / DV);
+  const int segments = PASS == ALONE ? 1 : OUT ? seg.count : seg.count - 1, id = blockIdx.x / groups, part = id % segments;
+  const int eh = id / segments, h = eh % a.heads_v, e = eh / a.heads_v, hk = h / (a.heads_v / a.heads_k);
+  const bool unit = !OUT && (int)(blockIdx.x % groups) >= all / DV;
+  const int c0 = (int)(blockIdx.x % groups) * DV - (unit ? all : 0), col = 16 * w + m;
+  const int n = steps_of(a, e), chunks = (a.steps + C - 1) / C, live = (n + C - 1) / C;
+  const int at = part;              // the segment
+  const int begin = PASS == ALONE ? 0 : at * seg.chunks, end = PASS == ALONE ? live : min(begin + seg.chunks, live);
+  if (!OUT && (part + 1) * seg.chunks >= live) return;   // no boundary before the rollout's end
 
   f32x4 S[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      S[d][r] = a.state ? a.state[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] : 0.0f;
+      S[d][r] = !OUT ? unit && 16 * d + 4 * g + r == c0 + col ? 1.0f : 0.0f
+                     : at == 0 && a.state ? a.state[((int64_t)eh * DK + 16 * d + 4 * g + r) * all + c0 + col] : 0.0f;
+  if (PASS == JOINED && at > 0 && begin < end) {
+    const float* p = tiles(boundary(seg, eh, at - 1, DK, all), 0, 1, DT, c0 / 16 + w, lane);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) S[d] = *reinterpret_cast<const f32x4*>(p + 256 * d);
+  }
 
   Fetch<T, C, DK, NT> fk, fq;
-  Columns<T, NW> fv;
-  FetchSolved<T, NT> fs;
+  Columns<T, NW, LDS> fv;
+  FetchSolved<T, NT, OUT> fs;
   RawGates raw = {0, 0, 0};
-  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), v = steps_in<const T>(a.v, e, h, c0);
+  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), v = steps_in<const T>(a.v, e, h, unit ? 0 : c0);
   const Steps<T> out = steps_in<T>(a.out, e, h, c0);
   const GateSteps gate(a, e, h);
-  float *const ks = a.kept_states ? tiles(a.kept_states, eh * chunks, all / 16, DT, c0 / 16 + w, lane) : nullptr;
-  float *const kw = a.kept_w ? tiles(a.kept_w, eh * chunks, all / 16, 4, c0 / 16 + w, lane) : nullptr;
-  if (live > 0) {
+  float *const ks = OUT && a.kept_states ? tiles(a.kept_states, (int64_t)eh * chunks, all / 16, DT, c0 / 16 + w, lane) : nullptr;
+  float *const kw = OUT && a.kept_w ? tiles(a.kept_w, (int64_t)eh * chunks, all / 16, 4, c0 / 16 + w, lane) : nullptr;
+  if (begin < end) {
+    const int t0 = begin * C;
     if (AHEAD) {
-      fk.load(k.p, k.step, n, tid);
-      fq.load(q.p, q.step, n, tid);
-      fv.load(v.p, v.step, n, tid, col);
+      fk.load(k.at(t0), k.step, n - t0, tid);
+      if (OUT) fq.load(q.at(t0), q.step, n - t0, tid);
+      if (!unit) fv.load(v.at(t0), v.step, n - t0, tid, col);
     }
-    if (SOLVED) fs.load(a.work, eh * chunks, tid);
-    else {
+    if constexpr (PASS != ALONE) {
+      fs.load(a.work, (int64_t)eh * chunks + begin, tid);
+    } else {
       if (w == 0) make_gates(s.s.gates[0], load_gates(gate, 0, n, lane), gate.half, lane);
       clear_above(s.s, tid, NT);
     }
   }
-  for (int ch = 0; ch < live; ++ch) {
+  for (int ch = begin; ch < end; ++ch) {
     const int t0 = ch * C, rows = min(C, n - t0), t1 = t0 + C;
-    const Gates& gates = s.s.gates[SOLVED ? 0 : ch & 1];
+    const bool more = ch + 1 < end;
+    const Gates& gates = s.s.gates[PASS == ALONE ? ch & 1 : 0];
     if (!AHEAD) {
       fk.load(k.at(t0), k.step, rows, tid);
       fq.load(q.at(t0), q.step, rows, tid);
@@ -441,20 +536,20 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
     }
     __syncthreads();               // the chunk before is done with LDS
     fk.store(s.k, rows, tid);
-    fq.store(s.q, rows, tid);
-    fv.store(s.v, rows, tid);
-    if (SOLVED) fs.store(s.s, tid);
-    if (t1 < n) {
+    if (OUT) fq.store(s.q, rows, tid);
+    if (!unit) fv.store(s.v, rows, tid);
+    if constexpr (PASS != ALONE) fs.store(s.s, tid);
+    if (more) {
       if (AHEAD) {
         fk.load(k.at(t1), k.step, n - t1, tid);
-        fq.load(q.at(t1), q.step, n - t1, tid);
-        fv.load(v.at(t1), v.step, n - t1, tid, col);
+        if (OUT) fq.load(q.at(t1), q.step, n - t1, tid);
+        if (!unit) fv.load(v.at(t1), v.step, n - t1, tid, col);
       }
-      if (SOLVED) fs.load(a.work, eh * chunks + ch + 1, tid);
+      if (PASS != ALONE) fs.load(a.work, (int64_t)eh * chunks + ch + 1, tid);
       else if (w == 0) raw = load_gates(gate, t1, n - t1, lane);
     }
     __syncthreads();
-    if (!SOLVED) solve_chunk<T, DK, NW, false>(s, gates, a.scale, lane, w);
+    if constexpr (PASS == ALONE) solve_chunk<T, DK, NW, false>(s, gates, a.scale, lane, w);
 
     if (ks) {
 #pragma unroll
@@ -472,21 +567,21 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         kf[b] = load_tile(s.k + (16 * b + m) * LD, 32 * c, g);
-        qf[b] = load_tile(s.q + (16 * b + m) * LD, 32 * c, g);
+        if (OUT) qf[b] = load_tile(s.q + (16 * b + m) * LD, 32 * c, g);
       }
       mma_all<T>(x, kf, sw);
-      mma_all<T>(o, qf, front(sw));
+      if (OUT) mma_all<T>(o, qf, front(sw));
     }
-    f32x4 vs[4];
-    fv.get(vs, s.v, rows, w, lane);
+    f32x4 vs[4] = {};
+    if (!unit) fv.get(vs, s.v, rows, w, lane);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const f32x4 in = *reinterpret_cast<const f32x4*>(&gates.in[16 * b + 4 * g]);
       x[b] = vs[b] - in * x[b];
       o[b] *= in * a.scale;
     }
-    if (!SOLVED) {
-      if (w == 0 && t1 < n) make_gates(s.s.gates[(ch + 1) & 1], raw, gate.half, lane);
+    if (PASS == ALONE) {
+      if (w == 0 && more) make_gates(s.s.gates[(ch + 1) & 1], raw, gate.half, lane);
       __syncthreads();             // the inverses are there
     }
     f32x4 W[4];
@@ -494,7 +589,7 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
     for (int b = 0; b < 4; ++b) {
 #pragma unroll
       for (int u = 0; u < b; ++u)
-        mma16(x[b], *reinterpret_cast<const f32x4*>(&s.s.n[(16 * b + m) * AP + 16 * u + 4 * g]), W[u]);
+        mma16(x[b], *reinterpret_cast<const f32x4*>(&s.s.n[s.s.tile(b, u) + m * IP + 4 * g]), W[u]);
       W[b] = f32x4{0, 0, 0, 0};
       mma16(W[b], *reinterpret_cast<const f32x4*>(&s.s.inv[(16 * b + m) * IP + 4 * g]), x[b]);
     }
@@ -504,14 +599,16 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) W[b] *= *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);   // U
+    if constexpr (OUT) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      WideOf<T, 2> uw;
-      split(uw, join(W[2 * c], W[2 * c + 1]));
+      for (int c = 0; c < 2; ++c) {
+        WideOf<T, 2> uw;
+        split(uw, join(W[2 * c], W[2 * c + 1]));
 #pragma unroll
-      for (int b = 2 * c; b < 4; ++b) mma<T>(o[b], s.s.p_row(16 * b + m, 32 * c, g), uw);
+        for (int b = 2 * c; b < 4; ++b) mma<T>(o[b], s.s.p_row(16 * b + m, 32 * c, g), uw);
+      }
     }
-    fv.put(s.v, o, out.at(t0), out.step, rows, min(C, a.steps - t0), w, lane);
+    if (OUT) fv.put(s.v, o, out.at(t0), out.step, rows, min(C, a.steps - t0), w, lane);
 #pragma unroll
     for (int d = 0; d < DT; ++d) S[d] *= gates.across;
 #pragma unroll
@@ -526,65 +623,85 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
       for (int d = 0; d < DT; ++d) kf[d] = load_col(s.k, LD, 32 * c, 16 * d, lane);
       mma_all<T>(S, kf, uw);
     }
-    fv.write(s.v, out.at(t0), out.step, rows, min(C, a.steps - t0), w, lane);
+    if (OUT) fv.write(s.v, out.at(t0), out.step, rows, min(C, a.steps - t0), w, lane);
   }
-  for (int t = live * C + tid / DV; t < a.steps; t += NT / DV) out.at(t)[tid % DV] = (T)0.0f;   // padding
-  if (a.final_state) {
+  if (!OUT) {
+    put_carry<DT>(boundary(seg, eh, part, DK, all), S, unit, all, c0, w, lane);
+    return;
+  }
+  const int to = PASS == ALONE || at + 1 == seg.count ? a.steps : (begin + seg.chunks) * C;
+  for (int t = max(live, begin) * C + tid / DV; t < to; t += NT / DV) out.at(t)[tid % DV] = (T)0.0f;   // padding
+  if (a.final_state && end == live && (begin < end || at == 0)) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) a.final_state[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] = S[d][r];
+      for (int r = 0; r < 4; ++r) a.final_state[((int64_t)eh * DK + 16 * d + 4 * g + r) * all + c0 + col] = S[d][r];
   }
 }
 
 // ---- backward along the rollout ------------------------------------------------------------
 // The gradient of the state, from the last chunk to the first, and with it M and v'.  Every
 // product's columns are value columns, so a wave works on its 16 alone, as in the forward pass.
-template <class T, int DK, int NW, bool SOLVED>
-__global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())) void backward_state_kernel(bsg_delta a) {
+template <class T, int DK, int NW, Pass PASS>
+__global__ __launch_bounds__(64 * NW, (PASS == ALONE ? waves_per_simd<T, DK, NW>() : PASS == CARRY && sizeof(T) == 2 ? 2 : 1)) void backward_state_kernel(bsg_delta a, Segments seg) {
   constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW;
-  constexpr bool AHEAD = SOLVED || sizeof(T) == 2;   // fp32 rows a chunk ahead would cost spilled registers
-  __shared__ __align__(16) Chunk<T, DK, NW> s;
+  constexpr bool AHEAD = PASS != ALONE || sizeof(T) == 2;   // fp32 rows a chunk ahead would cost spilled registers
+  constexpr bool OUT = PASS != CARRY, LDS = sizeof(T) == 2;
+  __shared__ __align__(16) Chunk<T, DK, NW, PASS == ALONE, true, LDS> s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
-  // the workgroup's columns of all: all of them, but where the chunks are solved beforehand
-  const int all = SOLVED ? a.dim_v : DV, groups = all / DV, id = blockIdx.x / groups, c0 = blockIdx.x % groups * DV;
-  const int h = id % a.heads_v, e = id / a.heads_v, hk = h / (a.heads_v / a.heads_k);
-  const int n = steps_of(a, e), col = 16 * w + m;
-  const int chunks = (a.steps + C - 1) / C, live = (n + C - 1) / C;
-  const int64_t eh = (int64_t)e * a.heads_v + h;
+  // the workgroup's columns of all (CARRY: and of the unit matrix's, behind them) and its segment
+  const int all = PASS == ALONE ? DV : a.dim_v, groups = all / DV + (OUT ? 0 : (DK + DV - 1) / DV);
+  const int segments = PASS == ALONE ? 1 : OUT ? seg.count : seg.count - 1, id = blockIdx.x / groups, part = id % segments;
+  const int eh = id / segments, h = eh % a.heads_v, e = eh / a.heads_v, hk = h / (a.heads_v / a.heads_k);
+  const bool unit = !OUT && (int)(blockIdx.x % groups) >= all / DV;
+  const int c0 = (int)(blockIdx.x % groups) * DV - (unit ? all : 0), col = 16 * w + m;
+  const int n = steps_of(a, e), chunks = (a.steps + C - 1) / C, live = (n + C - 1) / C;
+  const int at = OUT ? part : part + 1;              // the segment
+  const int begin = PASS == ALONE ? 0 : at * seg.chunks, end = PASS == ALONE ? live : min(begin + seg.chunks, live);
+  if (!OUT && (part + 1) * seg.chunks >= live) return;   // no boundary before the rollout's end
 
-  constexpr int SIDE = SOLVED ? DT : 2;          // tiles of D side by side: registers allow no more
+  constexpr int SIDE = PASS == JOINED ? DT : 2;          // tiles of D side by side: registers allow no more
   f32x4 D[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      D[d][r] = a.dfinal ? a.dfinal[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] : 0.0f;
+      D[d][r] = !OUT ? unit && 16 * d + 4 * g + r == c0 + col ? 1.0f : 0.0f
+                     : a.dfinal ? a.dfinal[((int64_t)eh * DK + 16 * d + 4 * g + r) * all + c0 + col] : 0.0f;
+  if (PASS == JOINED && end < live) {
+    const float* p = tiles(boundary(seg, eh, at, DK, all), 0, 1, DT, c0 / 16 + w, lane);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) D[d] = *reinterpret_cast<const f32x4*>(p + 256 * d);
+  }
 
   Fetch<T, C, DK, NT> fk, fq;
-  Columns<T, NW> fv;
-  FetchSolved<T, NT> fs;
+  Columns<T, NW, LDS> fv;
+  FetchSolved<T, NT, true> fs;
   RawGates raw = {0, 0, 0};
-  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), dout = steps_in<const T>(a.dout, e, h, c0);
+  const Steps<const T> k = steps_in<const T>(a.k, e, hk), q = steps_in<const T>(a.q, e, hk), dout = steps_in<const T>(a.dout, e, h, unit ? 0 : c0);
   const Steps<T> dv = steps_in<T>(a.dv, e, h, c0);
   const GateSteps gate(a, e, h);
-  float *const ws = tiles(a.work_states, eh * chunks, all / 16, DT, c0 / 16 + w, lane), *const wm = tiles(a.work_w, eh * chunks, all / 16, 4, c0 / 16 + w, lane);
-  if (live > 0) {
-    const int t0 = (live - 1) * C;
+  float *const ws = tiles(a.work_states, (int64_t)eh * chunks, all / 16, DT, c0 / 16 + w, lane), *const wm = tiles(a.work_w, (int64_t)eh * chunks, all / 16, 4, c0 / 16 + w, lane);
+  if (begin < end) {
+    const int t0 = (end - 1) * C;
     if (AHEAD) {
       fk.load(k.at(t0), k.step, n - t0, tid);
-      fq.load(q.at(t0), q.step, n - t0, tid);
-      fv.load(dout.at(t0), dout.step, n - t0, tid, col);
+      if (!unit) {
+        fq.load(q.at(t0), q.step, n - t0, tid);
+        fv.load(dout.at(t0), dout.step, n - t0, tid, col);
+      }
     }
-    if (SOLVED) fs.load(a.work, eh * chunks + live - 1, tid);
-    else {
-      if (w == 0) make_gates(s.s.gates[(live - 1) & 1], load_gates(gate, t0, n - t0, lane), gate.half, lane);
+    if constexpr (PASS != ALONE) {
+      fs.load(a.work, (int64_t)eh * chunks + end - 1, tid);
+    } else {
+      if (w == 0) make_gates(s.s.gates[(end - 1) & 1], load_gates(gate, t0, n - t0, lane), gate.half, lane);
       clear_above(s.s, tid, NT);
     }
   }
-  for (int ch = live - 1; ch >= 0; --ch) {
+  for (int ch = end - 1; ch >= begin; --ch) {
     const int t0 = ch * C, rows = min(C, n - t0), t1 = t0 - C;
-    const Gates& gates = s.s.gates[SOLVED ? 0 : ch & 1];
+    const bool more = ch > begin;
+    const Gates& gates = s.s.gates[PASS == ALONE ? ch & 1 : 0];
     if (!AHEAD) {
       fk.load(k.at(t0), k.step, rows, tid);
       fq.load(q.at(t0), q.step, rows, tid);
@@ -592,28 +709,33 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
     }
     __syncthreads();               // the chunk after is done with LDS
     fk.store(s.k, rows, tid);
-    fq.store(s.q, rows, tid);
-    fv.store(s.v, rows, tid);
-    if (SOLVED) fs.store(s.s, tid);
-    if (t1 >= 0) {
+    if (!unit) {
+      fq.store(s.q, rows, tid);
+      fv.store(s.v, rows, tid);
+    }
+    if constexpr (PASS != ALONE) fs.store(s.s, tid);
+    if (more) {
       if (AHEAD) {
         fk.load(k.at(t1), k.step, C, tid);
-        fq.load(q.at(t1), q.step, C, tid);
-        fv.load(dout.at(t1), dout.step, C, tid, col);
+        if (!unit) {
+          fq.load(q.at(t1), q.step, C, tid);
+          fv.load(dout.at(t1), dout.step, C, tid, col);
+        }
       }
-      if (SOLVED) fs.load(a.work, eh * chunks + ch - 1, tid);
+      if (PASS != ALONE) fs.load(a.work, (int64_t)eh * chunks + ch - 1, tid);
       else if (w == 0) raw = load_gates(gate, t1, C, lane);
     }
     __syncthreads();
-    if (!SOLVED) solve_chunk<T, DK, NW, true>(s, gates, a.scale, lane, w);
+    if constexpr (PASS == ALONE) solve_chunk<T, DK, NW, true>(s, gates, a.scale, lane, w);
 
+    if (OUT)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(ws + (int64_t)ch * DK * all + 256 * d) = D[d];
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(ws + (int64_t)ch * DK * all + 256 * d) = D[d];
 
-    f32x4 x[4], go[4];
+    f32x4 x[4], go[4] = {};
 #pragma unroll
     for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
-    fv.get(go, s.v, rows, w, lane);
+    if (!unit) fv.get(go, s.v, rows, w, lane);
 #pragma unroll
     for (int c = 0; c < DK / 32; ++c) {
       WideOf<T, 3> dw;
@@ -625,14 +747,15 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) x[b] *= *reinterpret_cast<const f32x4*>(&gates.out[16 * b + 4 * g]);
+    if (!unit)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const Frag<T> gf = round_frag<T>(join(go[2 * c], go[2 * c + 1]));   // as it was read
+      for (int c = 0; c < 2; ++c) {
+        const Frag<T> gf = round_frag<T>(join(go[2 * c], go[2 * c + 1]));   // as it was read
 #pragma unroll
-      for (int b = 0; b < 2 * c + 2; ++b) mma<T>(x[b], s.s.p_col(16 * b, 32 * c, lane), gf);
-    }
-    if (!SOLVED) {
-      if (w == 0 && t1 >= 0) make_gates(s.s.gates[(ch + 1) & 1], raw, gate.half, lane);
+        for (int b = 0; b < 2 * c + 2; ++b) mma<T>(x[b], s.s.p_col(16 * b, 32 * c, lane), gf);
+      }
+    if (PASS == ALONE) {
+      if (w == 0 && more) make_gates(s.s.gates[(ch + 1) & 1], raw, gate.half, lane);
       __syncthreads();             // the inverses are there
     }
     f32x4 M[4];
@@ -640,8 +763,8 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
     for (int b = 3; b >= 0; --b) {
 #pragma unroll
       for (int u = b + 1; u < 4; ++u) {
-        const float* p = &s.s.n[(16 * u + 4 * g) * AP + 16 * b + m];
-        mma16(x[b], f32x4{p[0], p[AP], p[2 * AP], p[3 * AP]}, M[u]);
+        const float* p = &s.s.n[s.s.tile(u, b) + 4 * g * IP + m];
+        mma16(x[b], f32x4{p[0], p[IP], p[2 * IP], p[3 * IP]}, M[u]);
       }
       const float* p = &s.s.inv[(16 * b + 4 * g) * IP + m];
       M[b] = f32x4{0, 0, 0, 0};
@@ -649,10 +772,10 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      *reinterpret_cast<f32x4*>(wm + (int64_t)ch * C * all + 256 * b) = M[b];
+      if (OUT) *reinterpret_cast<f32x4*>(wm + (int64_t)ch * C * all + 256 * b) = M[b];
       M[b] *= *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);
     }
-    fv.put(s.v, M, dv.at(t0), dv.step, rows, min(C, a.steps - t0), w, lane);
+    if (OUT) fv.put(s.v, M, dv.at(t0), dv.step, rows, min(C, a.steps - t0), w, lane);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const f32x4 in = *reinterpret_cast<const f32x4*>(&gates.in[16 * b + 4 * g]);
@@ -668,28 +791,33 @@ __global__ __launch_bounds__(64 * NW, (SOLVED ? 1 : waves_per_simd<T, DK, NW>())
       split(ow, join(go[2 * c], go[2 * c + 1]));
 #pragma unroll
       for (int d0 = 0; d0 < DT; d0 += SIDE) {
-        f32x4 part[SIDE];
+        f32x4 x[SIDE];
         Frag<T> kf[SIDE], qf[SIDE];
 #pragma unroll
         for (int d = 0; d < SIDE; ++d) {
-          part[d] = D[d0 + d];
+          x[d] = D[d0 + d];
           kf[d] = load_col(s.k, LD, 32 * c, 16 * (d0 + d), lane);
-          qf[d] = load_col(s.q, LD, 32 * c, 16 * (d0 + d), lane);
+          if (!unit) qf[d] = load_col(s.q, LD, 32 * c, 16 * (d0 + d), lane);
         }
-        mma_all<T>(part, kf, lw);
-        mma_all<T>(part, qf, ow);
+        mma_all<T>(x, kf, lw);
+        if (!unit) mma_all<T>(x, qf, ow);
 #pragma unroll
-        for (int d = 0; d < SIDE; ++d) D[d0 + d] = part[d];
+        for (int d = 0; d < SIDE; ++d) D[d0 + d] = x[d];
       }
     }
-    fv.write(s.v, dv.at(t0), dv.step, rows, min(C, a.steps - t0), w, lane);
+    if (OUT) fv.write(s.v, dv.at(t0), dv.step, rows, min(C, a.steps - t0), w, lane);
   }
-  for (int t = live * C + tid / DV; t < a.steps; t += NT / DV) dv.at(t)[tid % DV] = (T)0.0f;   // padding
-  if (a.dstate) {
+  if (!OUT) {
+    put_carry<DT>(boundary(seg, eh, part, DK, all), D, unit, all, c0, w, lane);
+    return;
+  }
+  const int to = PASS == ALONE || at + 1 == seg.count ? a.steps : (begin + seg.chunks) * C;
+  for (int t = max(live, begin) * C + tid / DV; t < to; t += NT / DV) dv.at(t)[tid % DV] = (T)0.0f;   // padding
+  if (a.dstate && at == 0) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) a.dstate[(eh * DK + 16 * d + 4 * g + r) * all + c0 + col] = D[d][r];
+      for (int r = 0; r < 4; ++r) a.dstate[((int64_t)eh * DK + 16 * d + 4 * g + r) * all + c0 + col] = D[d][r];
   }
 }
 
@@ -1088,7 +1216,7 @@ hipError_t run(const bsg_delta_act& a, bool, hipStream_t st) {
   return hipGetLastError();
 }
 // Where the rows (envs x value heads) leave CUs idle, the pass along a rollout is bound by the time
-// of one chunk, and the chunks are solved beforehand, side by side (SOLVED); where they do not, solving
+// of one chunk, and the chunks are solved beforehand, side by side; where they do not, solving
 // in place saves the way of the matrices through memory.
 bool solved_first(const bsg_delta& a) {
   return a.dim_v > 32 && a.steps > C && (int64_t)a.num_envs * a.heads_v < 256;
@@ -1098,29 +1226,58 @@ int64_t solved_work(const bsg_delta& a) {
   const int64_t chunks = (int64_t)a.num_envs * a.heads_v * ((a.steps + C - 1) / C);
   return chunks * (a.dtype == BSG_BF16 ? solved_bytes<bf16>() : solved_bytes<float>());
 }
+// ... and the rollout is cut into as many segments as give each CU a workgroup of the last pass, of three
+// chunks at least (a boundary costs its transition and its turn of the join).  Learning call, 4 heads, dim
+// 128: 4 envs x 4095 steps 854 -> 422 us, 1 x 4095 743 -> 232, 8 x 4095 1001 -> 740, 4 x 1000 238 -> 178,
+// 2 x 700 180 -> 161; at 500 steps the host's time for the launches takes what it saves (183 -> 198).
+// Two workgroups a CU: 4 x 4095 462 us; two segments: 16 x 4095 1327 -> 1288 us, hence three at least.
+Segments segments(const bsg_delta& a) {
+  const int chunks = (a.steps + C - 1) / C, rows = a.num_envs * a.heads_v;
+  Segments seg = {nullptr, 1, chunks};
+  if (!solved_first(a)) return seg;
+  const int most = min(256 / (rows * (a.dim_v / 64)), chunks / 3);
+  if (most < 3) return seg;
+  seg.chunks = (chunks + most - 1) / most;
+  seg.count = (chunks + seg.chunks - 1) / seg.chunks;
+  seg.carry = reinterpret_cast<float*>(static_cast<char*>(a.work) + solved_work(a));
+  return seg;
+}
+int64_t carry_work(const bsg_delta& a) {
+  return (int64_t)a.num_envs * a.heads_v * (segments(a).count - 1) * a.dim_k * (a.dim_k + a.dim_v) * 4;
+}
 template <class T, int DK, int NW>
 hipError_t run(const bsg_delta& a, bool back, hipStream_t st) {
   const dim3 rows((unsigned)(a.num_envs * a.heads_v));
+  const Segments seg = segments(a);
   if (solved_first(a)) {
     if constexpr (NW > 2) {
-      const dim3 all((unsigned)(a.num_envs * a.heads_v * ((a.steps + C - 1) / C))), groups(rows.x * (NW / 4));
+      const dim3 all((unsigned)(rows.x * ((a.steps + C - 1) / C))), groups(rows.x * (NW / 4) * seg.count);
+      const dim3 carries(rows.x * (NW / 4 + (DK + 63) / 64) * (seg.count - 1)), joins(rows.x * NW);
       if (back) {
         solve_kernel<T, DK, true><<<all, dim3(256), 0, st>>>(a);
-        backward_state_kernel<T, DK, 4, true><<<groups, dim3(256), 0, st>>>(a);
+        if (seg.count > 1) {
+          backward_state_kernel<T, DK, 4, CARRY><<<carries, dim3(256), 0, st>>>(a, seg);
+          join_kernel<DK, true><<<joins, dim3(4 * DK), 0, st>>>(a, seg);
+        }
+        backward_state_kernel<T, DK, 4, JOINED><<<groups, dim3(256), 0, st>>>(a, seg);
       } else {
         solve_kernel<T, DK, false><<<all, dim3(256), 0, st>>>(a);
-        forward_kernel<T, DK, 4, true><<<groups, dim3(256), 0, st>>>(a);
+        if (seg.count > 1) {
+          forward_kernel<T, DK, 4, CARRY><<<carries, dim3(256), 0, st>>>(a, seg);
+          join_kernel<DK, false><<<joins, dim3(4 * DK), 0, st>>>(a, seg);
+        }
+        forward_kernel<T, DK, 4, JOINED><<<groups, dim3(256), 0, st>>>(a, seg);
       }
     }
   } else if (back) {
-    backward_state_kernel<T, DK, NW, false><<<rows, dim3(64 * NW), 0, st>>>(a);
+    backward_state_kernel<T, DK, NW, ALONE><<<rows, dim3(64 * NW), 0, st>>>(a, seg);
   } else {
-    forward_kernel<T, DK, NW, false><<<rows, dim3(64 * NW), 0, st>>>(a);
+    forward_kernel<T, DK, NW, ALONE><<<rows, dim3(64 * NW), 0, st>>>(a, seg);
   }
   if (back) {
     const dim3 chunks((unsigned)(a.num_envs * a.heads_k * ((a.steps + C - 1) / C)));
     const int group = a.heads_v / a.heads_k;
-    float* sums = group > 1 ? reinterpret_cast<float*>(static_cast<char*>(a.work) + solved_work(a)) : nullptr;
+    float* sums = group > 1 ? reinterpret_cast<float*>(static_cast<char*>(a.work) + solved_work(a) + carry_work(a)) : nullptr;
     for (int head = 0; head < group; ++head) backward_chunk_kernel<T, DK><<<chunks, dim3(512), 0, st>>>(a, sums, head);
   }
   return hipGetLastError();
@@ -1146,7 +1303,7 @@ hipError_t launch_delta_forward(const bsg_delta& a, hipStream_t st) { return run
 hipError_t launch_delta_backward(const bsg_delta& a, hipStream_t st) { return run(a, true, st); }
 int64_t delta_work_bytes(const bsg_delta& a, bool back) {
   const int64_t chunks = (int64_t)a.num_envs * a.heads_k * ((a.steps + C - 1) / C);
-  return solved_work(a) + (back && a.heads_v > a.heads_k ? chunks * C * a.dim_k * 2 * 4 : 0);
+  return solved_work(a) + carry_work(a) + (back && a.heads_v > a.heads_k ? chunks * C * a.dim_k * 2 * 4 : 0);
 }
 hipError_t launch_delta_step(const bsg_delta_act& a, hipStream_t st) { return run(a, false, st); }
 

@@ -121,28 +121,36 @@ __device__ __forceinline__ bf16x8 load_col(const bf16* s, int ld, int k0, int m0
 }
 
 // ---- conversions ---------------------------------------------------------------------------
+// two values to bf16, a in the low half: one instruction (value by value it is two and one to join them)
+__device__ __forceinline__ uint32_t pair(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
 template <class T, int N>
 __device__ __forceinline__ void split(Wide<T, N>& w, const f32x8& x);
 __device__ __forceinline__ void split(Wide<float, 1>& w, const f32x8& x) { w.p[0] = x; }
 template <int N>
 __device__ __forceinline__ void split(Wide<bf16, N>& w, const f32x8& x) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   f32x8 rest = x;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
+    u32x4 part;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      w.p[i][j] = (bf16)rest[j];
-      rest[j] -= (float)w.p[i][j];
+    for (int j = 0; j < 4; ++j) {
+      part[j] = pair(rest[2 * j], rest[2 * j + 1]);
+      rest[2 * j] -= __uint_as_float(part[j] << 16);
+      rest[2 * j + 1] -= __uint_as_float(part[j] & 0xffff0000u);
     }
+    w.p[i] = __builtin_bit_cast(bf16x8, part);
   }
 }
 template <class T> __device__ __forceinline__ Frag<T> round_frag(const f32x8& x);
 template <> __device__ __forceinline__ f32x8 round_frag<float>(const f32x8& x) { return x; }
 template <> __device__ __forceinline__ bf16x8 round_frag<bf16>(const f32x8& x) {
-  bf16x8 r;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = (bf16)x[j];
-  return r;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(bf16x8, u32x4{pair(x[0], x[1]), pair(x[2], x[3]), pair(x[4], x[5]), pair(x[6], x[7])});
 }
 __device__ __forceinline__ f32x8 widen(const f32x8& x) { return x; }
 __device__ __forceinline__ f32x8 widen(const bf16x8& x) {

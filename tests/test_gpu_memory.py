@@ -129,6 +129,13 @@ DELTA = [  # E, T, Hk, H, Dk, Dv, dtype, first, lengths, order, state, gates
     (129, 65, 1, 2, 128, 32, "bf16", "edges", None, "te", True, None),
     (260, 65, 1, 1, 128, 64, "bf16", None, "ragged", "te", True, None),
     (256, 65, 1, 1, 128, 128, "fp32", "0.1", None, "te", True, None),
+    # few rows and many chunks: the rollout is cut into segments
+    (1, 700, 2, 4, 128, 128, "bf16", None, None, "te", True, None),
+    (3, 641, 1, 2, 32, 64, "fp32", "0.004", "ragged", "gap", True, "fp32"),
+    (2, 1025, 1, 1, 64, 64, "bf16", "0.002", "ragged", "te", False, None),
+    (2, 520, 1, 1, 128, 64, "fp32", None, None, "te", True, None),
+    (4, 577, 2, 2, 32, 128, "bf16", "0.01", "ragged", "te", True, "fp32"),
+    (2, 899, 1, 2, 64, 128, "fp32", "edges", None, "et", True, None),
 ]
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
 
