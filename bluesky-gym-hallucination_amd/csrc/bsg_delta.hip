@@ -117,6 +117,7 @@ __device__ __forceinline__ RawGates load_gates(const GateSteps& s, int t0, int r
   return r;
 }
 __device__ __forceinline__ void make_gates(Gates& s, const RawGates& raw, bool half, int lane) {
+  asm volatile("" : "+v"(lane));   // else a comparison's mask a step stays in scalar registers all along
   double c = (double)at_least_lowest(__uint_as_float(half ? raw.g << 16 : raw.g)) * 1.4426950408889634074;
   const unsigned long long begun = __ballot(raw.first != 0);
 #pragma unroll
@@ -266,7 +267,7 @@ struct Columns<T, NW, false> {
 
 // lane j of each row of 16 lanes, to all of them
 template <int J> __device__ __forceinline__ float from_lane(float x) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + J, 0xf, 0xf, false));
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + J, 0xf, 0xf, true));
 }
 // some columns x[c] of lane i's row: less n_iJ times row J of the inverse, which is done (and 0 before
 // the column's own row)
@@ -285,6 +286,7 @@ template <int J, int N> __device__ __forceinline__ void eliminate(float (&x)[N],
 template <class T, int DK, int NW, bool BACK, class X>
 __device__ __forceinline__ void solve_chunk(X& x, const Gates& gates, float scale, int lane, int w) {
   constexpr int LD = pitch<T>(DK), PD = pitch<T>(C);
+  asm volatile("" : "+v"(lane));
   auto& s = x.s;
   const int m = lane & 15, g = lane >> 4;
 #pragma unroll
