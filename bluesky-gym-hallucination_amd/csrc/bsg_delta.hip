@@ -166,8 +166,14 @@ struct Solved {
   float n[6 * 16 * IP];            // minus the matrix of the system: the tiles below the diagonal,
   float inv[4 * 16 * IP];          // ... the inverses of those on it,
   Gates gates[HERE ? 2 : 1];       // (of this chunk and the one that comes next)
-  float diagonal[HERE ? 4 * 16 * IP : 4];   // ... and those themselves
   static constexpr int tile(int b, int u) { return (b * (b - 1) / 2 + u) * 16 * IP; }
+  // ... and those themselves, needed for the inverses only, where P has zeros that no product reads: rows
+  // 0..31, columns 32..63 (in LDS of their own: dims 32 at 600 x 300 544 against 515 us, dims 128 and 64 at
+  // 300 x 300 833 against 777, where a workgroup more fits a CU).
+  static constexpr int DP = PD * (int)sizeof(T) / 4;
+  __device__ __forceinline__ float* diagonal(int b) {
+    return reinterpret_cast<float*>(p[sizeof(T) == 2 ? b & 1 : 0] + (b >> 1) * 16 * PD + 32 + (sizeof(T) == 2 ? 0 : (b & 1) * 16));
+  }
   __device__ __forceinline__ WideOf<T, 2> p_row(int r, int k0, int g) const {
     WideOf<T, 2> w;
 #pragma unroll
@@ -182,7 +188,7 @@ struct Solved {
   }
 };
 // ... which passes through memory up to the first gates where the chunks are solved beforehand.
-template <class T> constexpr int solved_bytes() { return sizeof(Solved<T, true, false>) - 16; }
+template <class T> constexpr int solved_bytes() { return sizeof(Solved<T, true, false>); }
 template <class T> constexpr int p_bytes() { return sizeof(Solved<T, true, false>::p); }
 
 // A workgroup of NW waves handles 16 NW value columns of one env and value head; wave w owns 16 of
@@ -303,11 +309,12 @@ __device__ __forceinline__ void solve_chunk(X& x, const Gates& gates, float scal
     const float bj = gates.beta[j];
     const f32x4 bi = *reinterpret_cast<const f32x4*>(&gates.beta[16 * b + 4 * g]);
     const f32x4 f = decays<false>(gates, 16 * b + 4 * g, step_of(gates, j));
-    float* n = (b == u ? s.diagonal + 16 * IP * b : s.n + s.tile(b, u)) + 4 * g * IP + m;
+    const int np = b == u ? s.DP : IP;
+    float* n = (b == u ? s.diagonal(b) : s.n + s.tile(b, u)) + 4 * g * np + m;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * b + 4 * g + r;
-      n[r * IP] = j < i ? -(BACK ? bi[r] : bj) * f[r] * kk[r] : 0.0f;
+      n[r * np] = j < i ? -(BACK ? bi[r] : bj) * f[r] * kk[r] : 0.0f;
       float y = j <= i ? scale * f[r] * qk[r] : 0.0f;
 #pragma unroll
       for (int o = 0; o < Parts<T, 2>::n; ++o) {
@@ -323,7 +330,7 @@ __device__ __forceinline__ void solve_chunk(X& x, const Gates& gates, float scal
   float v[N], n[16];               // lane: block g, row m
 #pragma unroll
   for (int j = 0; j < 16; j += 4) {
-    const f32x4 y = *reinterpret_cast<const f32x4*>(&s.diagonal[(16 * g + m) * IP + j]);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(s.diagonal(g) + m * s.DP + j);
 #pragma unroll
     for (int o = 0; o < 4; ++o) n[j + o] = y[o];
   }
@@ -476,7 +483,8 @@ __global__ __launch_bounds__(4 * DK) void join_kernel(bsg_delta a, Segments seg)
 template <class T, int DK, int NW, Pass PASS>
 __global__ __launch_bounds__(64 * NW, (PASS == ALONE ? waves_per_simd<T, DK, NW>() : PASS == CARRY && sizeof(T) == 2 ? 2 : 1)) void forward_kernel(bsg_delta a, Segments seg) {
   constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW;
-  constexpr bool AHEAD = PASS != ALONE || sizeof(T) == 2;   // fp32 rows a chunk ahead would cost spilled registers
+  // rows a chunk ahead; not for fp32 solved in place (600 envs x 50 steps, dims 32: 186 -> 198 us)
+  constexpr bool AHEAD = PASS != ALONE || sizeof(T) == 2;
   constexpr bool OUT = PASS != CARRY, LDS = sizeof(T) == 2;
   __shared__ __align__(16) Chunk<T, DK, NW, PASS == ALONE, OUT, LDS> s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
@@ -647,7 +655,8 @@ __global__ __launch_bounds__(64 * NW, (PASS == ALONE ? waves_per_simd<T, DK, NW>
 template <class T, int DK, int NW, Pass PASS>
 __global__ __launch_bounds__(64 * NW, (PASS == ALONE ? waves_per_simd<T, DK, NW>() : PASS == CARRY && sizeof(T) == 2 ? 2 : 1)) void backward_state_kernel(bsg_delta a, Segments seg) {
   constexpr int LD = pitch<T>(DK), DT = DK / 16, DV = 16 * NW, NT = 64 * NW;
-  constexpr bool AHEAD = PASS != ALONE || sizeof(T) == 2;   // fp32 rows a chunk ahead would cost spilled registers
+  // rows a chunk ahead; not for fp32 solved in place (600 envs x 50 steps, dims 32: 186 -> 198 us)
+  constexpr bool AHEAD = PASS != ALONE || sizeof(T) == 2;
   constexpr bool OUT = PASS != CARRY, LDS = sizeof(T) == 2;
   __shared__ __align__(16) Chunk<T, DK, NW, PASS == ALONE, true, LDS> s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
