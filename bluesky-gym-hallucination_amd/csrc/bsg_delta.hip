@@ -409,7 +409,7 @@ __device__ __forceinline__ float* tiles(float* p, int64_t chunk, int waves, int 
 // A rollout in segments of whole chunks.  What a segment does to the state before it is affine: with
 // the products of its chunks' transitions A[dim_k][dim_k] (the pass run on the unit matrix, without
 // values) and what it makes of no state, B[dim_k][dim_v], S' = A S + B.  `carry` holds, per row (env and
-// value head) and boundary of segments, B by D tiles and A by rows; join_kernel puts the state at the
+// value head) and boundary of segments, B by D tiles and A by the lanes that multiply it; join_kernel puts the state at the
 // boundary in B's place.
 struct Segments {
   float* carry;
@@ -430,7 +430,8 @@ __device__ __forceinline__ void put_carry(float* to, const f32x4 (&x)[DT], bool 
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) to[16 * DT * all + (16 * d + 4 * (lane >> 4) + r) * 16 * DT + col] = x[d][r];
+      for (int r = 0; r < 4; ++r)
+        to[16 * DT * all + ((d * DT + col / 16) * 64 + col % 16 / 4 * 16 + 4 * (lane >> 4) + r) * 4 + col % 4] = x[d][r];
   }
 }
 // S' = A S + B from boundary to boundary (BACK: from the last one to the first).  A workgroup holds 16
@@ -456,10 +457,10 @@ __global__ __launch_bounds__(4 * DK) void join_kernel(bsg_delta a, Segments seg)
     float* p = at(i);
     o.x = *reinterpret_cast<const f32x4*>(tiles(p, 0, 1, DT, c0 / 16, lane) + 256 * w);
 #pragma unroll
-    for (int u = 0; u < DT; ++u) o.a[u] = *reinterpret_cast<const f32x4*>(p + DK * all + (16 * w + m) * DK + 16 * u + 4 * g);
+    for (int u = 0; u < DT; ++u) o.a[u] = *reinterpret_cast<const f32x4*>(p + DK * all + ((w * DT + u) * 64 + lane) * 4);
   };
   const auto step = [&](Step& o, Step& next, int i) {
-    if (i + 1 < boundaries) load(next, i + 1);
+    load(next, min(i + 1, boundaries - 1));   // no branch: it would wait for all loads
     f32x4 y = {0, 0, 0, 0};        // two sums, so that products do not wait for each other
 #pragma unroll
     for (int u = 0; u < DT; u += 2) {
