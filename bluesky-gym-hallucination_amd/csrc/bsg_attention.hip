@@ -154,6 +154,10 @@ __global__ __launch_bounds__(256) void forward_kernel(bsg_attention a) {
       s[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) mma(s[t], load_run(sK + (16 * t + m) * LD, 32 * c, g), qf[c]);
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      if (sizeof(T) == 4 && k0 + 16 * t > qw + 15) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float y;

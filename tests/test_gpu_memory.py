@@ -708,3 +708,41 @@ def test_out_tensors_are_written_in_place():
     assert got.data_ptr() == big[:, 1:3].data_ptr()
     assert (big[:, 0] == -7).all() and (big[:, 3] == -7).all()
     assert torch.equal(big[:, 1:3].cpu(), x["v"][:, 0].expand(3, 2, 64))
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_acting_calls_look_at_every_address_and_number(dt):
+    """What is known of a call's layouts from the one before says nothing of its addresses, scale or cap."""
+    dtype, g = DT[dt], gen(77)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).to(DEV)  # noqa: E731
+    shift = lambda x: torch.cat([x.new_zeros(1), x.reshape(-1)])[1:].view(x.shape)  # noqa: E731  (one element further)
+    q, k, v = r(3, 2, 64), r(3, 2, 64), r(3, 2, 64)
+    gates = -torch.rand(3, 2, generator=g).to(DEV), torch.rand(3, 2, generator=g).to(DEV)
+    S, caches = torch.randn(3, 2, 64, 64, generator=g).to(DEV), (r(3, 2, 7, 64), r(3, 2, 7, 64))
+
+    def delta(q, k, v, state=None, **kw):
+        state = S.clone() if state is None else state
+        return memory.gated_delta_step(q, k, v, *gates, state, **kw), state
+
+    def attend(q, k, v, kc=None, **kw):
+        kc, vc = caches[0].clone() if kc is None else kc, caches[1].clone()
+        steps = torch.full((3,), 5, dtype=torch.int32, device=DEV)
+        return memory.episode_attention_step(q, k, v, kc, vc, steps, **kw), kc, vc, steps
+
+    for act, kw in ((delta, dict(scale=0.3)), (attend, dict(scale=0.3)), (attend, dict(softcap=0.5))):
+        plain, other = act(q, k, v), act(q, k, v, **kw)
+        assert not torch.equal(plain[0], other[0])
+        for args in ((shift(q), k, v), (q, shift(k), v), (q, k, shift(v)), (q, k, v)):
+            assert all(torch.equal(a, b) for a, b in zip(act(*args), plain))
+            assert all(torch.equal(a, b) for a, b in zip(act(*args, **kw), other))
+        assert torch.equal(act(q, k, v, out=torch.empty_like(q))[0], plain[0])
+        gap = torch.zeros(3, 4, 64, dtype=dtype, device=DEV)[:, ::2]
+        assert torch.equal(act(q, k, v, out=gap)[0], plain[0]) and gap.stride() == (256, 128, 1)
+        turned = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+        assert all(torch.equal(a, b) for a, b in zip(act(*turned), plain))
+        with pytest.raises(ValueError):
+            act(q, k, v, out=shift(torch.empty_like(q)))
+    with pytest.raises(ValueError):
+        delta(q, k, v, state=shift(S))
+    with pytest.raises(ValueError):
+        attend(q, k, v, kc=shift(caches[0]))
