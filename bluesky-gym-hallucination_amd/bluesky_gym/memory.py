@@ -46,16 +46,6 @@ __all__ = ["gated_delta_rule", "gated_delta_step", "episode_attention", "episode
 
 # ---- checks and views -----------------------------------------------------------------------
 
-def _tensors(who, ref, **named):
-    """Every tensor on one HIP device."""
-    dev = ref.device
-    if dev.type != "cuda":
-        raise nat.BsgError(f"{who} runs on a HIP device (no CPU fallback)")
-    for n, x in named.items():
-        if x is not None and x.device != dev:
-            raise ValueError(f"{who}: {n} is on {x.device}, q is on {dev}")
-
-
 class _Layout(NamedTuple):
     """What of a tensor its checks look at, its address aside."""
     dtype: torch.dtype
@@ -128,17 +118,26 @@ def _vectors(x):
     return x if _aligned(x) else x.clone(memory_format=torch.contiguous_format)
 
 
-def _empty_like(x):
-    """A dense tensor in the order of axes of x, whose rows the kernels can read, with rows they
-    can write."""
-    y = torch.empty_like(x)
-    return y if y.stride() == x.stride() or _aligned(y) else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+def _row_strides(shape, s):
+    """The strides of a bsg_rows: a rollout's [E, T, H, D], a gate's [E, T, H]."""
+    return (s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0)
 
 
 def _rows(x):
-    """A bsg_rows: a rollout's [E, T, H, D], a gate's [E, T, H]."""
-    s, n = x.stride(), x.shape
-    return (x.data_ptr(), s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+    return (x.data_ptr(), *_row_strides(x.shape, x.stride()))
+
+
+def _new_strides(x):
+    """The strides of a tensor made like one of this layout (in its order of axes, as torch.empty_like
+    would, where rows can be written so, else contiguous), and a bsg_rows' of them."""
+    y = torch.empty_like(torch.empty_strided(x.shape, x.strides, dtype=x.dtype, device="meta"))
+    if not _vector_strides(y.shape, y.stride(), y.element_size()):
+        y = torch.empty(x.shape, device="meta")
+    return y.stride(), _row_strides(y.shape, y.stride())
+
+
+def _new(x, strides):
+    return torch.empty_strided(x.shape, strides, dtype=x.dtype, device=x.device)
 
 
 def _step_strides(x):
@@ -152,10 +151,6 @@ _NO_ROWS = (0, 0, 0, 0)
 
 def _ptr(x):
     return 0 if x is None else x.data_ptr()
-
-
-def _flag_rows(first):
-    return (0, 0, 0) if first is None else (first.data_ptr(), first.stride(0), first.stride(1))
 
 
 def _numbers(who, scale, dim, softcap=0.0, window=0):
@@ -180,9 +175,9 @@ def _no_grad(who, *xs):
         raise ValueError(f"{who} has no gradient: act under torch.no_grad()")
 
 
-# An acting call of a few envs is host time, so what follows from the layouts alone (checks, strides)
-# is worked out once per combination of them (14.5 -> 9.8 us attention, 14.8 -> 8.9 us delta rule, 4 envs).
-# Addresses are looked at in every call.
+# A call on a few envs is host time, so what follows from the layouts alone (checks, strides, sizes) is
+# worked out once per combination of them (an acting step of 4 envs: attention 14.5 -> 9.8 us, delta rule
+# 14.8 -> 8.9 us).  Addresses are looked at in every call.
 
 _ROWS_OUT = "out must have contiguous, 16-byte aligned rows"
 
@@ -226,13 +221,6 @@ def _call(fn, block, i):
 _pack_delta, _pack_delta_act = nat.packer(nat.BsgDelta), nat.packer(nat.BsgDeltaAct)
 
 
-def _delta_inputs(dtype, scale, q, k, v, g, beta, out, first, lengths):
-    """The leading fields of bsg_delta, up to lengths."""
-    E, T, H, Dv = v.shape
-    return (E, T, q.shape[2], H, q.shape[3], Dv, dtype, _DTYPES[g.dtype], scale, 0, *_rows(q), *_rows(k),
-            *_rows(v), *_rows(g), *_rows(beta), *out, *_flag_rows(first), _ptr(lengths))
-
-
 def _delta_check(who, q, k, v, g, beta, state, first, lead):
     Hk, Dk = q.shape[-2:]
     H, Dv = v.shape[-2:]
@@ -260,15 +248,70 @@ def _delta_sizes(E, T, Hk, H, Dk, Dv, dtype):
     return rows * Dk, rows * nat.DELTA_CHUNK, *work
 
 
+class _Plan(NamedTuple):
+    """What a learning call takes from its layouts."""
+    head: tuple                            # the leading fields of its block
+    device: int
+    strides: tuple                         # of the tensors that the backward pass reads again
+    vectors: bool                          # whether q, k and v are read as they are
+    rows: list                             # their bsg_rows strides, and the gates'
+    like: tuple                            # strides of what is made like q, k and v (_new),
+    to: tuple                              # ... as bsg_rows has them (delta rule: and of the gates' gradients)
+    first: tuple                           # strides
+    sizes: tuple                           # of scratch
+    key: tuple                             # the numbers the plan was made with
+
+
+def _dense(*xs):
+    return [None if x is None else x.contiguous() for x in xs]
+
+
+def _strides(*xs):
+    return tuple([None if x is None else x.stride() for x in xs])
+
+
+@lru_cache(maxsize=256)
+def _delta_plan(q, k, v, g, beta, state, first, lengths, scale):
+    who = "gated_delta_rule"
+    named = dict(q=q, k=k, v=v, g=g, beta=beta, state=state, first=first, lengths=lengths)
+    q, k, v, g, beta, state, first, lengths = (None if x is None else _Layout(*x) for x in named.values())
+    dtype = _heads(who, q, k, v, 4, Dk=q.shape[-1], Dv=v.shape[-1])
+    E, T, H, Dv = v.shape
+    _delta_check(who, q, k, v, g, beta, state, first, (E, T))
+    if lengths is not None:
+        _shape(who, "lengths", lengths, (E,), _INT32)
+    device, Hk, Dk = _layouts(who, **named), q.shape[2], q.shape[3]
+    like, to = zip(*(_new_strides(x) for x in (q, k, v)))
+    return _Plan((E, T, Hk, H, Dk, Dv, dtype, _DTYPES[g.dtype], _numbers(who, scale, Dk), 0), device,
+                 tuple([None if x is None else x.strides for x in (q, k, v, g, beta, first)]),
+                 all(_vector_strides(x.shape, x.strides, x.dtype.itemsize) for x in (q, k, v)),
+                 [_row_strides(x.shape, x.strides) for x in (q, k, v, g, beta)], like,
+                 (*to, _row_strides(g.shape, (T * H, H, 1))), (0, 0) if first is None else first.strides,
+                 _delta_sizes(E, T, Hk, H, Dk, Dv, dtype) if E and T else (), (scale,))
+
+
+def _plan_again(plan, numbers, *xs):
+    return plan(*[_layout(x) for x in xs], *numbers)
+
+
+def _delta_inputs(p, q, k, v, g, beta, out, first, lengths):
+    """The leading fields of bsg_delta, up to lengths."""
+    r = p.rows
+    return (*p.head, q.data_ptr(), *r[0], k.data_ptr(), *r[1], v.data_ptr(), *r[2], g.data_ptr(), *r[3],
+            beta.data_ptr(), *r[4], *out, _ptr(first), *p.first, _ptr(lengths))
+
+
 class _DeltaRule(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, first, lengths, scale, dtype, keep):
-        q, k, v = _vectors(q), _vectors(k), _vectors(v)
+    def forward(ctx, q, k, v, g, beta, state, first, lengths, p, keep):
+        if not p.vectors or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+            q, k, v = _vectors(q), _vectors(k), _vectors(v)
+            p = _plan_again(_delta_plan, p.key, q, k, v, g, beta, state, first, lengths)
         state = None if state is None else state.contiguous()
-        E, T, H, Dv = v.shape
-        Hk, Dk, dev = q.shape[2], q.shape[3], v.device
-        ns, nw, work, _ = _delta_sizes(E, T, Hk, H, Dk, Dv, dtype)
-        out = _empty_like(v)
+        E, T, Hk, H, Dk, Dv = p.head[:6]
+        dev = v.device
+        ns, nw, work, _ = p.sizes
+        out = _new(v, p.like[2])
         final = torch.empty((E, H, Dk, Dv), dtype=torch.float32, device=dev)
         scratch = torch.empty(work, dtype=torch.uint8, device=dev) if work else None
         kept, at = None, (0, 0)
@@ -276,35 +319,39 @@ class _DeltaRule(torch.autograd.Function):
             kept = torch.empty(ns + nw, dtype=torch.float32, device=dev)
             at = kept.data_ptr(), kept.data_ptr() + 4 * ns
         _call("bsg_delta_forward", _pack_delta(
-            *_delta_inputs(dtype, scale, q, k, v, g, beta, _rows(out), first, lengths), _ptr(state), final.data_ptr(),
-            *at, _ptr(scratch), *_NO_ROWS * 6, 0, 0, 0, 0), dev.index)
+            *_delta_inputs(p, q, k, v, g, beta, (out.data_ptr(), *p.to[2]), first, lengths), _ptr(state),
+            final.data_ptr(), *at, _ptr(scratch), *_NO_ROWS * 6, 0, 0, 0, 0), p.device)
         if keep:
             ctx.save_for_backward(q, k, v, g, beta, first, lengths, kept)
-            ctx.rest = scale, dtype
+            ctx.plan = p
             ctx.set_materialize_grads(False)
         return out, final
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dfinal):
-        q, k, v, g, beta, first, lengths, kept = ctx.saved_tensors
-        scale, dtype = ctx.rest
-        E, T, H, Dv = v.shape
-        Hk, Dk, dev = q.shape[2], q.shape[3], v.device
-        ns, nw, _, work = _delta_sizes(E, T, Hk, H, Dk, Dv, dtype)
+        q, k, v, g, beta, first, *rest = ctx.saved_tensors
+        lengths, kept = _dense(*rest)
+        p = ctx.plan
+        if _strides(q, k, v, g, beta, first) != p.strides:     # a saved tensor that came back in another order
+            q, k, v = _vectors(q), _vectors(k), _vectors(v)
+            p = _plan_again(_delta_plan, p.key, q, k, v, g, beta, None, first, lengths)
+        E, T, Hk, H, Dk, Dv = p.head[:6]
+        dev = v.device
+        ns, nw, _, work = p.sizes
         dout = torch.zeros_like(v, memory_format=torch.contiguous_format) if dout is None else _vectors(dout)
         dfinal = None if dfinal is None else dfinal.contiguous()
-        dq, dk, dv = _empty_like(q), _empty_like(k), _empty_like(v)
+        dq, dk, dv = _new(q, p.like[0]), _new(k, p.like[1]), _new(v, p.like[2])
         dg = torch.empty(g.shape, dtype=g.dtype, device=dev)
         db = torch.empty(beta.shape, dtype=beta.dtype, device=dev)
         dstate = torch.empty((E, H, Dk, Dv), dtype=torch.float32, device=dev) if ctx.needs_input_grad[5] else None
         scratch = torch.empty(4 * (ns + nw) + work, dtype=torch.uint8, device=dev)
-        p, s = kept.data_ptr(), scratch.data_ptr()
+        at, s, to = kept.data_ptr(), scratch.data_ptr(), p.to
         _call("bsg_delta_backward", _pack_delta(
-            *_delta_inputs(dtype, scale, q, k, v, g, beta, _NO_ROWS, first, lengths), 0, 0, p, p + 4 * ns,
-            s + 4 * (ns + nw), *_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv), *_rows(dg), *_rows(db), _ptr(dfinal),
-            _ptr(dstate), s, s + 4 * ns), dev.index)
-        return dq, dk, dv, dg, db, dstate, None, None, None, None, None
+            *_delta_inputs(p, q, k, v, g, beta, _NO_ROWS, first, lengths), 0, 0, at, at + 4 * ns, s + 4 * (ns + nw),
+            *_rows(dout), dq.data_ptr(), *to[0], dk.data_ptr(), *to[1], dv.data_ptr(), *to[2], dg.data_ptr(), *to[3],
+            db.data_ptr(), *to[3], _ptr(dfinal), _ptr(dstate), s, s + 4 * ns), p.device)
+        return dq, dk, dv, dg, db, dstate, None, None, None, None
 
 
 def gated_delta_rule(q, k, v, g, beta, state=None, first=None, lengths=None, *, scale=None):
@@ -319,21 +366,17 @@ def gated_delta_rule(q, k, v, g, beta, state=None, first=None, lengths=None, *, 
 
     Returns ``out`` [E, T, Hv, Dv] and the state after the last step, fp32.  Differentiable once in
     q, k, v, g, beta and state."""
-    who = "gated_delta_rule"
-    dtype = _heads(who, q, k, v, 4, Dk=q.shape[-1], Dv=v.shape[-1])
-    E, T, H, Dv = v.shape
-    _delta_check(who, q, k, v, g, beta, state, first, (E, T))
     if lengths is not None:
-        _shape(who, "lengths", lengths, (E,), _INT32)
         lengths = lengths.contiguous()
-    _tensors(who, q, k=k, v=v, g=g, beta=beta, state=state, first=first, lengths=lengths)
-    scale = _numbers(who, scale, q.shape[-1])
+    p = _delta_plan(_layout(q), _layout(k), _layout(v), _layout(g), _layout(beta), _layout(state), _layout(first),
+                    _layout(lengths), None if scale is None else float(scale))
+    E, T, Hk, H, Dk, Dv = p.head[:6]
     if E == 0 or T == 0:
-        zero = torch.zeros((E, H, q.shape[-1], Dv), dtype=torch.float32, device=v.device)
+        zero = torch.zeros((E, H, Dk, Dv), dtype=torch.float32, device=v.device)
         return v.clone(), zero if state is None else zero + state
     keep = torch.is_grad_enabled() and any(
         x is not None and x.requires_grad for x in (q, k, v, g, beta, state))
-    return _DeltaRule.apply(q, k, v, g, beta, state, first, lengths, scale, dtype, keep)
+    return _DeltaRule.apply(q, k, v, g, beta, state, first, lengths, p, keep)
 
 
 def gated_delta_step(q, k, v, g, beta, state, first=None, *, scale=None, out=None):
@@ -391,12 +434,11 @@ def _delta_step_plan(q, k, v, g, beta, state, first, out, scale):
 _pack_attention, _pack_attention_act = nat.packer(nat.BsgAttention), nat.packer(nat.BsgAttentionAct)
 
 
-def _attention_block(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, rest, out, grads=_NO_ROWS * 4, delta=0, parts=0):
-    E, T, H, D = q.shape
-    scale, softcap, window = numbers
-    return _pack_attention(E, T, H, k.shape[2], D, dtype, window, scale, softcap, 0, *_rows(q), *_rows(k), *_rows(v),
-                           *_rows(out), _ptr(slopes), *_flag_rows(first), _ptr(lengths), _ptr(begins), _ptr(lse),
-                           _ptr(rest), *grads, delta, parts)
+def _attention_block(p, q, k, v, slopes, first, lengths, begins, lse, rest, out, out_rows, grads=_NO_ROWS * 4, delta=0, parts=0):
+    r = p.rows
+    return _pack_attention(*p.head, q.data_ptr(), *r[0], k.data_ptr(), *r[1], v.data_ptr(), *r[2], out.data_ptr(), *out_rows,
+                           _ptr(slopes), _ptr(first), *p.first, _ptr(lengths), _ptr(begins), _ptr(lse), _ptr(rest), *grads,
+                           delta, parts)
 
 
 @lru_cache(maxsize=256)
@@ -419,41 +461,74 @@ def _attention_step_work(E, S, H, Hk, D, dtype):
     return n
 
 
+@lru_cache(maxsize=256)
+def _attention_plan(q, k, v, first, lengths, slopes, scale, softcap, window):
+    who = "episode_attention"
+    named = dict(q=q, k=k, v=v, first=first, lengths=lengths, slopes=slopes)
+    q, k, v, first, lengths, slopes = (None if x is None else _Layout(*x) for x in named.values())
+    dtype = _heads(who, q, k, v, 4, D=q.shape[-1])
+    E, T, H, D = q.shape
+    Hk = k.shape[2]
+    _shape(who, "k", k, (E, T, Hk, D))
+    _shape(who, "v", v, (E, T, Hk, D))
+    if Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"{who}: {H} query heads do not share {Hk} key heads evenly")
+    if first is not None:
+        _shape(who, "first", first, (E, T), _FLAGS)
+    if lengths is not None:
+        _shape(who, "lengths", lengths, (E,), _INT32)
+    if slopes is not None:
+        _shape(who, "slopes", slopes, (H,), _FP32)
+    device = _layouts(who, **named)
+    like, to = zip(*(_new_strides(x) for x in (q, k, v)))
+    return _Plan((E, T, H, Hk, D, dtype, min(window, T), _numbers(who, scale, D, softcap, window), softcap, 0), device,
+                 tuple([None if x is None else x.strides for x in (q, k, v, first)]),
+                 all(_vector_strides(x.shape, x.strides, x.dtype.itemsize) for x in (q, k, v)),
+                 [_row_strides(x.shape, x.strides) for x in (q, k, v)], like, to, (0, 0) if first is None else first.strides,
+                 (_attention_parts(E, T, H, Hk, D, dtype) if E and T else 0,), (scale, softcap, window))
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, first, lengths, slopes, numbers, dtype, keep):
-        q, k, v = _vectors(q), _vectors(k), _vectors(v)
-        E, T, H, D = q.shape
+    def forward(ctx, q, k, v, first, lengths, slopes, p, keep):
+        if not p.vectors or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+            q, k, v = _vectors(q), _vectors(k), _vectors(v)
+            p = _plan_again(_attention_plan, p.key, q, k, v, first, lengths, slopes)
+        E, T, H, Hk, D, dtype, window = p.head[:7]
         dev = q.device
-        out = _empty_like(q)
+        out = _new(q, p.like[0])
         begins = lse = rest = None
-        if first is not None or numbers[2] > 0:
+        if first is not None or window > 0:
             begins = torch.empty((E, T), dtype=torch.int32, device=dev)
         if keep:
             lse = torch.empty((E, H, T), dtype=torch.float32, device=dev)
             if dtype == nat.BF16 and T > nat.ATTENTION_TILE:
                 rest = torch.empty((E, H, T, D), dtype=q.dtype, device=dev)
         _call("bsg_attention_forward",
-              _attention_block(dtype, numbers, q, k, v, slopes, first, lengths, begins, lse, rest, out), dev.index)
+              _attention_block(p, q, k, v, slopes, first, lengths, begins, lse, rest, out, p.to[0]), p.device)
         if keep:
             ctx.save_for_backward(q, k, v, slopes, first, lengths, begins, lse, rest, out)   # as _attention_block takes them
-            ctx.rest = numbers, dtype
+            ctx.plan = p
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        *saved, out = ctx.saved_tensors
-        q, k, v, lse = saved[0], saved[1], saved[2], saved[7]
-        numbers, dtype = ctx.rest
-        dout = _vectors(dout)
-        dq, dk, dv, delta = _empty_like(q), _empty_like(k), _empty_like(v), torch.empty_like(lse)
-        need = _attention_parts(*q.shape[:3], k.shape[2], q.shape[3], dtype)
+        q, k, v, slopes, first, *more, out = ctx.saved_tensors
+        slopes, lengths, begins, lse, rest = _dense(slopes, *more)
+        p = ctx.plan
+        if _strides(q, k, v, first) != p.strides:      # a saved tensor that came back in another order
+            q, k, v = _vectors(q), _vectors(k), _vectors(v)
+            p = _plan_again(_attention_plan, p.key, q, k, v, first, lengths, slopes)
+        dout, out = _vectors(dout), _vectors(out)
+        dq, dk, dv, delta = _new(q, p.like[0]), _new(k, p.like[1]), _new(v, p.like[2]), torch.empty_like(lse)
+        need, to = p.sizes[0], p.to
         parts = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         _call("bsg_attention_backward", _attention_block(
-            dtype, numbers, *saved, out, (*_rows(dout), *_rows(dq), *_rows(dk), *_rows(dv)), delta.data_ptr(), _ptr(parts)),
-            q.device.index)
-        return dq, dk, dv, None, None, None, None, None, None
+            p, q, k, v, slopes, first, lengths, begins, lse, rest, out, _row_strides(out.shape, out.stride()),
+            (*_rows(dout), dq.data_ptr(), *to[0], dk.data_ptr(), *to[1], dv.data_ptr(), *to[2]), delta.data_ptr(),
+            _ptr(parts)), p.device)
+        return dq, dk, dv, None, None, None, None, None
 
 
 def episode_attention(q, k, v, first=None, lengths=None, *, scale=None, softcap=0.0, slopes=None, window=0):
@@ -467,25 +542,15 @@ def episode_attention(q, k, v, first=None, lengths=None, *, scale=None, softcap=
     the number of last steps that are seen (0 = all of the episode).  scale: D ** -0.5 by default.
     Returns out [E, T, Hq, D].  Differentiable once in q, k and v."""
     who = "episode_attention"
-    dtype = _heads(who, q, k, v, 4, D=q.shape[-1])
-    E, T, H, D = q.shape
-    Hk = k.shape[2]
-    _shape(who, "k", k, (E, T, Hk, D))
-    _shape(who, "v", v, (E, T, Hk, D))
-    if Hk < 1 or H < 1 or H % Hk:
-        raise ValueError(f"{who}: {H} query heads do not share {Hk} key heads evenly")
-    if first is not None:
-        _shape(who, "first", first, (E, T), _FLAGS)
     if lengths is not None:
-        _shape(who, "lengths", lengths, (E,), _INT32)
         lengths = lengths.contiguous()
-    _tensors(who, q, k=k, v=v, first=first, lengths=lengths, slopes=slopes)
-    scale = _numbers(who, scale, D, softcap, window)
-    slopes = _slopes(who, slopes, H)
-    if E == 0 or T == 0:
+    p = _attention_plan(_layout(q), _layout(k), _layout(v), _layout(first), _layout(lengths), _layout(slopes),
+                        None if scale is None else float(scale), float(softcap), int(window))
+    slopes = _slopes(who, slopes, p.head[2])
+    if q.numel() == 0:
         return q.clone()
     keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    return _Attention.apply(q, k, v, first, lengths, slopes, (scale, float(softcap), min(int(window), T)), dtype, keep)
+    return _Attention.apply(q, k, v, first, lengths, slopes, p, keep)
 
 
 def episode_attention_step(q, k, v, k_cache, v_cache, steps, first=None, *, scale=None, softcap=0.0,

@@ -746,3 +746,19 @@ def test_acting_calls_look_at_every_address_and_number(dt):
         delta(q, k, v, state=shift(S))
     with pytest.raises(ValueError):
         attend(q, k, v, kc=shift(caches[0]))
+
+
+def test_saved_tensors_in_another_order():
+    """A hook on saved tensors may give them back with other strides: the gradients stay the same."""
+    x, dout, g = attention_data(2, 70, 2, 1, 64, torch.bfloat16, 5)
+    d, ddout, state, g = delta_data(2, 70, 1, 2, 64, 64, torch.float32, 6)
+    first = flags(2, 70, "0.05", g).to(DEV)
+    turn = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1) if t.dim() in (2, 3, 4) and t.shape[1] == 70 else t  # noqa: E731
+    dev = lambda y: {n: t.to(DEV).requires_grad_(True) for n, t in y.items()}  # noqa: E731
+    for call, y, go in ((lambda y: memory.episode_attention(**y, first=first, window=40), x, dout),
+                        (lambda y: memory.gated_delta_rule(**y, state=state.to(DEV), first=first)[0], d, ddout)):
+        y = dev(y)
+        want = torch.autograd.grad(call(y), list(y.values()), go.to(DEV))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, turn):
+            out = call(y)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, list(y.values()), go.to(DEV)), want))
