@@ -24,9 +24,10 @@ steps behind it are padding, never read, and their outputs and gradients are zer
 value may reach every output of its env's rollout, but no other env's.
 
 Work is enqueued on the current stream of the tensors' device; all calls can be captured into a
-HIP graph.  ``first`` and ``lengths`` are read again by the backward pass: they may not change
-in between.  Sums have a fixed order, so results repeat bit for bit.  ``out=`` tensors may not overlap
-inputs.  No CPU fallback.
+HIP graph (a backward pass, as any in torch, once no eager graph of the same leaves is alive:
+their gradients would be accumulated on that graph's stream).  ``first`` and ``lengths`` are read
+again by the backward pass: they may not change in between.  Sums have a fixed order, so results
+repeat bit for bit.  ``out=`` tensors may not overlap inputs.  No CPU fallback.
 """
 from __future__ import annotations
 
