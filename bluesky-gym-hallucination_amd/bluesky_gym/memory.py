@@ -129,12 +129,17 @@ def _rows(x):
 
 
 def _new_strides(x):
-    """The strides of a tensor made like one of this layout (in its order of axes, as torch.empty_like
-    would, where rows can be written so, else contiguous), and a bsg_rows' of them."""
-    y = torch.empty_like(torch.empty_strided(x.shape, x.strides, dtype=x.dtype, device="meta"))
-    if not _vector_strides(y.shape, y.stride(), y.element_size()):
-        y = torch.empty(x.shape, device="meta")
-    return y.stride(), _row_strides(y.shape, y.stride())
+    """The strides of a tensor made like one of this layout (the same where it is dense and its rows
+    can be written, else contiguous), and a bsg_rows' of them."""
+    size, strides = 1, x.strides
+    for y, n in sorted((y, n) for y, n in zip(strides, x.shape) if n > 1):
+        if y != size:                      # a gap or an overlap
+            break
+        size *= n
+    if size != x.shape.numel() or not _vector_strides(x.shape, strides, x.dtype.itemsize):
+        _, T, H, D = x.shape
+        strides = (T * H * D, H * D, D, 1)
+    return strides, _row_strides(x.shape, strides)
 
 
 def _new(x, strides):
