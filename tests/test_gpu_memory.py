@@ -13,7 +13,8 @@ fp32 2^-24; e = 2^-24 for what is held in fp32):
    derivative (its error is at most twice the score's): |ds err| <= (2 u + 3 r + (D + 16) e) B, and dq,
    dk are sums of it.  A p under 2^-126 is 0 in fp32: at most 2^9 such terms in a sum, each with
    factors |dp| + |delta| <= 2^10 and |k|, |q| <= 2^6, so 2^-100 in all (UNDER).
- - delta rule: fp32 chains of sums; a value passes at most 8 products, each a sum of up to 192 terms
+ - delta rule: fp32 chains of sums; a value passes at most 8 products (that of a boundary of
+   segments among them), each a sum of up to 192 terms
    (a chunk's 64 and dim_k), so 8 * 192 e of the path's magnitude, taken as the largest
    entry of the output for that env and head, plus the growth along the rollout bounded by
    the same (unit keys, beta < 1: S does not grow).  With bf16 operands the values split into two

@@ -157,6 +157,17 @@ def test_delta_work_is_wanted_where_rows_are_few():
         assert getattr(lib, fn)(C.byref(delta_args(steps=65, work=P + 4)), None) == INVALID
 
 
+def test_delta_work_holds_the_segments_of_long_rollouts():
+    """From nine chunks on, few rows: a transition [dim_k][dim_k + dim_v] of fp32 per row and boundary."""
+    lib = nat.load_library()
+    need = lambda back=0, **kw: lib.bsg_delta_work_bytes(C.byref(delta_args(**kw)), back)  # noqa: E731
+    chunk = need(steps=128) // 4                                       # two rows of two chunks
+    for back in (0, 1):
+        assert need(back, steps=512) == 2 * 8 * chunk
+        assert need(back, steps=513) == 2 * 9 * chunk + 2 * 2 * 64 * 128 * 4
+        assert need(back, steps=64 * 64, num_envs=255) == 255 * 64 * chunk      # rows for every CU: one segment
+
+
 def test_parts_are_wanted_where_key_tiles_are_few():
     """By query head where shared key heads leave CUs idle, from bsg_attention_parts_bytes alone."""
     lib = nat.load_library()
