@@ -763,3 +763,39 @@ def test_saved_tensors_in_another_order():
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t, turn):
             out = call(y)
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, list(y.values()), go.to(DEV)), want))
+
+
+def test_segments_replay_with_lengths_that_end_at_their_boundaries():
+    """A long rollout's learning call captured once and replayed for other lengths, two graphs in turn."""
+    E, T = 3, 700
+    d, dout, state, g = delta_data(E, T, 1, 2, 64, 64, torch.bfloat16, 91)
+    first = flags(E, T, "0.003", g).to(DEV)
+    lengths = torch.full((E,), T, dtype=torch.int32, device=DEV)
+    x, dout, state = {n: v.to(DEV).requires_grad_(True) for n, v in d.items()}, dout.to(DEV), state.to(DEV).requires_grad_(True)
+
+    def learner():
+        o, fin = memory.gated_delta_rule(**x, state=state, first=first, lengths=lengths)
+        return [o.detach(), fin.detach(), *torch.autograd.grad([o, fin], [*x.values(), state], [dout, state.detach()])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        learner()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    captured = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            captured.append(learner())
+    for n in ((T, 0, 1), (256, 257, 255), (512, 640, 699), (64, 192, 384)):
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        want = learner()
+        torch.cuda.synchronize()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for got in captured:
+            assert all(torch.equal(a, w) for a, w in zip(got, want))
+        for e in range(E):
+            assert not want[0][e, n[e]:].any() and (n[e] > 0 or torch.equal(want[1][e], state[e]))
